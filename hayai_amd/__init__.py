@@ -9,6 +9,7 @@ operation runs on the GPU or raises.
 from .engine import (  # noqa: F401
     ACT_GELU_TANH,
     ACT_SILU,
+    BF16,
     BUF_DEVICE,
     BUF_PINNED_HOST,
     F16,
@@ -19,6 +20,7 @@ from .engine import (  # noqa: F401
     Q4_K,
     Q6_K,
     Q8_0,
+    BorrowedBuffer,
     DeviceBuffer,
     HipEngine,
     HipError,

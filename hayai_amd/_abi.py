@@ -127,6 +127,62 @@ class MoeDesc(C.Structure):
     ]
 
 
+class QuantI8Desc(C.Structure):
+    _fields_ = [
+        ("type", C.c_int),
+        ("act", C.c_int),
+        ("rows", C.c_size_t),
+        ("cols", C.c_size_t),
+        ("x_stride", C.c_size_t),
+        ("up_stride", C.c_size_t),
+        ("q_stride", C.c_size_t),
+    ]
+
+
+class RmsNormI8Desc(C.Structure):
+    _fields_ = [
+        ("type", C.c_int),
+        ("eps", C.c_float),
+        ("rows", C.c_size_t),
+        ("cols", C.c_size_t),
+        ("x_stride", C.c_size_t),
+        ("res_stride", C.c_size_t),
+        ("sum_stride", C.c_size_t),
+        ("q_stride", C.c_size_t),
+    ]
+
+
+class GemmI8Desc(C.Structure):
+    _fields_ = [
+        ("type", C.c_int),
+        ("m", C.c_size_t),
+        ("n", C.c_size_t),
+        ("tokens", C.c_size_t),
+        ("w_stride", C.c_size_t),
+        ("x_stride", C.c_size_t),
+        ("res_stride", C.c_size_t),
+        ("y_stride", C.c_size_t),
+    ]
+
+
+class SampleParams(C.Structure):
+    _fields_ = [
+        ("temperature", C.c_float),
+        ("top_k", C.c_int32),
+        ("top_p", C.c_float),
+        ("min_p", C.c_float),
+    ]
+
+
+class SampleDesc(C.Structure):
+    _fields_ = [
+        ("type", C.c_int),
+        ("rows", C.c_size_t),
+        ("vocab", C.c_size_t),
+        ("stride", C.c_size_t),
+    ]
+
+
 SIGNATURES = {
     "hh_gguf_open": (ST, [C.c_char_p, PP]),
     "hh_gguf_close": (None, [P]),
@@ -154,6 +210,7 @@ SIGNATURES = {
     "hh_engine_sync": (ST, [P]),
     "hh_engine_ffn_calls": (C.c_uint64, [P]),
     "hh_buf_alloc": (ST, [P, SZ, I, PP]),
+    "hh_buf_wrap": (ST, [P, P, SZ, PP]),
     "hh_buf_free": (None, [P]),
     "hh_buf_size": (SZ, [P]),
     "hh_buf_kind": (C.c_int, [P]),
@@ -189,6 +246,10 @@ SIGNATURES = {
     "hh_route_experts": (ST, [P, C.POINTER(MoeDesc), P, P, SZ, P, P]),
     "hh_moe_ffn_dev": (ST, [P, C.POINTER(MoeDesc), P, SZ, P, SZ, SZ, P, SZ, P, SZ, P, SZ]),
     "hh_moe_dev": (ST, [P, C.POINTER(MoeDesc), P, SZ, P, SZ, P, SZ, P, SZ, SZ, P, SZ]),
+    "hh_quant_i8_dev": (ST, [P, C.POINTER(QuantI8Desc)] + [P, SZ] * 5),
+    "hh_rms_norm_i8_dev": (ST, [P, C.POINTER(RmsNormI8Desc)] + [P, SZ] * 7),
+    "hh_gemm_i8_dev": (ST, [P, C.POINTER(GemmI8Desc)] + [P, SZ] * 6),
+    "hh_sample_dev": (ST, [P, C.POINTER(SampleDesc)] + [P, SZ] * 5),
     "hh_streamer_create": (ST, [P, SZ, SZ, SZ, PP]),
     "hh_streamer_destroy": (None, [P]),
     "hh_streamer_slot_for": (ST, [P, SZ, C.POINTER(SZ)]),

@@ -15,6 +15,7 @@
 #define HH_TYPE_Q6_K 14
 #define HH_TYPE_IQ2_XXS 16
 #define HH_TYPE_IQ3_XXS 18
+#define HH_TYPE_BF16 30
 
 #define HH_ACT_SILU 0
 #define HH_ACT_GELU_TANH 1
@@ -82,6 +83,47 @@ struct hh_dequant_args {
     const uint8_t* w;
     float* out;
     uint64_t n;
+};
+
+// Rows into int8 codes (i8_rows.hip).  b: up, or the residual (null: none); strides in elements.
+struct hh_i8_rows_args {
+    const void* x;
+    const void* b;
+    const float* norm;
+    void* sum;
+    int8_t* q;
+    float* scale;
+    float* values;
+    uint64_t x_stride, b_stride, sum_stride, q_stride;
+    uint32_t cols;
+    int32_t act;
+    float eps;
+    uint32_t pad;
+};
+
+// y[t][r] = sum_k x[t][k] w[r][k] * xs[t] * ws[r] (+ res[t][r]) over codes (i8_gemm.hip);
+// w and x strides in bytes, y and res strides in elements.
+struct hh_i8_gemm_args {
+    const int8_t* w;
+    const int8_t* x;
+    const float* ws;
+    const float* xs;
+    const void* res;
+    void* y;
+    uint64_t w_stride, x_stride, res_stride, y_stride;
+    uint32_t m, n, t, pad;
+};
+
+// The next token of each row of logits (sample.hip); stride in elements.
+struct hh_sample_args {
+    const void* x;
+    const void* params;  // hh_sample_params
+    const float* u;
+    int32_t* ids;
+    float* probs;
+    uint64_t stride;
+    uint32_t vocab;
+    uint32_t pad;
 };
 
 // Synthetic GGUF bytes: splitmix64 stream, then f16 scale fields drawn U(lo, hi).

@@ -148,12 +148,40 @@ hh_status hh_buf_alloc(hh_engine* e, size_t bytes, int kind, hh_buf** out) {
     return HH_OK;
 }
 
+hh_status hh_buf_wrap(hh_engine* e, void* ptr, size_t bytes, hh_buf** out) {
+    HH_NOT_NULL(e, "engine");
+    HH_NOT_NULL(out, "out");
+    *out = nullptr;
+    HH_NOT_NULL(ptr, "ptr");
+    HH_TRY(e->no_capture("buf_wrap"));
+    HH_TRY(e->select());
+    hipPointerAttribute_t at{};
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    if (hipPointerGetAttributes(&at, ptr) != hipSuccess || at.type != hipMemoryTypeDevice || at.device != e->device ||
+        hipMemGetAddressRange(&base, &size, ptr) != hipSuccess) {
+        (void)hipGetLastError();  // not a fault of the next call
+        return fail(HH_ERR_INVALID, "hh_buf_wrap: not device memory of GPU %d", e->device);
+    }
+    const size_t at_off = (size_t)((char*)ptr - (char*)base);
+    if (at_off > size || bytes > size - at_off)
+        return fail(HH_ERR_INVALID, "hh_buf_wrap: %zu bytes reach past the allocation's end", bytes);
+    hh_buf* b = new (std::nothrow) hh_buf{e, ptr, bytes, HH_BUF_DEVICE, true};
+    if (!b) return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
+    *out = b;
+    return HH_OK;
+}
+
 void hh_buf_free(hh_buf* b) {
     if (!b) return;
     (void)hipSetDevice(b->engine->device);
     // Work queued on the engine may still read the buffer.
     (void)hipStreamSynchronize(b->engine->stream);
     (void)hipStreamSynchronize(b->engine->copy_stream);
+    if (b->borrowed) {
+        delete b;
+        return;
+    }
     if (b->kind == HH_BUF_DEVICE)
         (void)hipFree(b->ptr);
     else
@@ -709,6 +737,201 @@ hh_status hh_gateup_dev(hh_engine* e, int tg, int tu, size_t d_ff, size_t d_mode
     e->ffn_calls += 2;
     return e->enqueue_gateup(tg, tu, d_ff, d_model, (const uint8_t*)wg->ptr + wg_off, (const uint8_t*)wu->ptr + wu_off,
                              (const float*)((const char*)x->ptr + x_off), (float*)((char*)h->ptr + h_off), act);
+}
+
+// ---------------------------------------------------------------- 8-bit path ---------
+
+static hh_status check_act_type(int type, const char* what) {
+    if (!act_type(type)) return fail(HH_ERR_KERNEL_MISSING, "%s: no kernel for activations of GGML type %d", what, type);
+    return HH_OK;
+}
+
+// A matrix of `rows` rows of `cols` elements of `elem` bytes, *stride elements apart (0: packed,
+// filled in), in a device-visible buffer of the engine; whole: the last row has its whole stride too.
+static hh_status check_rows(hh_engine* e, const hh_buf* b, size_t off, size_t rows, size_t cols, size_t elem,
+                            size_t* stride, const char* what, bool whole = false) {
+    HH_TRY(check_engine(e, b, what));
+    if (*stride == 0) *stride = cols;
+    if (*stride < cols) return fail(HH_ERR_INVALID, "%s: stride %zu < %zu columns", what, *stride, cols);
+    if (*stride > SIZE_MAX / elem / (rows ? rows : 1)) return fail(HH_ERR_INVALID, "%s: size overflow", what);
+    const size_t bytes = rows ? ((rows - 1) * *stride + (whole ? *stride : cols)) * elem : 0;
+    HH_TRY(check_range(b, off, bytes, what));
+    if (((uintptr_t)b->ptr + off) % elem) return fail(HH_ERR_INVALID, "%s: offset %zu splits an element", what, off);
+    return HH_OK;
+}
+
+static hh_status check_vector(hh_engine* e, const hh_buf* b, size_t off, size_t n, const char* what) {
+    size_t stride = 0;
+    return check_rows(e, b, off, 1, n, 4, &stride, what);
+}
+
+// Grids and row indexes are 32 bits; columns are addressed in 32 bits with room for a vector past the end.
+static hh_status check_sizes(size_t rows, size_t cols, const char* what) {
+    if (cols == 0) return fail(HH_ERR_INVALID, "%s: rows of no columns", what);
+    if (rows > INT32_MAX || cols > INT32_MAX)
+        return fail(HH_ERR_INVALID, "%s: %zu x %zu exceeds 31-bit sizes", what, rows, cols);
+    return HH_OK;
+}
+
+static void* at(const hh_buf* b, size_t off) { return b ? (char*)b->ptr + off : nullptr; }
+
+hh_status hh_quant_i8_dev(hh_engine* e, const hh_quant_i8_desc* d, const hh_buf* x, size_t x_off, const hh_buf* up,
+                          size_t up_off, hh_buf* q, size_t q_off, hh_buf* scale, size_t scale_off, hh_buf* values,
+                          size_t values_off) {
+    HH_NOT_NULL(e, "engine");
+    HH_NOT_NULL(d, "quant_i8 desc");
+    HH_TRY(check_act_type(d->type, "quant_i8"));
+    HH_TRY(check_sizes(d->rows, d->cols, "quant_i8"));
+    if (up && d->act != HH_ACT_SILU && d->act != HH_ACT_GELU_TANH)
+        return fail(HH_ERR_INVALID, "quant_i8: unknown act %d", d->act);
+    const size_t el = act_type(d->type)->bytes;
+    size_t xs = d->x_stride, us = d->up_stride, qs = d->q_stride, vs = 0;
+    HH_TRY(check_rows(e, x, x_off, d->rows, d->cols, el, &xs, "quant_i8 x"));
+    if (up) HH_TRY(check_rows(e, up, up_off, d->rows, d->cols, el, &us, "quant_i8 up"));
+    HH_TRY(check_rows(e, q, q_off, d->rows, d->cols, 1, &qs, "quant_i8 q"));
+    HH_TRY(check_vector(e, scale, scale_off, d->rows, "quant_i8 scale"));
+    if (values) HH_TRY(check_rows(e, values, values_off, d->rows, d->cols, 4, &vs, "quant_i8 values"));
+    if (d->rows == 0) return HH_OK;
+    HH_TRY(e->select());
+    hh_i8_rows_args a{};
+    a.x = at(x, x_off);
+    a.b = at(up, up_off);
+    a.q = (int8_t*)at(q, q_off);
+    a.scale = (float*)at(scale, scale_off);
+    a.values = (float*)at(values, values_off);
+    a.x_stride = xs;
+    a.b_stride = us;
+    a.q_stride = qs;
+    a.cols = (uint32_t)d->cols;
+    a.act = d->act;
+    try {
+        return e->enqueue_i8_rows(d->type, d->rows, a);
+    } catch (const std::bad_alloc&) {
+        return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
+}
+
+hh_status hh_rms_norm_i8_dev(hh_engine* e, const hh_rms_norm_i8_desc* d, const hh_buf* x, size_t x_off,
+                             const hh_buf* res, size_t res_off, const hh_buf* norm, size_t norm_off, hh_buf* sum,
+                             size_t sum_off, hh_buf* q, size_t q_off, hh_buf* scale, size_t scale_off, hh_buf* values,
+                             size_t values_off) {
+    HH_NOT_NULL(e, "engine");
+    HH_NOT_NULL(d, "rms_norm_i8 desc");
+    HH_TRY(check_act_type(d->type, "rms_norm_i8"));
+    HH_TRY(check_sizes(d->rows, d->cols, "rms_norm_i8"));
+    if (!(d->eps >= 0.f) || d->eps > 1.f)
+        return fail(HH_ERR_INVALID, "rms_norm_i8: eps=%g outside [0, 1]", (double)d->eps);
+    if (!res != !sum) return fail(HH_ERR_INVALID, "rms_norm_i8: res and sum come together");
+    const size_t el = act_type(d->type)->bytes;
+    size_t xs = d->x_stride, rs = d->res_stride, ss = d->sum_stride, qs = d->q_stride, vs = 0;
+    HH_TRY(check_rows(e, x, x_off, d->rows, d->cols, el, &xs, "rms_norm_i8 x"));
+    if (res) {
+        HH_TRY(check_rows(e, res, res_off, d->rows, d->cols, el, &rs, "rms_norm_i8 res"));
+        HH_TRY(check_rows(e, sum, sum_off, d->rows, d->cols, el, &ss, "rms_norm_i8 sum"));
+    }
+    HH_TRY(check_vector(e, norm, norm_off, d->cols, "rms_norm_i8 norm"));
+    HH_TRY(check_rows(e, q, q_off, d->rows, d->cols, 1, &qs, "rms_norm_i8 q"));
+    HH_TRY(check_vector(e, scale, scale_off, d->rows, "rms_norm_i8 scale"));
+    if (values) HH_TRY(check_rows(e, values, values_off, d->rows, d->cols, 4, &vs, "rms_norm_i8 values"));
+    if (d->rows == 0) return HH_OK;
+    HH_TRY(e->select());
+    hh_i8_rows_args a{};
+    a.x = at(x, x_off);
+    a.b = at(res, res_off);
+    a.norm = (const float*)at(norm, norm_off);
+    a.sum = at(sum, sum_off);
+    a.q = (int8_t*)at(q, q_off);
+    a.scale = (float*)at(scale, scale_off);
+    a.values = (float*)at(values, values_off);
+    a.x_stride = xs;
+    a.b_stride = rs;
+    a.sum_stride = ss;
+    a.q_stride = qs;
+    a.cols = (uint32_t)d->cols;
+    a.eps = d->eps;
+    try {
+        return e->enqueue_i8_rows(d->type, d->rows, a);
+    } catch (const std::bad_alloc&) {
+        return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
+}
+
+hh_status hh_gemm_i8_dev(hh_engine* e, const hh_gemm_i8_desc* d, const hh_buf* w, size_t w_off, const hh_buf* w_scale,
+                         size_t w_scale_off, const hh_buf* x, size_t x_off, const hh_buf* x_scale, size_t x_scale_off,
+                         const hh_buf* res, size_t res_off, hh_buf* y, size_t y_off) {
+    HH_NOT_NULL(e, "engine");
+    HH_NOT_NULL(d, "gemm_i8 desc");
+    HH_TRY(check_act_type(d->type, "gemm_i8"));
+    HH_TRY(check_sizes(d->m, d->n, "gemm_i8"));
+    if (d->m == 0) return fail(HH_ERR_INVALID, "gemm_i8: empty shape m=0 n=%zu", d->n);
+    if (d->n > HH_I8_MAX_N)
+        return fail(HH_ERR_INVALID, "gemm_i8: n=%zu > %u, sums could pass 32 bits", d->n, HH_I8_MAX_N);
+    HH_TRY(check_sizes(d->tokens, d->m, "gemm_i8"));
+    const size_t el = act_type(d->type)->bytes;
+    size_t ws = d->w_stride, xs = d->x_stride, rs = d->res_stride, ys = d->y_stride;
+    HH_TRY(check_rows(e, w, w_off, d->m, d->n, 1, &ws, "gemm_i8 w", true));
+    HH_TRY(check_vector(e, w_scale, w_scale_off, d->m, "gemm_i8 w_scale"));
+    HH_TRY(check_rows(e, x, x_off, d->tokens, d->n, 1, &xs, "gemm_i8 x", true));
+    HH_TRY(check_vector(e, x_scale, x_scale_off, d->tokens, "gemm_i8 x_scale"));
+    if (res) HH_TRY(check_rows(e, res, res_off, d->tokens, d->m, el, &rs, "gemm_i8 res"));
+    HH_TRY(check_rows(e, y, y_off, d->tokens, d->m, el, &ys, "gemm_i8 y"));
+    if ((((uintptr_t)w->ptr + w_off) | ((uintptr_t)x->ptr + x_off) | ws | xs) % 16)
+        return fail(HH_ERR_INVALID, "gemm_i8: rows of codes must start on 16-byte boundaries (strides %zu, %zu)", ws, xs);
+    if (d->tokens == 0) return HH_OK;
+    HH_TRY(e->select());
+    hh_i8_gemm_args a{};
+    a.w = (const int8_t*)at(w, w_off);
+    a.x = (const int8_t*)at(x, x_off);
+    a.ws = (const float*)at(w_scale, w_scale_off);
+    a.xs = (const float*)at(x_scale, x_scale_off);
+    a.res = at(res, res_off);
+    a.y = at(y, y_off);
+    a.w_stride = ws;
+    a.x_stride = xs;
+    a.res_stride = rs;
+    a.y_stride = ys;
+    a.m = (uint32_t)d->m;
+    a.n = (uint32_t)d->n;
+    a.t = (uint32_t)d->tokens;
+    try {
+        std::lock_guard<std::mutex> lk(e->ws_mutex);
+        return e->enqueue_i8_gemm(d->type, a);
+    } catch (const std::bad_alloc&) {
+        return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
+}
+
+hh_status hh_sample_dev(hh_engine* e, const hh_sample_desc* d, const hh_buf* logits, size_t logits_off,
+                        const hh_buf* params, size_t params_off, const hh_buf* u, size_t u_off, hh_buf* ids,
+                        size_t ids_off, hh_buf* probs, size_t probs_off) {
+    HH_NOT_NULL(e, "engine");
+    HH_NOT_NULL(d, "sample desc");
+    HH_TRY(check_act_type(d->type, "sample"));
+    HH_TRY(check_sizes(d->rows, d->vocab, "sample"));
+    if (d->vocab > HH_SAMPLE_MAX_VOCAB)
+        return fail(HH_ERR_INVALID, "sample: vocab=%zu > %u", d->vocab, HH_SAMPLE_MAX_VOCAB);
+    size_t stride = d->stride;
+    HH_TRY(check_rows(e, logits, logits_off, d->rows, d->vocab, act_type(d->type)->bytes, &stride, "sample logits"));
+    HH_TRY(check_vector(e, params, params_off, d->rows * 4, "sample params"));
+    HH_TRY(check_vector(e, u, u_off, d->rows, "sample u"));
+    HH_TRY(check_vector(e, ids, ids_off, d->rows, "sample ids"));
+    if (probs) HH_TRY(check_vector(e, probs, probs_off, d->rows, "sample probs"));
+    if (d->rows == 0) return HH_OK;
+    HH_TRY(e->select());
+    hh_sample_args a{};
+    a.x = at(logits, logits_off);
+    a.params = at(params, params_off);
+    a.u = (const float*)at(u, u_off);
+    a.ids = (int32_t*)at(ids, ids_off);
+    a.probs = (float*)at(probs, probs_off);
+    a.stride = stride;
+    a.vocab = (uint32_t)d->vocab;
+    try {
+        std::lock_guard<std::mutex> lk(e->ws_mutex);
+        return e->enqueue_sample(d->type, d->rows, a);
+    } catch (const std::bad_alloc&) {
+        return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
 }
 
 // ---------------------------------------------------------------- MoE ----------------

@@ -2100,6 +2100,7 @@ static std::vector<std::string> required_kernels() {
     k.push_back("hh_add_kernel");
     for (int t : {16, 32, 64})
         for (const char* kind : {"hh_moe_gateup_t", "hh_moe_down_t"}) k.push_back(std::string(kind) + std::to_string(t));
+    i8_kernels(k);
     return k;
 }
 

@@ -58,6 +58,15 @@ hh_status validate_weights(int ggml_type, size_t m, size_t n, size_t len);
 // f32 scale per 8 elements, + 16 bytes of slack for the kernels' vector tail).
 inline size_t ring_digits_bytes(size_t n) { return 2 * n + (n / 8) * 4 + 16; }
 
+// Element types of the 8-bit path's activations: kernel-name stem and bytes, or null.
+struct ActType {
+    const char* name;
+    size_t bytes;
+};
+const ActType* act_type(int ggml_type);
+// Names of the 8-bit path's kernels, for the check at engine creation.
+void i8_kernels(std::vector<std::string>& names);
+
 // The device address of noalloc.hip's fixed scratch array on `device` (which must be the
 // current device): looked up once per device and kept.
 hh_status noalloc_scratch(int device, void** out);
@@ -77,6 +86,7 @@ struct hh_buf {
     void* ptr;  // device pointer, or pinned host pointer (also device-accessible)
     size_t size;
     int kind;
+    bool borrowed = false;  // hh_buf_wrap: the memory is the caller's
 };
 
 struct hh_event {
@@ -328,6 +338,11 @@ struct hh_engine {
     hh_status enqueue_moe_shared(const hh_moe_desc* d, const uint8_t* experts, const float* x, size_t T, float* y);
     // Q4 LUT GEMV (hayai's 4-bit dictionary format): W m rows of n/2 bytes, lut 16 f32.
     hh_status enqueue_lut(size_t m, size_t n, const uint8_t* w, const float* lut, const float* x, float* y);
+    // The 8-bit path (i8.cpp); device pointers, strides resolved (elements for activations, bytes
+    // for codes).  b: up (norm null, act) or the residual (norm given); null: none.
+    hh_status enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_args& a);
+    hh_status enqueue_i8_gemm(int type, const hh_i8_gemm_args& a);
+    hh_status enqueue_sample(int type, size_t rows, const hh_sample_args& a);
     // Reports (and clears) a grid-barrier timeout recorded by a fused kernel.  Syncs.
     hh_status check_device_error();
 };

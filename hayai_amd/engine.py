@@ -24,6 +24,7 @@ import numpy as np
 from . import _abi
 
 F32, F16, Q4_0, Q8_0, Q4_K, Q6_K, IQ2_XXS, IQ3_XXS = 0, 1, 2, 8, 12, 14, 16, 18
+BF16 = 30  # activations of the 8-bit operators
 ACT_SILU, ACT_GELU_TANH = 0, 1
 BUF_DEVICE, BUF_PINNED_HOST = 0, 1
 TYPE_NAMES = {F32: "f32", F16: "f16", Q4_0: "q4_0", Q8_0: "q8_0", Q4_K: "q4_k", Q6_K: "q6_k", IQ2_XXS: "iq2_xxs",
@@ -45,6 +46,11 @@ def _check(st: int) -> None:
 
 def _ptr(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
+
+
+def _handle(b):
+    """The handle of an optional buffer."""
+    return None if b is None else b.handle
 
 
 def row_bytes(ggml_type: int, n: int) -> int:
@@ -113,6 +119,20 @@ class DeviceBuffer:
             self.free()
         except Exception:
             pass
+
+
+class BorrowedBuffer(DeviceBuffer):
+    """A handle on device memory that someone else owns (HipEngine.wrap)."""
+
+    def __init__(self, engine: "HipEngine", address: int, nbytes: int):
+        self.engine = engine
+        self.nbytes = int(nbytes)
+        self.kind = BUF_DEVICE
+        self.handle = None
+        h = C.c_void_p()
+        _check(engine.lib.hh_buf_wrap(engine.handle, address, self.nbytes, C.byref(h)))
+        self.handle = h
+        engine._children.add(self)
 
 
 class MirrorView:
@@ -366,6 +386,11 @@ class HipEngine:
         b = DeviceBuffer(self, data.nbytes)
         b.write(data)
         return b
+
+    def wrap(self, address: int, nbytes: int) -> BorrowedBuffer:
+        """A buffer over device memory of the caller's (a torch tensor's data_ptr(), say), which has
+        to outlive it; work on other streams is the caller's to order (hh_buf_wrap)."""
+        return BorrowedBuffer(self, address, nbytes)
 
     def event(self) -> Event:
         return Event(self)
@@ -636,6 +661,67 @@ class HipEngine:
         tg, tu = types
         _check(self.lib.hh_gateup_dev(self.handle, tg, tu, d_ff, d_model, wg.handle, wg_off, wu.handle, wu_off,
                                       x.handle, x_off, h.handle, h_off, act))
+
+    # ---------------------------------------------------------------- 8-bit path
+    # No counterpart in the reference; the definitions stand in include/hayai_hip.h.
+    @staticmethod
+    def quant_i8_desc(ggml_type: int, rows: int, cols: int, x_stride: int = 0, up_stride: int = 0, q_stride: int = 0,
+                      act: int = ACT_SILU) -> _abi.QuantI8Desc:
+        return _abi.QuantI8Desc(ggml_type, act, rows, cols, x_stride, up_stride, q_stride)
+
+    def quant_i8_dev(self, desc: _abi.QuantI8Desc, x: DeviceBuffer, x_off: int, up, up_off: int, q: DeviceBuffer,
+                     q_off: int, scale: DeviceBuffer, scale_off: int, values=None, values_off: int = 0) -> None:
+        """Rows of x, or of act(x) * up, as int8 codes and a scale per row; values (optional): what
+        the codes stand for, f32.  Enqueue only."""
+        _check(self.lib.hh_quant_i8_dev(self.handle, C.byref(desc), x.handle, x_off, _handle(up), up_off, q.handle, q_off,
+                                        scale.handle, scale_off, _handle(values), values_off))
+
+    @staticmethod
+    def rms_norm_i8_desc(ggml_type: int, rows: int, cols: int, eps: float, x_stride: int = 0, res_stride: int = 0,
+                         sum_stride: int = 0, q_stride: int = 0) -> _abi.RmsNormI8Desc:
+        return _abi.RmsNormI8Desc(ggml_type, eps, rows, cols, x_stride, res_stride, sum_stride, q_stride)
+
+    def rms_norm_i8_dev(self, desc: _abi.RmsNormI8Desc, x: DeviceBuffer, x_off: int, res, res_off: int,
+                        norm: DeviceBuffer, norm_off: int, sum, sum_off: int, q: DeviceBuffer, q_off: int,
+                        scale: DeviceBuffer, scale_off: int, values=None, values_off: int = 0) -> None:
+        """The RMS norm of x (with res: of x + res, which goes to sum) as int8 codes and a scale per
+        row.  Enqueue only."""
+        _check(self.lib.hh_rms_norm_i8_dev(self.handle, C.byref(desc), x.handle, x_off, _handle(res), res_off,
+                                           norm.handle, norm_off, _handle(sum), sum_off, q.handle, q_off,
+                                           scale.handle, scale_off, _handle(values), values_off))
+
+    @staticmethod
+    def gemm_i8_desc(ggml_type: int, m: int, n: int, tokens: int, w_stride: int = 0, x_stride: int = 0,
+                     res_stride: int = 0, y_stride: int = 0) -> _abi.GemmI8Desc:
+        return _abi.GemmI8Desc(ggml_type, m, n, tokens, w_stride, x_stride, res_stride, y_stride)
+
+    def gemm_i8_dev(self, desc: _abi.GemmI8Desc, w: DeviceBuffer, w_off: int, w_scale: DeviceBuffer, w_scale_off: int,
+                    x: DeviceBuffer, x_off: int, x_scale: DeviceBuffer, x_scale_off: int, res, res_off: int,
+                    y: DeviceBuffer, y_off: int) -> None:
+        """y = (codes x . codes w^T) * x_scale * w_scale (+ res; y may be res).  Enqueue only."""
+        _check(self.lib.hh_gemm_i8_dev(self.handle, C.byref(desc), w.handle, w_off, w_scale.handle, w_scale_off, x.handle,
+                                       x_off, x_scale.handle, x_scale_off, _handle(res), res_off, y.handle,
+                                       y_off))
+
+    @staticmethod
+    def sample_desc(ggml_type: int, rows: int, vocab: int, stride: int = 0) -> _abi.SampleDesc:
+        return _abi.SampleDesc(ggml_type, rows, vocab, stride)
+
+    @staticmethod
+    def sample_params(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, rows: int | None = None) -> np.ndarray:
+        """hh_sample_params for each row (scalars or one value a row), ready to upload."""
+        p = np.empty(np.broadcast(np.empty(1 if rows is None else rows), temperature, top_k, top_p, min_p).shape,
+                     dtype=[("temperature", "<f4"), ("top_k", "<i4"), ("top_p", "<f4"), ("min_p", "<f4")])
+        p["temperature"], p["top_k"], p["top_p"], p["min_p"] = temperature, top_k, top_p, min_p
+        return p
+
+    def sample_dev(self, desc: _abi.SampleDesc, logits: DeviceBuffer, logits_off: int, params: DeviceBuffer,
+                   params_off: int, u: DeviceBuffer, u_off: int, ids: DeviceBuffer, ids_off: int, probs=None,
+                   probs_off: int = 0) -> None:
+        """The next token of each row of logits (temperature, top-k, top-p, min-p and the row's
+        random number u): ids int32, probs f32.  Enqueue only."""
+        _check(self.lib.hh_sample_dev(self.handle, C.byref(desc), logits.handle, logits_off, params.handle, params_off,
+                                      u.handle, u_off, ids.handle, ids_off, _handle(probs), probs_off))
 
     # ---------------------------------------------------------------- synthetic data
     def synth_weights_dev(self, ggml_type: int, dst: DeviceBuffer, off: int, n_blocks: int, seed: int,

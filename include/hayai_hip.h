@@ -62,7 +62,9 @@ enum {
     HH_TYPE_Q4_K = 12,
     HH_TYPE_Q6_K = 14,
     HH_TYPE_IQ2_XXS = 16,
-    HH_TYPE_IQ3_XXS = 18
+    HH_TYPE_IQ3_XXS = 18,
+    /* activations of the 8-bit operators only (no GEMV over BF16 weights) */
+    HH_TYPE_BF16 = 30
 };
 
 /* FFN activation: SiLU(gate)*up (stream_infer.rs:3836-3840) or tanh-GELU(gate)*up
@@ -136,6 +138,12 @@ hh_status hh_buf_alloc(hh_engine* e, size_t bytes, int kind, hh_buf** out);
 void hh_buf_free(hh_buf* b);
 size_t hh_buf_size(const hh_buf* b);
 int hh_buf_kind(const hh_buf* b);
+/* No counterpart in the reference.  A handle on device memory that the caller owns (a tensor of
+ * another library, say): `bytes` bytes at `ptr`, which must lie inside one device allocation of
+ * this engine's GPU (HH_ERR_INVALID otherwise).  hh_buf_free drops the handle after the engine's
+ * queued work and leaves the memory alone.  The engine's stream knows nothing of other streams:
+ * the caller orders work on the memory between them. */
+hh_status hh_buf_wrap(hh_engine* e, void* ptr, size_t bytes, hh_buf** out);
 /* Host address of a pinned buffer (NULL for device buffers). */
 void* hh_buf_host_ptr(hh_buf* b);
 /* Blocking host <-> buffer copies (enqueue_write_buffer / enqueue_read_buffer with
@@ -388,6 +396,101 @@ hh_status hh_moe_ffn_dev(hh_engine* e, const hh_moe_desc* d, const hh_buf* exper
 hh_status hh_moe_dev(hh_engine* e, const hh_moe_desc* d, const hh_buf* experts, size_t experts_off,
                      const hh_buf* logits, size_t logits_off, const hh_buf* bias, size_t bias_off,
                      const hh_buf* x, size_t x_off, size_t T, hh_buf* y, size_t y_off);
+
+/* ------------------------------------------------------------------ 8-bit path ------ */
+
+/* No counterpart in the reference.  The steps of a decoder that runs its matrices as 8-bit
+ * integers with one scale per token and one per weight row: rows into codes (hh_quant_i8_dev,
+ * hh_rms_norm_i8_dev), the products (hh_gemm_i8_dev) and, after the output projection, the choice
+ * of the next token (hh_sample_dev).  An FFN is rms_norm_i8, gemm_i8 over the rows of gate and up
+ * together, quant_i8 of its two halves, gemm_i8 over down with the residual added.
+ *
+ * Activations are HH_TYPE_F32, HH_TYPE_F16 or HH_TYPE_BF16 (`type`; anything else is
+ * HH_ERR_KERNEL_MISSING), addressed by element-aligned byte offsets; their rows may be `*_stride`
+ * elements apart (0: packed).  Codes are int8, their rows `*_stride` bytes apart (0: packed).
+ * Scales are f32.  Zero rows or tokens is a call that does nothing.  All calls are enqueue-only,
+ * may be captured into a graph (hh_sample_dev and hh_gemm_i8_dev after one eager call of the same
+ * sizes, for their workspaces) and give the same bits every time.  Buffers of one call must not
+ * overlap except where said. */
+
+/* Rows into codes: of x itself, or of the gated intermediate u = act(x) * up.  For each row,
+ * with a = max |u|:  q = rint(127 u / a) (ties to even, decided as in 64-bit arithmetic, in -127..127)
+ * and scale = a / 127.  A row of zeros has scale 0 and codes 0; a row holding a NaN or an infinity
+ * has scale NaN and codes 0.  values (or NULL): rows of `cols` f32, packed, q * scale as the codes
+ * stand for them, for consumers that stay in float and must see the same numbers. */
+typedef struct hh_quant_i8_desc {
+    int type;          /* of x and up */
+    int act;           /* HH_ACT_*, with up */
+    size_t rows, cols;
+    size_t x_stride, up_stride; /* elements, >= cols; 0: cols */
+    size_t q_stride;            /* bytes, >= cols; 0: cols */
+} hh_quant_i8_desc;
+hh_status hh_quant_i8_dev(hh_engine* e, const hh_quant_i8_desc* d, const hh_buf* x, size_t x_off, const hh_buf* up,
+                          size_t up_off, hh_buf* q, size_t q_off, hh_buf* scale, size_t scale_off, hh_buf* values,
+                          size_t values_off);
+
+/* The RMS norm of x, or of x + res, into codes: v = x (+ res), u = v * norm with norm `cols`
+ * f32, codes of u as above, scale = a / (127 sqrt(mean(v^2) + eps)): what q * scale stands for is
+ * v * norm / sqrt(mean(v^2) + eps).  With res, sum receives v rounded to `type` (the new residual
+ * stream) and may be res or x; the codes are of v before that rounding.  res and sum: both or
+ * neither. */
+typedef struct hh_rms_norm_i8_desc {
+    int type;          /* of x, res and sum */
+    float eps;         /* 0..1 */
+    size_t rows, cols;
+    size_t x_stride, res_stride, sum_stride; /* elements, >= cols; 0: cols */
+    size_t q_stride;                         /* bytes, >= cols; 0: cols */
+} hh_rms_norm_i8_desc;
+hh_status hh_rms_norm_i8_dev(hh_engine* e, const hh_rms_norm_i8_desc* d, const hh_buf* x, size_t x_off,
+                             const hh_buf* res, size_t res_off, const hh_buf* norm, size_t norm_off, hh_buf* sum,
+                             size_t sum_off, hh_buf* q, size_t q_off, hh_buf* scale, size_t scale_off,
+                             hh_buf* values, size_t values_off);
+
+/* The product of codes: y[t][r] = (sum_k x[t][k] w[r][k]) * x_scale[t] * w_scale[r] (+ res[t][r])
+ * for t < tokens, r < m, the sum over n exact in 32-bit integers, the rest in f32, rounded once to
+ * `type`.  n <= HH_I8_MAX_N.  Rows of w and x start on 16-byte boundaries: both addresses and
+ * strides are multiples of 16 and each of the matrices' rows has its whole stride in the buffer;
+ * bytes n..stride of a row may hold anything.  y may be res (same offset and stride). */
+#define HH_I8_MAX_N 131071u
+typedef struct hh_gemm_i8_desc {
+    int type;          /* of y and res */
+    size_t m, n, tokens;
+    size_t w_stride, x_stride;   /* bytes, multiples of 16, >= n; 0: n */
+    size_t res_stride, y_stride; /* elements, >= m; 0: m */
+} hh_gemm_i8_desc;
+hh_status hh_gemm_i8_dev(hh_engine* e, const hh_gemm_i8_desc* d, const hh_buf* w, size_t w_off, const hh_buf* w_scale,
+                         size_t w_scale_off, const hh_buf* x, size_t x_off, const hh_buf* x_scale,
+                         size_t x_scale_off, const hh_buf* res, size_t res_off, hh_buf* y, size_t y_off);
+
+/* The next token of each row of logits from a given random number u in [0, 1).
+ * With the row's temperature T, a token's weight is exp((logit - max) / T).  Sorted by logit
+ * (equal logits: the lowest index first) the row keeps
+ *   top_k: its first top_k tokens (off where <= 0);
+ *   top_p: of those, the shortest prefix with at least top_p of their weight (off where >= 1);
+ *   min_p: of those, the tokens whose weight is at least min_p (the first has weight 1);
+ * but always the first.  The answer is the kept token, by index, at which the running weight first
+ * exceeds u times the kept weight, and its share of the kept weight.  T <= 0 (or NaN) takes the
+ * first token with probability 1.  A NaN logit counts as -inf; where the largest is +inf those
+ * tokens have weight 1 and the others 0.  A row without a token above -inf gets id -1 and
+ * probability 0.  u outside [0, 1) is taken to its nearest end (NaN: 0).  Weights are held as
+ * whole multiples of 2^-42 (lighter tokens are never drawn), so a row's answer depends on nothing
+ * but the row.  vocab <= HH_SAMPLE_MAX_VOCAB. */
+#define HH_SAMPLE_MAX_VOCAB 2097152u
+typedef struct hh_sample_params {
+    float temperature;
+    int32_t top_k;
+    float top_p;
+    float min_p;
+} hh_sample_params;
+typedef struct hh_sample_desc {
+    int type;          /* of the logits */
+    size_t rows, vocab;
+    size_t stride;     /* elements, >= vocab; 0: vocab */
+} hh_sample_desc;
+/* params: hh_sample_params[rows]; u: f32[rows]; ids: int32[rows]; probs: f32[rows] or NULL. */
+hh_status hh_sample_dev(hh_engine* e, const hh_sample_desc* d, const hh_buf* logits, size_t logits_off,
+                        const hh_buf* params, size_t params_off, const hh_buf* u, size_t u_off, hh_buf* ids,
+                        size_t ids_off, hh_buf* probs, size_t probs_off);
 
 /* ------------------------------------------------------------------ streaming ------- */
 
