@@ -111,7 +111,10 @@ struct hh_i8_gemm_args {
     const void* res;
     void* y;
     uint64_t w_stride, x_stride, res_stride, y_stride;
-    uint32_t m, n, t, pad;
+    uint32_t m, n, t;
+    uint32_t mtiles, ttiles, pad;
+    int* cut;         // sums of tiles cut between workgroups, two tiles a workgroup
+    uint32_t* count;  // arrivals at each tile: zero between launches
 };
 
 // The next token of each row of logits (sample.hip); stride in elements.

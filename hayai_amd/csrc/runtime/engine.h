@@ -341,7 +341,7 @@ struct hh_engine {
     // The 8-bit path (i8.cpp); device pointers, strides resolved (elements for activations, bytes
     // for codes).  b: up (norm null, act) or the residual (norm given); null: none.
     hh_status enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_args& a);
-    hh_status enqueue_i8_gemm(int type, const hh_i8_gemm_args& a);
+    hh_status enqueue_i8_gemm(int type, hh_i8_gemm_args a);
     hh_status enqueue_sample(int type, size_t rows, const hh_sample_args& a);
     // Reports (and clears) a grid-barrier timeout recorded by a fused kernel.  Syncs.
     hh_status check_device_error();

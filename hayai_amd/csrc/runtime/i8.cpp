@@ -16,7 +16,9 @@ void i8_kernels(std::vector<std::string>& k) {
         const std::string ty = act_type(t)->name;
         for (const char* kind : {"plain", "act", "norm"})
             for (const char* v : {"c1", "c2", "loop"}) k.push_back("hh_i8_rows_" + ty + "_" + kind + "_" + v);
-        k.push_back("hh_i8_gemm_simple_" + ty);
+        for (const char* v : {"rowdot_t1", "rowdot_t2", "rowdot_t4", "rowdot_t8", "tile_32x32", "tile_64x64", "big_128x128",
+                              "big_128x256", "big_192x256", "big_256x256"})
+            k.push_back(std::string("hh_i8_") + v + "_" + ty);
         k.push_back("hh_sample_simple_" + ty);
     }
 }
@@ -36,13 +38,89 @@ hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_arg
     return launch(f, (uint32_t)rows, (uint32_t)threads, a);
 }
 
-hh_status hh_engine::enqueue_i8_gemm(int type, const hh_i8_gemm_args& a) {
+// Which form, by the weights' bytes, the tokens and the tiles (28672 x 4096, 4096 x 14336, 4096 x 4096,
+// 128256 x 4096, 32000 x 2048 and 576 x 1536, weights from HBM; us):
+//   rows by v_dot4: one or two tokens (28672 x 4096: 22.0 and 23.8, small tiles 26.6; 4096 x 14336:
+//     11.3 and 12.3, 12.8); up to four where their codes take 32 KB of LDS or less (4096 x 4096 6.6,
+//     6.9; 32000 x 2048 15.8, 17.3; 4096 x 14336 14.3, 12.8); up to eight under 4 MB of weights
+//     (576 x 1536 4.0, 7.2; 4096 x 4096 8.4, 6.9)
+//   tiles of 32 x 32 to 32 tokens (28672 x 4096, 32 tokens: 29.4, of 64 x 64 30.9), and to 64 where 64-row
+//     tiles are few (4096 x 14336, 61 tokens: 15.0, 16.3; 28672 x 4096, 64 tokens: 40.8, 32.5)
+//   past that the least of the estimates below.
+struct I8Big {
+    const char* name;
+    size_t tm, tn, threads, per_cu;
+    double first, round, stage;  // us: once, per round of tiles, per stage of 128 codes and round
+};
+// 28672 x 4096 and 4096 x 14336 at 128 to 4096 tokens: estimates within 15% of most, and the choice
+// within 10% of the best
+static const I8Big kI8Big[] = {
+    {"128x128", 128, 128, 256, 2, 8, 2, 1.04},  // one a CU: 0.67 a stage
+    {"128x256", 128, 256, 512, 1, 6, 2, 0.98},
+    {"192x256", 192, 256, 512, 1, 5, 10, 1.2},
+    {"256x256", 256, 256, 512, 1, 5, 13, 1.45},
+};
+
+hh_status hh_engine::enqueue_i8_gemm(int type, hh_i8_gemm_args a) {
+    const std::string ty = act_type(type)->name;
+    const size_t cus = (size_t)props.multiProcessorCount, chunk_bytes = (a.n + 1023) / 1024 * 1024;
+    const size_t weights = (size_t)a.m * a.n, stages = (a.n + 127) / 128;
     hipFunction_t f;
-    HH_TRY(kernel(std::string("hh_i8_gemm_simple_") + act_type(type)->name, &f));
-    void* params[] = {const_cast<hh_i8_gemm_args*>(&a)};
-    HH_TRY_HIP(hipModuleLaunchKernel(f, (a.m + 63) / 64, (a.t + 63) / 64, 1, 256, 1, 1, 0, stream, params, nullptr),
-               "hipModuleLaunchKernel(i8_gemm)");
-    return HH_OK;
+    const uint32_t T = a.t <= 2 ? a.t : a.t <= 4 ? 4 : 8;
+    const size_t lds = T * chunk_bytes;
+    if (lds <= 131072 && (a.t <= 2 || (a.t <= 4 && lds <= 32768) || (a.t <= 8 && weights < (4u << 20)))) {
+        HH_TRY(kernel("hh_i8_rowdot_t" + std::to_string(T) + "_" + ty, &f));
+        const size_t grid = std::min(cus, ((size_t)a.m + 15) / 16);
+        void* params[] = {&a};
+        HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)grid, 1, 1, 512, 1, 1, (unsigned)lds, stream, params, nullptr),
+                   "hipModuleLaunchKernel(i8_gemm rows)");
+        return HH_OK;
+    }
+    auto tiles = [&](size_t tm, size_t tn) { return (a.m + tm - 1) / tm * ((a.t + tn - 1) / tn); };
+    size_t tm = 64;  // the small tiles' side
+    if (a.t <= 32 || (a.t <= 64 && a.m < 8192)) tm = 32;
+    if (a.t > 64) {
+        const I8Big* best = nullptr;
+        double least = 6 + 0.27 * (double)(tiles(64, 64) * stages) / (double)cus;
+        for (const I8Big& b : kI8Big) {
+            const size_t n = tiles(b.tm, b.tn), slots = cus * b.per_cu;
+            const double stage = b.per_cu > 1 && n <= cus ? 0.67 : b.stage;
+            const double t = b.first + (double)((n + slots - 1) / slots) * (b.round + stage * (double)stages);
+            if (t < least) {
+                least = t;
+                best = &b;
+            }
+        }
+        if (best) {
+            a.mtiles = (uint32_t)((a.m + best->tm - 1) / best->tm);
+            a.ttiles = (uint32_t)((a.t + best->tn - 1) / best->tn);
+            const size_t n = (size_t)a.mtiles * a.ttiles, grid = std::min(cus * best->per_cu, (n + 7) / 8 * 8);
+            if (n > UINT32_MAX / 2) return fail(HH_ERR_INVALID, "gemm_i8: %u x %u outputs are too many", a.t, a.m);
+            HH_TRY(kernel(std::string("hh_i8_big_") + best->name + "_" + ty, &f));
+            return launch(f, (uint32_t)grid, (uint32_t)best->threads, a);
+        }
+    }
+    a.mtiles = (uint32_t)((a.m + tm - 1) / tm);
+    a.ttiles = (uint32_t)((a.t + tm - 1) / tm);
+    const size_t n = (size_t)a.mtiles * a.ttiles, units = n * stages;
+    if (n > UINT32_MAX / 2) return fail(HH_ERR_INVALID, "gemm_i8: %u x %u outputs are too many", a.t, a.m);
+    // workgroups, each at least a stage: two a CU where that cuts few tiles (28672 x 4096, 32 tokens, 896
+    // tiles: 29.4, one a CU 35.6; 4096 x 14336, 32 tokens, 128 tiles: 14.4, 13.2)
+    size_t W = n >= (tm == 32 ? 1 : 2) * cus ? 2 * cus : cus;
+    W = std::max<size_t>(1, std::min(W, units / 2));
+    W = W >= 8 ? W / 8 * 8 : 1;
+    HH_TRY(grow(&ws_part, &ws_part_cap, W * 2 * tm * tm * sizeof(int)));
+    if (ws_cnt_cap < n * sizeof(uint32_t)) {
+        HH_TRY(grow(&ws_cnt, &ws_cnt_cap, n * sizeof(uint32_t)));
+        if (hipError_t err = hipMemsetAsync(ws_cnt, 0, ws_cnt_cap, stream); err != hipSuccess) {
+            ws_cnt_cap = 0;
+            return hip_fail(err, "hipMemsetAsync(counters)");
+        }
+    }
+    a.cut = (int*)ws_part;
+    a.count = (uint32_t*)ws_cnt;
+    HH_TRY(kernel(std::string("hh_i8_tile_") + (tm == 32 ? "32x32_" : "64x64_") + ty, &f));
+    return launch(f, (uint32_t)W, 256, a);
 }
 
 hh_status hh_engine::enqueue_sample(int type, size_t rows, const hh_sample_args& a) {
