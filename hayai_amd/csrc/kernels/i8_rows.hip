@@ -13,36 +13,70 @@
 // vector rate equals the 32-bit one on this chip.
 //
 // One workgroup per row, the row in registers between the two phases (CH chunks of 16 bytes a
-// thread); rows past 1024 threads * 4 chunks are read twice (hh_i8_rows_<...>_loop).
+// thread); rows of more than 2048 chunks are read twice (hh_i8_rows_<...>_loop).
 #include "act_types.h"
 
+template <int CTRL, int ROWS = 0xf>
+HH_DEV uint64_t hh_i8_dpp64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, true);
+    return (uint64_t)hi << 32 | lo;
+}
+HH_DEV uint64_t hh_i8_lane64(uint64_t v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+    return (uint64_t)hi << 32 | lo;
+}
+struct hh_i8_max64 {
+    HH_DEV static uint64_t of(uint64_t a, uint64_t b) { return b > a ? b : a; }
+};
+struct hh_i8_add64 {
+    HH_DEV static uint64_t of(uint64_t a, uint64_t b) {
+        return (uint64_t)__double_as_longlong(__longlong_as_double((long long)a) + __longlong_as_double((long long)b));
+    }
+};
+// Op over each row of 16 lanes, then over the wave (in lane 63).  Zero is neutral to both.
+template <class Op>
+HH_DEV uint64_t hh_i8_row16(uint64_t v) {
+    v = Op::of(v, hh_i8_dpp64<0xB1>(v));
+    v = Op::of(v, hh_i8_dpp64<0x4E>(v));
+    v = Op::of(v, hh_i8_dpp64<0x124>(v));
+    return Op::of(v, hh_i8_dpp64<0x128>(v));
+}
+template <class Op>
+HH_DEV uint64_t hh_i8_wave64(uint64_t v) {
+    v = hh_i8_row16<Op>(v);
+    v = Op::of(v, hh_i8_dpp64<0x142, 0xa>(v));
+    v = Op::of(v, hh_i8_dpp64<0x143, 0xc>(v));
+    return hh_i8_lane64(v, 63);
+}
+// Op over the workgroup of up to 16 waves; red: 16 words of LDS not read since the last meeting.
+template <class Op>
+HH_DEV uint64_t hh_i8_block64(uint64_t v, uint64_t* red) {
+    v = hh_i8_wave64<Op>(v);
+    const uint32_t waves = blockDim.x / HH_WAVE, lane = threadIdx.x % HH_WAVE;
+    if (waves == 1) return v;
+    if (lane == 0) red[threadIdx.x / HH_WAVE] = v;
+    __syncthreads();
+    return hh_i8_lane64(hh_i8_row16<Op>(lane < waves ? red[lane] : 0), 0);
+}
 struct hh_i8_red {
-    uint64_t top[16];
-    double ss[16];
+    uint64_t top[16], ss[16];
 };
 
 // |u| of the row's largest element as bits (NaN sorts above infinity above every number) and the
 // sum of squares, over the workgroup.
+template <bool SUM>
 HH_DEV void hh_i8_reduce(uint64_t& top, double& ss, hh_i8_red& red) {
-#pragma unroll
-    for (int off = 32; off; off >>= 1) {
-        const uint64_t o = __shfl_xor(top, off, HH_WAVE);
-        top = o > top ? o : top;
-        ss += __shfl_xor(ss, off, HH_WAVE);
+    if (SUM) {
+        const uint64_t s = hh_i8_wave64<hh_i8_add64>((uint64_t)__double_as_longlong(ss));
+        if (threadIdx.x % HH_WAVE == 0) red.ss[threadIdx.x / HH_WAVE] = s;
+        ss = __longlong_as_double((long long)s);
     }
-    const uint32_t waves = blockDim.x / HH_WAVE;
-    if (waves == 1) return;
-    if (threadIdx.x % HH_WAVE == 0) {
-        red.top[threadIdx.x / HH_WAVE] = top;
-        red.ss[threadIdx.x / HH_WAVE] = ss;
-    }
-    __syncthreads();
-    top = red.top[0];
-    ss = red.ss[0];
-    for (uint32_t w = 1; w < waves; w++) {
-        top = red.top[w] > top ? red.top[w] : top;
-        ss += red.ss[w];
-    }
+    top = hh_i8_block64<hh_i8_max64>(top, red.top);  // meets
+    const uint32_t waves = blockDim.x / HH_WAVE, lane = threadIdx.x % HH_WAVE;
+    if (SUM && waves > 1)
+        ss = __longlong_as_double((long long)hh_i8_lane64(hh_i8_row16<hh_i8_add64>(lane < waves ? red.ss[lane] : 0), 0));
 }
 
 enum { HH_I8_PLAIN, HH_I8_ACT, HH_I8_NORM };
@@ -177,7 +211,7 @@ HH_DEV void hh_i8_rows_regs(const hh_i8_rows_args& a) {
             if (KIND == HH_I8_NORM) ss += v[i] * v[i];
         }
     }
-    hh_i8_reduce(bits, ss, red);
+    hh_i8_reduce<KIND == HH_I8_NORM>(bits, ss, red);
     double top, inv;
     const float scale = hh_i8_factors<KIND>(a, bits, ss, top, inv);
     const bool zero = !(scale > 0.f);
@@ -212,7 +246,7 @@ HH_DEV void hh_i8_rows_loop(const hh_i8_rows_args& a) {
             if (KIND == HH_I8_NORM) ss += v[i] * v[i];
         }
     }
-    hh_i8_reduce(bits, ss, red);
+    hh_i8_reduce<KIND == HH_I8_NORM>(bits, ss, red);
     double top, inv;
     const float scale = hh_i8_factors<KIND>(a, bits, ss, top, inv);
     const bool zero = !(scale > 0.f);
@@ -229,15 +263,123 @@ HH_DEV void hh_i8_rows_loop(const hh_i8_rows_args& a) {
     }
 }
 
-#define HH_I8_ROWS_CH(T, F, NAME, KIND, CH)                                                                         \
-    extern "C" __global__ void __launch_bounds__(1024) hh_i8_rows_##T##_##NAME##_c##CH(const hh_i8_rows_args a) {  \
-        hh_i8_rows_regs<F, KIND, CH>(a);                                                                            \
+// The gated intermediate in 32 bits, decided in 64: act costs ~60 64-bit operations an element, which
+// is twice the memory's time (509 x 14336 bf16: 27 us).  h = act(g) u is computed in f32 with a bound e
+// on its relative error: the exponent y is within 8 2^-24 |y| (GELU's polynomial, log2 e), v_exp_f32 and
+// v_rcp_f32 within 2^-23, and the products, the sum and 127 / a add at most 2^-24 each.  A code whose t lies within e |t| of a border,
+// and every element that may be the row's largest, is recomputed in 64 bits.  Rows whose largest element
+// is outside 1e-25..1e25 (or NaN) take the 64-bit form whole, elements past |y| = 80 singly.
+HH_DEV float hh_i8_act32(float g, float u, int act, float& e) {
+    const float y = act == HH_ACT_GELU_TANH ? 1.5957691216f * (g + 0.044715f * g * g * g) : g;
+    e = (8.f * fabsf(y) + 32.f) * 0x1p-24f;
+    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y * -1.4426950409f)) * u;
+}
+
+template <class F, int CH>
+HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
+    typedef typename F::E E;
+    constexpr int VEC = F::VEC;
+    constexpr float FAR = (8.f * 80.f + 32.f) * 0x1p-24f;  // e at |y| = 80
+    __shared__ uint64_t red[2][16];
+    const hh_i8_row<F, HH_I8_ACT> row(a, blockIdx.x);
+    E g[CH][VEC], p[CH][VEC];
+    auto count = [&](int c) {
+        const uint32_t e = (c * blockDim.x + threadIdx.x) * VEC;
+        return e >= a.cols ? 0u : min((uint32_t)VEC, a.cols - e);
+    };
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        const uint32_t e = (c * blockDim.x + threadIdx.x) * VEC, n = count(c);
+        if (n == VEC) {
+            hh_load_n(row.x + e, g[c]);
+            hh_load_n(row.b + e, p[c]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                const bool in = (uint32_t)i < n;
+                g[c][i] = in ? row.x[e + i] : F::put(0.f);
+                p[c][i] = in ? row.b[e + i] : F::put(0.f);
+            }
+        }
     }
+    float h[CH][VEC];
+    uint32_t seen = 0;  // largest |h| as bits: NaN and infinities sort above every number
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            float e;
+            h[c][i] = hh_i8_act32(F::get(g[c][i]), F::get(p[c][i]), a.act, e);
+            if (!(e <= FAR)) h[c][i] = (float)hh_i8_act((double)F::get(g[c][i]), (double)F::get(p[c][i]), a.act);
+            seen = max(seen, __float_as_uint(fabsf(h[c][i])));
+        }
+    // then the 64-bit magnitude of whatever may be the largest: |h| (1 +- FAR) holds it
+    const float top32 = __uint_as_float((uint32_t)hh_i8_block64<hh_i8_max64>(seen, red[0]));
+    const bool wide = !(top32 >= 1e-25f && top32 <= 1e25f);
+    const float least = wide ? 0.f : top32 * (1.f - 2.f * FAR);
+    uint64_t bits = 0;
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++)
+            if (wide || fabsf(h[c][i]) >= least) {
+                const double v = hh_i8_act((double)F::get(g[c][i]), (double)F::get(p[c][i]), a.act);
+                const uint64_t m = (uint64_t)__double_as_longlong(v) & 0x7fffffffffffffffull;
+                bits = m > bits ? m : bits;
+            }
+    bits = hh_i8_block64<hh_i8_max64>(bits, red[1]);
+    double top, inv;
+    const float scale = hh_i8_factors<HH_I8_ACT>(a, bits, 0.0, top, inv);
+    const bool zero = !(scale > 0.f);
+    const float inv32 = (float)inv;
+    if (threadIdx.x == 0) a.scale[blockIdx.x] = scale;
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        const uint32_t at = (c * blockDim.x + threadIdx.x) * VEC, n = count(c);
+        if (!n) break;
+        int8_t code[VEC];
+        float val[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            const float t = h[c][i] * inv32;
+            float k = rintf(t);
+            const float y = F::get(g[c][i]);
+            float e;
+            hh_i8_act32(y, 0.f, a.act, e);
+            // |t - k| is exact; the border is at one half
+            if (wide || !(0.5f - fabsf(t - k) > fabsf(t) * e)) {
+                const double u = hh_i8_act((double)y, (double)F::get(p[c][i]), a.act);
+                k = zero ? 0.f : (float)rint(127.0 * u / top);
+            }
+            const int v = zero ? 0 : (int)k;
+            code[i] = (int8_t)v;
+            val[i] = (float)v * scale;
+        }
+        if (n == VEC) {
+            hh_store_n(row.q + at, code);
+            if (row.values) hh_store_n(row.values + at, val);
+        } else {
+            for (uint32_t i = 0; i < n; i++) {
+                row.q[at + i] = code[i];
+                if (row.values) row.values[at + i] = val[i];
+            }
+        }
+    }
+}
+
 #define HH_I8_ROWS_KIND(T, F, NAME, KIND)                                                                           \
-    HH_I8_ROWS_CH(T, F, NAME, KIND, 1)                                                                              \
-    HH_I8_ROWS_CH(T, F, NAME, KIND, 2)                                                                              \
+    HH_I8_ROWS_CH(T, F, NAME, KIND, 1, 1024)                                                                        \
+    HH_I8_ROWS_CH(T, F, NAME, KIND, 2, 1024)                                                                        \
+    HH_I8_ROWS_CH(T, F, NAME, KIND, 4, 512)                                                                         \
     extern "C" __global__ void __launch_bounds__(1024) hh_i8_rows_##T##_##NAME##_loop(const hh_i8_rows_args a) {   \
         hh_i8_rows_loop<F, KIND>(a);                                                                                \
+    }
+#define HH_I8_ROWS_CH(T, F, NAME, KIND, CH, MAX)                                                                    \
+    extern "C" __global__ void __launch_bounds__(MAX) hh_i8_rows_##T##_##NAME##_c##CH(const hh_i8_rows_args a) {   \
+        if constexpr (KIND == HH_I8_ACT)                                                                            \
+            hh_i8_act_rows<F, CH>(a);                                                                               \
+        else                                                                                                        \
+            hh_i8_rows_regs<F, KIND, CH>(a);                                                                        \
     }
 #define HH_I8_ROWS(T, F)                                                                                            \
     HH_I8_ROWS_KIND(T, F, plain, HH_I8_PLAIN)                                                                       \

@@ -15,7 +15,7 @@ void i8_kernels(std::vector<std::string>& k) {
     for (int t : {HH_TYPE_F32, HH_TYPE_F16, HH_TYPE_BF16}) {
         const std::string ty = act_type(t)->name;
         for (const char* kind : {"plain", "act", "norm"})
-            for (const char* v : {"c1", "c2", "loop"}) k.push_back("hh_i8_rows_" + ty + "_" + kind + "_" + v);
+            for (const char* v : {"c1", "c2", "c4", "loop"}) k.push_back("hh_i8_rows_" + ty + "_" + kind + "_" + v);
         for (const char* v : {"rowdot_t1", "rowdot_t2", "rowdot_t4", "rowdot_t8", "tile_32x32", "tile_64x64", "big_128x128",
                               "big_128x256", "big_192x256", "big_256x256"})
             k.push_back(std::string("hh_i8_") + v + "_" + ty);
@@ -30,9 +30,12 @@ using namespace hh;
 hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_args& a) {
     const ActType* ty = act_type(type);
     const size_t chunks = (a.cols * ty->bytes + 15) / 16;
-    const size_t threads = std::min<size_t>(1024, (chunks + 63) / 64 * 64);
+    // Few rows: as many threads as chunks, for latency.  Rows enough to fill the chip twice: four chunks a
+    // thread, so that a CU holds more rows and asks for more of them at once.
+    const bool many = rows >= 2 * (size_t)props.multiProcessorCount && chunks <= 2048;
+    const size_t threads = std::min<size_t>(1024, ((many ? (chunks + 3) / 4 : chunks) + 63) / 64 * 64);
     const char* kind = a.norm ? "norm" : a.b ? "act" : "plain";
-    const char* v = chunks <= threads ? "c1" : chunks <= 2 * threads ? "c2" : "loop";
+    const char* v = many ? "c4" : chunks <= threads ? "c1" : chunks <= 2 * threads ? "c2" : "loop";
     hipFunction_t f;
     HH_TRY(kernel(std::string("hh_i8_rows_") + ty->name + "_" + kind + "_" + v, &f));
     return launch(f, (uint32_t)rows, (uint32_t)threads, a);
@@ -55,8 +58,8 @@ struct I8Big {
 // 28672 x 4096 and 4096 x 14336 at 128 to 4096 tokens: estimates within 15% of most, and the choice
 // within 10% of the best
 static const I8Big kI8Big[] = {
-    {"128x128", 128, 128, 256, 2, 8, 2, 1.04},  // one a CU: 0.67 a stage
-    {"128x256", 128, 256, 512, 1, 6, 2, 0.98},
+    {"128x128", 128, 128, 256, 2, 2, 10, 1.04},  // one a CU: 0.67 a stage
+    {"128x256", 128, 256, 512, 1, 3, 8, 0.98},
     {"192x256", 192, 256, 512, 1, 5, 10, 1.2},
     {"256x256", 256, 256, 512, 1, 5, 13, 1.45},
 };
