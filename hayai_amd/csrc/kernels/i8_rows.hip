@@ -265,95 +265,102 @@ HH_DEV void hh_i8_rows_loop(const hh_i8_rows_args& a) {
 
 // The gated intermediate in 32 bits, decided in 64: act costs ~60 64-bit operations an element, which
 // is twice the memory's time (509 x 14336 bf16: 27 us).  h = act(g) u is computed in f32 with a bound e
-// on its relative error: the exponent y is within 8 2^-24 |y| (GELU's polynomial, log2 e), v_exp_f32 and
-// v_rcp_f32 within 2^-23, and the products, the sum and 127 / a add at most 2^-24 each.  A code whose t lies within e |t| of a border,
-// and every element that may be the row's largest, is recomputed in 64 bits.  Rows whose largest element
-// is outside 1e-25..1e25 (or NaN) take the 64-bit form whole, elements past |y| = 80 singly.
-HH_DEV float hh_i8_act32(float g, float u, int act, float& e) {
-    const float y = act == HH_ACT_GELU_TANH ? 1.5957691216f * (g + 0.044715f * g * g * g) : g;
-    e = (8.f * fabsf(y) + 32.f) * 0x1p-24f;
+// on its relative error: the exponent y is within 8 2^-24 |y| (GELU's polynomial, log2 e; it counts
+// where y < 0, as exp(-y) / (1 + exp(-y)) of it reaches h), v_exp_f32 and v_rcp_f32 are within 2^-23,
+// and the products, the sum and 127 / a add at most 2^-24 each.  A code whose t lies within e |t| of
+// a border, every element that may be the row's largest, and all with y < -80, are recomputed in 64
+// bits from memory, one by one (about one element in 4000).  Rows whose largest element is outside
+// 1e-25..1e25 (or NaN) are recomputed whole.
+HH_DEV float hh_i8_act32(float g, float u, int act, float& y) {
+    y = act == HH_ACT_GELU_TANH ? 1.5957691216f * (g + 0.044715f * g * g * g) : g;
     return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y * -1.4426950409f)) * u;
 }
+HH_DEV float hh_i8_act32_error(float y) { return (8.f * fmaxf(-y, 0.f) + 36.f) * 0x1p-24f; }
 
 template <class F, int CH>
 HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
     typedef typename F::E E;
     constexpr int VEC = F::VEC;
-    constexpr float FAR = (8.f * 80.f + 32.f) * 0x1p-24f;  // e at |y| = 80
+    static_assert(CH * VEC <= 32, "a bit for each element of a thread");
+    constexpr float FAR = (8.f * 80.f + 36.f) * 0x1p-24f;  // the error bound at y = -80
     __shared__ uint64_t red[2][16];
     const hh_i8_row<F, HH_I8_ACT> row(a, blockIdx.x);
-    E g[CH][VEC], p[CH][VEC];
     auto count = [&](int c) {
         const uint32_t e = (c * blockDim.x + threadIdx.x) * VEC;
         return e >= a.cols ? 0u : min((uint32_t)VEC, a.cols - e);
     };
+    E g[CH][VEC];
+    float h[CH][VEC];
+    uint32_t seen = 0, far = 0, here = 0;  // largest |h| as bits: NaN and infinities sort above every number
+    {
+        E p[CH][VEC];
 #pragma unroll
-    for (int c = 0; c < CH; c++) {
-        const uint32_t e = (c * blockDim.x + threadIdx.x) * VEC, n = count(c);
-        if (n == VEC) {
-            hh_load_n(row.x + e, g[c]);
-            hh_load_n(row.b + e, p[c]);
-        } else {
+        for (int c = 0; c < CH; c++) {
+            const uint32_t e = (c * blockDim.x + threadIdx.x) * VEC, n = count(c);
+            if (n == VEC) {
+                hh_load_n(row.x + e, g[c]);
+                hh_load_n(row.b + e, p[c]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    const bool in = (uint32_t)i < n;
+                    g[c][i] = in ? row.x[e + i] : F::put(0.f);
+                    p[c][i] = in ? row.b[e + i] : F::put(0.f);
+                }
+            }
+            here |= ((1u << n) - 1u) << (c * VEC);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; c++)
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                const bool in = (uint32_t)i < n;
-                g[c][i] = in ? row.x[e + i] : F::put(0.f);
-                p[c][i] = in ? row.b[e + i] : F::put(0.f);
+                float y;
+                h[c][i] = hh_i8_act32(F::get(g[c][i]), F::get(p[c][i]), a.act, y);
+                seen = max(seen, __float_as_uint(fabsf(h[c][i])));
+                far |= (y < -80.f ? 1u : 0u) << (c * VEC + i);
             }
-        }
     }
-    float h[CH][VEC];
-    uint32_t seen = 0;  // largest |h| as bits: NaN and infinities sort above every number
-#pragma unroll
-    for (int c = 0; c < CH; c++)
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            float e;
-            h[c][i] = hh_i8_act32(F::get(g[c][i]), F::get(p[c][i]), a.act, e);
-            if (!(e <= FAR)) h[c][i] = (float)hh_i8_act((double)F::get(g[c][i]), (double)F::get(p[c][i]), a.act);
-            seen = max(seen, __float_as_uint(fabsf(h[c][i])));
-        }
-    // then the 64-bit magnitude of whatever may be the largest: |h| (1 +- FAR) holds it
+    auto exact = [&](uint32_t bit, uint32_t& e) {  // element `bit` of this thread in 64 bits
+        e = (bit / VEC * blockDim.x + threadIdx.x) * VEC + bit % VEC;
+        return hh_i8_act((double)F::get(row.x[e]), (double)F::get(row.b[e]), a.act);
+    };
+    // the 64-bit magnitude of whatever may be the largest: |h| (1 +- FAR) holds it
     const float top32 = __uint_as_float((uint32_t)hh_i8_block64<hh_i8_max64>(seen, red[0]));
     const bool wide = !(top32 >= 1e-25f && top32 <= 1e25f);
-    const float least = wide ? 0.f : top32 * (1.f - 2.f * FAR);
-    uint64_t bits = 0;
+    const float least = top32 * (1.f - 2.f * FAR);
+    uint32_t todo = far;
 #pragma unroll
     for (int c = 0; c < CH; c++)
 #pragma unroll
-        for (int i = 0; i < VEC; i++)
-            if (wide || fabsf(h[c][i]) >= least) {
-                const double v = hh_i8_act((double)F::get(g[c][i]), (double)F::get(p[c][i]), a.act);
-                const uint64_t m = (uint64_t)__double_as_longlong(v) & 0x7fffffffffffffffull;
-                bits = m > bits ? m : bits;
-            }
+        for (int i = 0; i < VEC; i++) todo |= (fabsf(h[c][i]) >= least ? 1u : 0u) << (c * VEC + i);
+    todo = (wide ? ~0u : todo) & here;
+    uint64_t bits = 0;
+    for (; todo; todo &= todo - 1) {
+        uint32_t e;
+        const double v = exact((uint32_t)__builtin_ctz(todo), e);
+        const uint64_t m = (uint64_t)__double_as_longlong(v) & 0x7fffffffffffffffull;
+        bits = m > bits ? m : bits;
+    }
     bits = hh_i8_block64<hh_i8_max64>(bits, red[1]);
     double top, inv;
     const float scale = hh_i8_factors<HH_I8_ACT>(a, bits, 0.0, top, inv);
-    const bool zero = !(scale > 0.f);
-    const float inv32 = (float)inv;
+    const float inv32 = scale > 0.f && !wide ? (float)inv : 0.f;  // 0: codes 0 until recomputed
     if (threadIdx.x == 0) a.scale[blockIdx.x] = scale;
+    todo = far;
 #pragma unroll
     for (int c = 0; c < CH; c++) {
         const uint32_t at = (c * blockDim.x + threadIdx.x) * VEC, n = count(c);
-        if (!n) break;
         int8_t code[VEC];
         float val[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
-            const float t = h[c][i] * inv32;
-            float k = rintf(t);
-            const float y = F::get(g[c][i]);
-            float e;
-            hh_i8_act32(y, 0.f, a.act, e);
+            const float t = inv32 > 0.f ? h[c][i] * inv32 : 0.f;
+            const float k = rintf(t), gi = F::get(g[c][i]);
+            const float y = a.act == HH_ACT_GELU_TANH ? 1.5957691216f * (gi + 0.044715f * gi * gi * gi) : gi;
             // |t - k| is exact; the border is at one half
-            if (wide || !(0.5f - fabsf(t - k) > fabsf(t) * e)) {
-                const double u = hh_i8_act((double)y, (double)F::get(p[c][i]), a.act);
-                k = zero ? 0.f : (float)rint(127.0 * u / top);
-            }
-            const int v = zero ? 0 : (int)k;
-            code[i] = (int8_t)v;
-            val[i] = (float)v * scale;
+            todo |= (0.5f - fabsf(t - k) > fabsf(t) * hh_i8_act32_error(y) ? 0u : 1u) << (c * VEC + i);
+            code[i] = (int8_t)(int)k;
+            val[i] = k * scale;
         }
         if (n == VEC) {
             hh_store_n(row.q + at, code);
@@ -364,6 +371,13 @@ HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
                 if (row.values) row.values[at + i] = val[i];
             }
         }
+    }
+    if (!(scale > 0.f)) return;
+    for (todo = (wide ? ~0u : todo) & here; todo; todo &= todo - 1) {
+        uint32_t e;
+        const float k = (float)rint(127.0 * exact((uint32_t)__builtin_ctz(todo), e) / top);
+        row.q[e] = (int8_t)(int)k;
+        if (row.values) row.values[e] = k * scale;
     }
 }
 
