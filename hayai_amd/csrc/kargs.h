@@ -117,16 +117,22 @@ struct hh_i8_gemm_args {
     uint32_t* count;  // arrivals at each tile: zero between launches
 };
 
-// The next token of each row of logits (sample.hip); stride in elements.
+// The next token of each row of logits (sample.hip); stride in elements.  The workspaces hold, per row:
 struct hh_sample_args {
     const void* x;
     const void* params;  // hh_sample_params
     const float* u;
     int32_t* ids;
     float* probs;
+    uint64_t* top;     // `parts`: a part's first token
+    uint64_t* mass;    // 1024: weight by distance from the largest logit
+    uint64_t* sure;    // `chunks`: weight surely kept
+    uint64_t* list;    // 8192: tokens at the filters' ends
+    uint32_t* count;   // 1024: tokens by distance
+    uint32_t* listed;  // the list's length
+    void* cut;         // hh_smp_cut
     uint64_t stride;
-    uint32_t vocab;
-    uint32_t pad;
+    uint32_t vocab, parts, chunks, pad;
 };
 
 // Synthetic GGUF bytes: splitmix64 stream, then f16 scale fields drawn U(lo, hi).

@@ -1,12 +1,21 @@
 // The next token of each row of logits: temperature, top-k, top-p and min-p, then the draw by a
 // given random number u (include/hayai_hip.h has the definition).
 //
-// No sort: each filter keeps a prefix of the row's order (logit descending, index ascending), so it
-// is described by the key of its last token and how many of that key's tokens are in, found by a
-// radix select over the 32-bit ordered keys (8 bits at a time, counts or weights per digit).
-// Weights are exp((logit - max) / T) in 64 bits, held as whole multiples of 2^-42: sums of whole
-// numbers do not depend on their order, so atomics leave the answer fixed, and 2^21 tokens of weight 1
-// stay below 2^63.  One workgroup per row.
+// No sort: each filter keeps a prefix of the row's order (logit descending, index ascending), which is
+// described by its last token's key and index.  Weights are exp((logit - max) / T) in 64 bits, held
+// as whole multiples of 2^-42: sums of whole numbers do not depend on their order, so atomics leave the
+// answer fixed, and 2^21 tokens of weight 1 stay below 2^63.
+//
+// Four launches, the row cut into parts (workgroups) of whole 512-token chunks:
+//   hh_sample_max     the part's largest key and its first index
+//   hh_sample_hist    counts and weights of the row's tokens by distance from the largest logit, in
+//                     1023 bins of T / 32 and one for what weighs nothing
+//   hh_sample_gather  the bins in which top-k and top-p end; the weight that each chunk surely keeps,
+//                     and the tokens of those bins into a list
+//   hh_sample_pick    one workgroup a row: where in the list the prefix ends (radix select), the
+//                     chunk at which the running weight passes u, the token in it
+// A row whose list passes 8192 tokens (nearly equal logits throughout) is done by one workgroup from
+// the logits (hh_sample_row).
 #include "act_types.h"
 
 struct hh_sample_row_params {
@@ -29,12 +38,23 @@ HH_DEV uint32_t hh_smp_key(float v) {
 #define HH_SMP_KEY_INF 0xff800000u   // of +inf
 HH_DEV float hh_smp_value(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu)); }
 
+// e^x for x <= 0: 2^n times the Taylor polynomial of e^(f ln 2), |f| <= 1/2, whose 13 terms leave
+// 0.35^13 / 13! = 2e-16.
+HH_DEV double hh_smp_exp(double x) {
+    const double y = fmax(x * 1.4426950408889634074, -1100.0), n = rint(y), f = (y - n) * 0.69314718055994530942;
+    double p = 1.0 / 479001600.0;
+    constexpr double c[12] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
+                              1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800};
+#pragma unroll
+    for (int i = 11; i >= 0; i--) p = fma(p, f, c[i]);
+    return ldexp(p, (int)n);
+}
 // Weight of the token with this key in a row whose largest key is top.
 HH_DEV double hh_smp_weight(uint32_t key, uint32_t top, float temperature) {
     if (key <= HH_SMP_KEY_NINF) return 0.0;
     if (key == top) return 1.0;
     if (top == HH_SMP_KEY_INF) return 0.0;
-    return exp(((double)hh_smp_value(key) - (double)hh_smp_value(top)) / (double)temperature);
+    return hh_smp_exp(((double)hh_smp_value(key) - (double)hh_smp_value(top)) / (double)temperature);
 }
 HH_DEV uint64_t hh_smp_mass(double w) { return (uint64_t)(w * HH_SMP_ONE); }
 
@@ -42,6 +62,7 @@ struct hh_smp_lds {
     unsigned long long hist[256];
     uint64_t wave[16];
     uint64_t before, found;
+    unsigned long long any, all;
     uint32_t digit, top;
 };
 
@@ -100,9 +121,9 @@ HH_DEV uint32_t hh_smp_select(const typename F::E* x, uint32_t n, uint32_t floor
     return prefix;
 }
 
+// A whole row by one workgroup of 1024.
 template <class F>
-HH_DEV void hh_sample_simple(const hh_sample_args& a) {
-    __shared__ hh_smp_lds s;
+HH_DEV void hh_sample_row(const hh_sample_args& a, hh_smp_lds& s) {
     const uint32_t row = blockIdx.x, n = a.vocab, tid = threadIdx.x;
     const typename F::E* x = (const typename F::E*)a.x + row * a.stride;
     const hh_sample_row_params p = ((const hh_sample_row_params*)a.params)[row];
@@ -218,9 +239,480 @@ HH_DEV void hh_sample_simple(const hh_sample_args& a) {
     }
 }
 
-#define HH_SAMPLE(T, F)                                                                               \
-    extern "C" __global__ void __launch_bounds__(1024) hh_sample_simple_##T(const hh_sample_args a) { \
-        hh_sample_simple<F>(a);                                                                       \
+// ------------------------------------------------------------------ the four launches
+#define HH_SMP_CHUNK 512u    // tokens whose kept weight is one sum (4096 of them at most)
+#define HH_SMP_BINS 1024u
+#define HH_SMP_LIST 8192u
+#define HH_SMP_THREADS 512u  // of the first three
+
+// What hh_sample_gather finds about a row, for hh_sample_pick.
+struct hh_smp_cut {
+    uint32_t kbin, plo, phi;  // top-k ends in kbin, top-p in plo..phi (HH_SMP_BINS: no such end)
+    uint32_t kneed;           // tokens of kbin that top-k keeps
+    uint64_t kmass, pmass;    // weight of the bins before kbin (all: no such end), before plo
+};
+
+// A row's distance bins: 32 to a temperature; the largest key's is the first, the last one's tokens
+// are 31 temperatures below or more, which weighs less than 2^-42.
+struct hh_smp_bins {
+    uint32_t top;
+    double value, scale;
+    HH_DEV hh_smp_bins(uint32_t top_, float temperature) : top(top_) {
+        value = (double)hh_smp_value(top_);
+        scale = 32.0 / (double)temperature;
+    }
+    // rounding keeps the order: a lower logit never has a lower bin
+    HH_DEV uint32_t of(uint32_t key) const {
+        if (key == top) return 0;
+        const double d = (value - (double)hh_smp_value(key)) * scale;
+        return d < 1023.0 ? (uint32_t)d : HH_SMP_BINS - 1;  // infinite or NaN (an infinite top): the last
+    }
+};
+
+// A token as one number: the row's order is that of falling numbers.
+#define HH_SMP_INDEX_BITS 21
+HH_DEV uint64_t hh_smp_entry(uint32_t key, uint32_t i) {
+    return (uint64_t)key << HH_SMP_INDEX_BITS | ((1u << HH_SMP_INDEX_BITS) - 1u - i);
+}
+HH_DEV uint32_t hh_smp_entry_key(uint64_t e) { return (uint32_t)(e >> HH_SMP_INDEX_BITS); }
+HH_DEV uint32_t hh_smp_entry_index(uint64_t e) {
+    const uint32_t mask = (1u << HH_SMP_INDEX_BITS) - 1u;
+    return mask - ((uint32_t)e & mask);
+}
+
+HH_DEV uint64_t hh_smp_max64(uint64_t v) {
+#pragma unroll
+    for (int off = 32; off; off >>= 1) {
+        const uint64_t o = __shfl_xor(v, off, HH_WAVE);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+// The row's first token, from the parts'.
+HH_DEV uint64_t hh_smp_top(const hh_sample_args& a, uint32_t row) {
+    uint64_t v = 0;
+    for (uint32_t i = threadIdx.x % HH_WAVE; i < a.parts; i += HH_WAVE) {
+        const uint64_t o = a.top[(size_t)row * a.parts + i];
+        v = o > v ? o : v;
+    }
+    return hh_smp_max64(v);
+}
+// The tokens [lo, hi) of this workgroup's part.
+HH_DEV void hh_smp_part(const hh_sample_args& a, uint32_t& lo, uint32_t& hi) {
+    const uint32_t chunks = (a.vocab + HH_SMP_CHUNK - 1) / HH_SMP_CHUNK, per = (chunks + a.parts - 1) / a.parts;
+    lo = min(a.vocab, blockIdx.x * per * HH_SMP_CHUNK);
+    hi = min(a.vocab, lo + per * HH_SMP_CHUNK);
+}
+// f(key, index) for each token of [lo, hi) by `threads` threads, of which this is one.
+template <class F, class Fn>
+HH_DEV void hh_smp_each(const typename F::E* x, uint32_t lo, uint32_t hi, uint32_t threads, uint32_t thread, Fn f) {
+    constexpr uint32_t VEC = F::VEC;
+    uint32_t i = lo + thread * VEC;
+#pragma unroll 2
+    for (; i + VEC <= hi; i += threads * VEC) {
+        typename F::E v[VEC];
+        hh_load_n(x + i, v);
+#pragma unroll
+        for (uint32_t e = 0; e < VEC; e++) f(hh_smp_key(F::get(v[e])), i + e);
+    }
+    if (i < hi)
+        for (uint32_t e = i; e < hi && e < i + VEC; e++) f(hh_smp_key(F::get(x[e])), e);
+}
+
+template <class F>
+HH_DEV void hh_sample_max(const hh_sample_args& a) {
+    __shared__ uint64_t red[HH_SMP_THREADS / HH_WAVE];
+    const uint32_t row = blockIdx.y, tid = threadIdx.x;
+    const typename F::E* x = (const typename F::E*)a.x + row * a.stride;
+    uint32_t lo, hi, key = 0, at = 0;
+    hh_smp_part(a, lo, hi);
+    hh_smp_each<F>(x, lo, hi, HH_SMP_THREADS, tid, [&](uint32_t k, uint32_t i) {
+        at = k > key ? i : at;  // a thread's indices ascend
+        key = k > key ? k : key;
+    });
+    uint64_t v = hh_smp_max64(hh_smp_entry(key, at));
+    if (tid % HH_WAVE == 0) red[tid / HH_WAVE] = v;
+    __syncthreads();
+    // this part's share of the row's bins and the list's length to zero, for the next launches
+    uint64_t* mass = a.mass + (size_t)row * HH_SMP_BINS;
+    uint32_t* count = a.count + (size_t)row * HH_SMP_BINS;
+    for (uint32_t i = blockIdx.x * HH_SMP_THREADS + tid; i < HH_SMP_BINS; i += a.parts * HH_SMP_THREADS) {
+        mass[i] = 0;
+        count[i] = 0;
+    }
+    if (tid == 0) {
+        for (uint32_t w = 1; w < HH_SMP_THREADS / HH_WAVE; w++) v = red[w] > v ? red[w] : v;
+        a.top[(size_t)row * a.parts + blockIdx.x] = v;
+        if (blockIdx.x == 0) a.listed[row] = 0;
+    }
+}
+
+HH_DEV bool hh_smp_filters(const hh_sample_row_params& p, uint32_t vocab) {
+    return (p.top_k > 0 && (uint32_t)p.top_k < vocab) || p.top_p < 1.f;
+}
+
+template <class F>
+HH_DEV void hh_sample_hist(const hh_sample_args& a) {
+    __shared__ unsigned long long mass[HH_SMP_BINS];
+    __shared__ uint32_t count[HH_SMP_BINS];
+    const uint32_t row = blockIdx.y, tid = threadIdx.x;
+    const hh_sample_row_params p = ((const hh_sample_row_params*)a.params)[row];
+    if (!(p.temperature > 0.f) || !hh_smp_filters(p, a.vocab)) return;
+    const uint32_t top = hh_smp_entry_key(hh_smp_top(a, row));
+    if (top <= HH_SMP_KEY_NINF) return;
+    for (uint32_t i = tid; i < HH_SMP_BINS; i += HH_SMP_THREADS) {
+        mass[i] = 0;
+        count[i] = 0;
+    }
+    __syncthreads();
+    const hh_smp_bins bins(top, p.temperature);
+    uint32_t lo, hi;
+    hh_smp_part(a, lo, hi);
+    const bool weigh = p.top_p < 1.f;
+    hh_smp_each<F>((const typename F::E*)a.x + row * a.stride, lo, hi, HH_SMP_THREADS, tid, [&](uint32_t key, uint32_t) {
+        const uint32_t b = bins.of(key);
+        if (key <= HH_SMP_KEY_NINF || b == HH_SMP_BINS - 1) return;
+        atomicAdd(&count[b], 1u);
+        if (weigh) atomicAdd(&mass[b], (unsigned long long)hh_smp_mass(hh_smp_weight(key, top, p.temperature)));
+    });
+    __syncthreads();
+    for (uint32_t i = tid; i < HH_SMP_BINS; i += HH_SMP_THREADS)
+        if (count[i]) {
+            atomicAdd(&a.count[(size_t)row * HH_SMP_BINS + i], count[i]);
+            if (weigh) atomicAdd((unsigned long long*)&a.mass[(size_t)row * HH_SMP_BINS + i], mass[i]);
+        }
+}
+
+// Inclusive sums over the workgroup's threads in thread order; red: a word a wave.
+HH_DEV uint64_t hh_smp_scan_block(uint64_t v, uint64_t* red) {
+    const uint32_t lane = threadIdx.x % HH_WAVE, w = threadIdx.x / HH_WAVE;
+#pragma unroll
+    for (int off = 1; off < HH_WAVE; off <<= 1) {
+        const uint64_t o = __shfl_up(v, off, HH_WAVE);
+        if (lane >= (uint32_t)off) v += o;
+    }
+    __syncthreads();
+    if (lane == HH_WAVE - 1) red[w] = v;
+    __syncthreads();
+    for (uint32_t i = 0; i < w; i++) v += red[i];
+    return v;
+}
+
+// The bins in which the filters end, from the row's sums: the same in every workgroup of the row.
+HH_DEV void hh_smp_find_cut(const hh_sample_args& a, uint32_t row, const hh_sample_row_params& p, hh_smp_cut& cut,
+                            uint64_t* red) {
+    static_assert(HH_SMP_BINS == 2 * HH_SMP_THREADS, "two bins a thread");
+    const uint32_t tid = threadIdx.x;
+    if (tid == 0) cut = hh_smp_cut{HH_SMP_BINS, HH_SMP_BINS, HH_SMP_BINS, 0, 0, 0};
+    const size_t at = (size_t)row * HH_SMP_BINS + 2 * tid;
+    const uint64_t c0 = a.count[at], c1 = a.count[at + 1], m0 = a.mass[at], m1 = a.mass[at + 1];
+    const uint64_t cs = hh_smp_scan_block(c0 + c1, red), cb = cs - c0 - c1;  // (meets: cut is set)
+    const uint64_t ms = hh_smp_scan_block(m0 + m1, red), mb = ms - m0 - m1;
+    const bool topk = p.top_k > 0 && (uint32_t)p.top_k < a.vocab;
+    if (topk) {
+        const uint64_t k = (uint32_t)p.top_k;
+        if (cb < k && cb + c0 >= k) {
+            cut.kbin = 2 * tid;
+            cut.kneed = (uint32_t)(k - cb);
+            cut.kmass = mb;
+        } else if (cb + c0 < k && cs >= k) {
+            cut.kbin = 2 * tid + 1;
+            cut.kneed = (uint32_t)(k - cb - c0);
+            cut.kmass = mb + m0;
+        }
+    }
+    __syncthreads();
+    if (tid == HH_SMP_THREADS - 1 && cut.kbin == HH_SMP_BINS) cut.kmass = ms;
+    if (p.top_p < 1.f) {
+        // between what top-k keeps at least and at most
+        __shared__ double want[2];
+        const uint32_t kbin = cut.kbin;
+        if (tid == HH_SMP_THREADS - 1 && kbin == HH_SMP_BINS) want[0] = want[1] = (double)p.top_p * (double)ms;
+        if (kbin < HH_SMP_BINS && tid == kbin / 2) {
+            want[0] = (double)p.top_p * (double)cut.kmass;
+            want[1] = (double)p.top_p * (double)(cut.kmass + (kbin % 2 ? m1 : m0));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            // the first bin with tokens at which the running weight reaches want
+            const uint64_t before = q ? mb + m0 : mb, here = q ? m1 : m0, n = q ? c1 : c0;
+            const bool first = n && (before == 0 || (double)before < want[0]);
+            if (first && (double)(before + here) >= want[0]) {
+                cut.plo = 2 * tid + q;
+                cut.pmass = before;
+            }
+            if (n && (before == 0 || (double)before < want[1]) && (double)(before + here) >= want[1]) cut.phi = 2 * tid + q;
+        }
+        __syncthreads();
+        if (tid == 0 && cut.plo > cut.kbin) {  // cannot be, but a bin past top-k's end is no end
+            cut.plo = cut.kbin;
+            cut.pmass = cut.kmass;
+        }
+        if (tid == 0) cut.phi = min(cut.phi, cut.kbin);
+    } else if (tid == 0) {
+        cut.plo = cut.phi = cut.kbin;
+        cut.pmass = cut.kmass;
+    }
+    __syncthreads();
+}
+
+template <class F>
+HH_DEV void hh_sample_gather(const hh_sample_args& a) {
+    __shared__ hh_smp_cut cut;
+    __shared__ uint64_t red[HH_SMP_THREADS / HH_WAVE];
+    const uint32_t row = blockIdx.y, tid = threadIdx.x;
+    const hh_sample_row_params p = ((const hh_sample_row_params*)a.params)[row];
+    if (!(p.temperature > 0.f)) return;
+    const uint32_t top = hh_smp_entry_key(hh_smp_top(a, row));
+    if (top <= HH_SMP_KEY_NINF) return;
+    if (hh_smp_filters(p, a.vocab)) {
+        hh_smp_find_cut(a, row, p, cut, red);
+    } else {
+        if (tid == 0) cut = hh_smp_cut{HH_SMP_BINS, HH_SMP_BINS, HH_SMP_BINS, 0, 0, 0};
+        __syncthreads();
+    }
+    if (blockIdx.x == 0 && tid == 0) ((hh_smp_cut*)a.cut)[row] = cut;
+    const uint32_t kbin = cut.kbin, plo = cut.plo, phi = cut.phi;
+    const hh_smp_bins bins(top, p.temperature);
+    const double heavy = p.min_p > 0.f ? (double)p.min_p : 0.0;
+    uint64_t* list = a.list + (size_t)row * HH_SMP_LIST;
+    uint32_t lo, hi;
+    hh_smp_part(a, lo, hi);
+    // a wave takes a chunk
+    for (uint32_t c = lo + tid / HH_WAVE * HH_SMP_CHUNK; c < hi; c += HH_SMP_THREADS / HH_WAVE * HH_SMP_CHUNK) {
+        uint64_t mine = 0;
+        hh_smp_each<F>((const typename F::E*)a.x + row * a.stride, c, min(hi, c + HH_SMP_CHUNK), HH_WAVE, tid % HH_WAVE,
+                       [&](uint32_t key, uint32_t i) {
+            if (key <= HH_SMP_KEY_NINF) return;
+            const uint32_t b = bins.of(key);
+            if (b < plo) {
+                const double w = hh_smp_weight(key, top, p.temperature);
+                if (w >= heavy || key == top) mine += hh_smp_mass(w);
+            } else if (b <= phi || b == kbin) {
+                const uint32_t at = atomicAdd(&a.listed[row], 1u);
+                if (at < HH_SMP_LIST) list[at] = hh_smp_entry(key, i);
+            }
+        });
+#pragma unroll
+        for (int off = 32; off; off >>= 1) mine += __shfl_xor(mine, off, HH_WAVE);
+        if (tid % HH_WAVE == 0) a.sure[(size_t)row * a.chunks + c / HH_SMP_CHUNK] = mine;
+    }
+}
+
+// The list's entries of a thread, 0: none.
+#define HH_SMP_EACH (HH_SMP_LIST / HH_SMP_BLOCK)
+
+// The entry at which the running amount, from the largest down over the entries that `take` takes, first
+// reaches want; before: the amount of the entries above it.  (want is within their sum.)
+template <class Take, class Amount>
+HH_DEV uint64_t hh_smp_list_cut(const uint64_t (&v)[HH_SMP_EACH], double want, Take take, Amount amount, hh_smp_lds& s,
+                                uint64_t& before) {
+    // the bits in which the entries differ
+    uint64_t any = 0, all = ~0ull;
+#pragma unroll
+    for (uint32_t i = 0; i < HH_SMP_EACH; i++)
+        if (take(v[i])) {
+            any |= v[i];
+            all &= v[i];
+        }
+#pragma unroll
+    for (int off = 32; off; off >>= 1) {
+        any |= __shfl_xor(any, off, HH_WAVE);
+        all &= __shfl_xor(all, off, HH_WAVE);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s.any = 0;
+        s.all = ~0ull;
+    }
+    __syncthreads();
+    if (threadIdx.x % HH_WAVE == 0) {
+        atomicOr(&s.any, (unsigned long long)any);
+        atomicAnd(&s.all, (unsigned long long)all);
+    }
+    __syncthreads();
+    const uint64_t differ = s.any & ~s.all;
+    uint64_t prefix = s.all, above = 0;  // bits above the first that differs are common
+    int shift = differ ? 64 - __builtin_clzll(differ) : 0;
+    if (shift < 64) prefix = shift ? prefix >> shift << shift : prefix;
+    else prefix = 0;
+    while (shift > 0) {
+        const int width = shift < 8 ? shift : 8;
+        shift -= width;
+        __syncthreads();
+        if (threadIdx.x < 256) s.hist[threadIdx.x] = 0;
+        if (threadIdx.x == 0) {  // the lowest, should rounding let none reach want
+            s.digit = 0;
+            s.before = above;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < HH_SMP_EACH; i++)
+            if (take(v[i]) && (shift + width >= 64 || (v[i] >> (shift + width)) == (prefix >> (shift + width))))
+                atomicAdd(&s.hist[(v[i] >> shift) & ((1u << width) - 1u)], (unsigned long long)amount(v[i]));
+        __syncthreads();
+        if (threadIdx.x < HH_WAVE) {
+            // lane l has digits 255 - 4 l down to 252 - 4 l
+            const uint32_t d0 = 255 - 4 * threadIdx.x;
+            uint64_t h[4], sum = 0;
+#pragma unroll
+            for (int q = 0; q < 4; q++) sum += h[q] = s.hist[d0 - q];
+            uint64_t run = sum;
+#pragma unroll
+            for (int off = 1; off < HH_WAVE; off <<= 1) {
+                const uint64_t o = __shfl_up(run, off, HH_WAVE);
+                if ((int)threadIdx.x >= off) run += o;
+            }
+            run += above - sum;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (h[q] && (run == 0 || (double)run < want) && (double)(run + h[q]) >= want) {
+                    s.digit = d0 - q;
+                    s.before = run;
+                }
+                run += h[q];
+            }
+        }
+        __syncthreads();
+        prefix |= (uint64_t)s.digit << shift;
+        above = s.before;
+    }
+    before = above;
+    return prefix;
+}
+
+template <class F>
+HH_DEV void hh_sample_pick(const hh_sample_args& a) {
+    __shared__ hh_smp_lds s;
+    __shared__ unsigned long long mass[2097152 / HH_SMP_CHUNK];
+    const uint32_t row = blockIdx.x, tid = threadIdx.x;
+    const typename F::E* x = (const typename F::E*)a.x + row * a.stride;
+    const hh_sample_row_params p = ((const hh_sample_row_params*)a.params)[row];
+    const uint64_t best = hh_smp_top(a, row);
+    const uint32_t top = hh_smp_entry_key(best), n = a.listed[row];
+    if (top <= HH_SMP_KEY_NINF || !(p.temperature > 0.f)) {
+        const bool none = top <= HH_SMP_KEY_NINF;
+        if (tid == 0) {
+            a.ids[row] = none ? -1 : (int32_t)hh_smp_entry_index(best);
+            if (a.probs) a.probs[row] = none ? 0.f : 1.f;
+        }
+        return;
+    }
+    if (n > HH_SMP_LIST) return hh_sample_row<F>(a, s);
+    const float T = p.temperature;
+    const hh_smp_cut cut = ((const hh_smp_cut*)a.cut)[row];
+    const hh_smp_bins bins(top, T);
+    auto weigh = [&](uint64_t e) { return hh_smp_mass(hh_smp_weight(hh_smp_entry_key(e), top, T)); };
+    uint64_t v[HH_SMP_EACH];
+#pragma unroll
+    for (uint32_t i = 0; i < HH_SMP_EACH; i++) {
+        const uint32_t at = i * HH_SMP_BLOCK + tid;
+        v[i] = at < n ? a.list[(size_t)row * HH_SMP_LIST + at] : 0;
+    }
+    // tokens from `last` on are in
+    uint64_t last = 0, before;
+    if (cut.kbin < HH_SMP_BINS) {
+        auto in_k = [&](uint64_t e) { return e && bins.of(hh_smp_entry_key(e)) == cut.kbin; };
+        last = hh_smp_list_cut(v, (double)cut.kneed, in_k, [](uint64_t) { return 1ull; }, s, before);
+    }
+    if (p.top_p < 1.f && cut.plo < HH_SMP_BINS) {
+        uint64_t kept = 0;  // of top-k's last bin
+        if (cut.kbin < HH_SMP_BINS) {
+#pragma unroll
+            for (uint32_t i = 0; i < HH_SMP_EACH; i++)
+                if (v[i] && v[i] >= last && bins.of(hh_smp_entry_key(v[i])) == cut.kbin) kept += weigh(v[i]);
+            kept = hh_smp_scan(kept, s);
+            __syncthreads();
+            if (tid == HH_SMP_BLOCK - 1) s.found = kept;
+            __syncthreads();
+            kept = s.found;
+        }
+        const double want = (double)p.top_p * (double)(cut.kmass + kept);
+        const uint64_t klast = last;
+        auto in_p = [&](uint64_t e) { return e && e >= klast && bins.of(hh_smp_entry_key(e)) <= cut.phi; };
+        last = hh_smp_list_cut(v, want - (double)cut.pmass, in_p, weigh, s, before);
+    }
+    if (p.min_p > 1.f) last = best;  // heavier than any token: the first alone
+    const double heavy = p.min_p > 0.f ? (double)p.min_p : 0.0;
+    auto kept_mass = [&](uint64_t e) -> uint64_t {
+        const uint32_t key = hh_smp_entry_key(e);
+        if (e < last || key <= HH_SMP_KEY_NINF) return 0;
+        const double w = hh_smp_weight(key, top, T);
+        return key == top || w >= heavy ? hh_smp_mass(w) : 0;
+    };
+    // the chunks' kept weight, four a thread: what is sure and the list's
+    constexpr uint32_t EACH = sizeof mass / sizeof mass[0] / HH_SMP_BLOCK;
+#pragma unroll
+    for (uint32_t q = 0; q < EACH; q++) {
+        const uint32_t c = EACH * tid + q;
+        mass[c] = c < a.chunks && !(p.min_p > 1.f) ? a.sure[(size_t)row * a.chunks + c] : 0;
+    }
+    __syncthreads();
+    if (p.min_p > 1.f) {
+        if (tid == 0) mass[hh_smp_entry_index(best) / HH_SMP_CHUNK] = (unsigned long long)HH_SMP_ONE;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < HH_SMP_EACH; i++) {
+            const uint64_t m = v[i] ? kept_mass(v[i]) : 0;
+            if (m) atomicAdd(&mass[hh_smp_entry_index(v[i]) / HH_SMP_CHUNK], (unsigned long long)m);
+        }
+    }
+    __syncthreads();
+    uint64_t mine = 0;
+#pragma unroll
+    for (uint32_t q = 0; q < EACH; q++) mine += mass[EACH * tid + q];
+    uint64_t after = hh_smp_scan(mine, s);
+    __syncthreads();
+    if (tid == HH_SMP_BLOCK - 1) s.found = after;
+    __syncthreads();
+    const uint64_t total = s.found;
+    double u = (double)a.u[row];
+    if (!(u > 0.0)) u = 0.0;
+    uint64_t want = u < 1.0 ? (uint64_t)(u * (double)total) : total - 1;
+    if (want >= total) want = total - 1;
+    // the chunk at which the running weight first exceeds `want`
+    if (after > want && after - mine <= want) {
+        uint64_t run = after - mine;
+        for (uint32_t q = 0; q < EACH; q++) {
+            const uint64_t m = mass[EACH * tid + q];
+            if (run + m > want) {
+                s.digit = EACH * tid + q;
+                s.before = want - run;
+                break;
+            }
+            run += m;
+        }
+    }
+    __syncthreads();
+    want = s.before;
+    // and the token in it
+    const uint32_t i = s.digit * HH_SMP_CHUNK + tid;
+    uint64_t m = 0;
+    uint32_t key = 0;
+    if (tid < HH_SMP_CHUNK && i < a.vocab) {
+        key = hh_smp_key(F::get(x[i]));
+        m = kept_mass(hh_smp_entry(key, i));
+    }
+    after = hh_smp_scan(m, s);
+    if (after > want && after - m <= want) {
+        a.ids[row] = (int32_t)i;
+        if (a.probs) a.probs[row] = (float)(hh_smp_weight(key, top, T) * HH_SMP_ONE / (double)total);
+    }
+}
+
+#define HH_SAMPLE(T, F)                                                                                      \
+    extern "C" __global__ void __launch_bounds__(512) hh_sample_max_##T(const hh_sample_args a) {            \
+        hh_sample_max<F>(a);                                                                                 \
+    }                                                                                                        \
+    extern "C" __global__ void __launch_bounds__(512) hh_sample_hist_##T(const hh_sample_args a) {           \
+        hh_sample_hist<F>(a);                                                                                \
+    }                                                                                                        \
+    extern "C" __global__ void __launch_bounds__(512) hh_sample_gather_##T(const hh_sample_args a) {         \
+        hh_sample_gather<F>(a);                                                                              \
+    }                                                                                                        \
+    extern "C" __global__ void __launch_bounds__(1024) hh_sample_pick_##T(const hh_sample_args a) {          \
+        hh_sample_pick<F>(a);                                                                                \
     }
 HH_SAMPLE(f32, hh_af32)
 HH_SAMPLE(f16, hh_af16)

@@ -171,6 +171,8 @@ struct hh_engine {
     size_t ws_moe_q_cap = 0;
     void* ws_stk = nullptr;     // FFN-stack exchange: tagged words of h (d_ff) then x (d_model); zeroed
     size_t ws_stk_cap = 0;      // when allocated and after a device error
+    void* ws_smp = nullptr;     // token choice: sums, lists (sample.hip)
+    size_t ws_smp_cap = 0;
     void* grid_sync = nullptr;  // grid-barrier state (counters, flags, error word, epochs)
     hh_ffn_desc ffn_stage{};    // FFN whose gate/up output is pending in ws_h (/ws_hq)
     bool ffn_stage_valid = false;
@@ -342,7 +344,7 @@ struct hh_engine {
     // for codes).  b: up (norm null, act) or the residual (norm given); null: none.
     hh_status enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_args& a);
     hh_status enqueue_i8_gemm(int type, hh_i8_gemm_args a);
-    hh_status enqueue_sample(int type, size_t rows, const hh_sample_args& a);
+    hh_status enqueue_sample(int type, size_t rows, hh_sample_args a);
     // Reports (and clears) a grid-barrier timeout recorded by a fused kernel.  Syncs.
     hh_status check_device_error();
 };

@@ -19,7 +19,7 @@ void i8_kernels(std::vector<std::string>& k) {
         for (const char* v : {"rowdot_t1", "rowdot_t2", "rowdot_t4", "rowdot_t8", "tile_32x32", "tile_64x64", "big_128x128",
                               "big_128x256", "big_192x256", "big_256x256"})
             k.push_back(std::string("hh_i8_") + v + "_" + ty);
-        k.push_back("hh_sample_simple_" + ty);
+        for (const char* v : {"max", "hist", "gather", "pick"}) k.push_back(std::string("hh_sample_") + v + "_" + ty);
     }
 }
 
@@ -126,8 +126,42 @@ hh_status hh_engine::enqueue_i8_gemm(int type, hh_i8_gemm_args a) {
     return launch(f, (uint32_t)W, 256, a);
 }
 
-hh_status hh_engine::enqueue_sample(int type, size_t rows, const hh_sample_args& a) {
-    hipFunction_t f;
-    HH_TRY(kernel(std::string("hh_sample_simple_") + act_type(type)->name, &f));
-    return launch(f, (uint32_t)rows, 1024, a);
+// Sizes of sample.hip.
+static const size_t kSmpChunk = 512, kSmpBins = 1024, kSmpList = 8192, kSmpCutBytes = 32;
+static const size_t kSmpRows = 1024;  // rows a pass: bounds the workspace (80 KB a row and 8 bytes a chunk)
+
+hh_status hh_engine::enqueue_sample(int type, size_t rows, hh_sample_args a) {
+    const ActType* ty = act_type(type);
+    hipFunction_t f[4];
+    const char* names[] = {"max", "hist", "gather", "pick"};
+    for (int i = 0; i < 4; i++) HH_TRY(kernel(std::string("hh_sample_") + names[i] + "_" + ty->name, &f[i]));
+    const size_t pass = std::min(rows, kSmpRows);
+    a.chunks = (uint32_t)((a.vocab + kSmpChunk - 1) / kSmpChunk);
+    // parts of 4096 tokens or more, and no more than fill the chip twice
+    a.parts = (uint32_t)std::max<size_t>(
+        1, std::min<size_t>((a.vocab + 4095) / 4096, (2 * (size_t)props.multiProcessorCount + pass - 1) / pass));
+    const size_t row_bytes = 8 * (a.parts + kSmpBins + a.chunks + kSmpList) + 4 * kSmpBins + kSmpCutBytes + 4;
+    HH_TRY(grow(&ws_smp, &ws_smp_cap, pass * row_bytes));
+    a.top = (uint64_t*)ws_smp;
+    a.mass = a.top + pass * a.parts;
+    a.sure = a.mass + pass * kSmpBins;
+    a.list = a.sure + pass * a.chunks;
+    a.cut = a.list + pass * kSmpList;
+    a.count = (uint32_t*)((char*)a.cut + pass * kSmpCutBytes);
+    a.listed = a.count + pass * kSmpBins;
+    for (size_t r = 0; r < rows; r += pass) {
+        const size_t n = std::min(pass, rows - r);
+        hh_sample_args b = a;
+        b.x = (const char*)a.x + r * a.stride * ty->bytes;
+        b.params = (const char*)a.params + r * sizeof(hh_sample_params);
+        b.u = a.u + r;
+        b.ids = a.ids + r;
+        b.probs = a.probs ? a.probs + r : nullptr;
+        void* params[] = {&b};
+        for (int i = 0; i < 3; i++)
+            HH_TRY_HIP(hipModuleLaunchKernel(f[i], a.parts, (uint32_t)n, 1, 512, 1, 1, 0, stream, params, nullptr),
+                       "hipModuleLaunchKernel(sample)");
+        HH_TRY(launch(f[3], (uint32_t)n, 1024, b));
+    }
+    return HH_OK;
 }
