@@ -38,31 +38,40 @@ HH_DEV uint32_t hh_smp_key(float v) {
 #define HH_SMP_KEY_INF 0xff800000u   // of +inf
 HH_DEV float hh_smp_value(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu)); }
 
-// e^x for x <= 0: 2^n times the Taylor polynomial of e^(f ln 2), |f| <= 1/2, whose 13 terms leave
-// 0.35^13 / 13! = 2e-16.
-HH_DEV double hh_smp_exp(double x) {
-    const double y = fmax(x * 1.4426950408889634074, -1100.0), n = rint(y), f = (y - n) * 0.69314718055994530942;
-    double p = 1.0 / 479001600.0;
-    constexpr double c[12] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
-                              1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800};
+// A row's weights, in units of 2^-42: 2^42 e^((logit - max) / T) is 2^(n + 42) times the Taylor polynomial
+// of e^(f ln 2), |f| <= 1/2, whose 12 terms leave 0.35^12 / 12! = 6e-15.  (T enters as log2 e / T: a
+// quotient an element would cost as much again.)
+struct hh_smp_weights {
+    uint32_t top;
+    double value, scale;
+    HH_DEV hh_smp_weights(uint32_t top_, float temperature) : top(top_) {
+        value = (double)hh_smp_value(top_);
+        scale = 1.4426950408889634074 / (double)temperature;
+    }
+    HH_DEV double of(uint32_t key) const {
+        if (key <= HH_SMP_KEY_NINF || (top == HH_SMP_KEY_INF && key != top)) return 0.0;
+        if (key == top) return HH_SMP_ONE;
+        const double y = fmax(((double)hh_smp_value(key) - value) * scale, -1100.0), n = rint(y);
+        const double f = (y - n) * 0.69314718055994530942;
+        constexpr double c[11] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
+                                  1.0 / 362880, 1.0 / 3628800};
+        double p = 1.0 / 39916800;
 #pragma unroll
-    for (int i = 11; i >= 0; i--) p = fma(p, f, c[i]);
-    return ldexp(p, (int)n);
+        for (int i = 10; i >= 0; i--) p = fma(p, f, c[i]);
+        return ldexp(p, (int)n + 42);
+    }
+};
+// The nearest whole number of a weight (below 2^43): the low bits of 2^52 + w.
+HH_DEV uint64_t hh_smp_mass(double w) {
+    return (uint64_t)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
 }
-// Weight of the token with this key in a row whose largest key is top.
-HH_DEV double hh_smp_weight(uint32_t key, uint32_t top, float temperature) {
-    if (key <= HH_SMP_KEY_NINF) return 0.0;
-    if (key == top) return 1.0;
-    if (top == HH_SMP_KEY_INF) return 0.0;
-    return hh_smp_exp(((double)hh_smp_value(key) - (double)hh_smp_value(top)) / (double)temperature);
-}
-HH_DEV uint64_t hh_smp_mass(double w) { return (uint64_t)(w * HH_SMP_ONE); }
 
 struct hh_smp_lds {
     unsigned long long hist[256];
     uint64_t wave[16];
     uint64_t before, found;
     unsigned long long any, all;
+    uint64_t sort[HH_SMP_BLOCK];
     uint32_t digit, top;
 };
 
@@ -144,8 +153,8 @@ HH_DEV void hh_sample_row(const hh_sample_args& a, hh_smp_lds& s) {
         }
         return;
     }
-    const float T = p.temperature;
-    auto mass = [&](uint32_t key) { return hh_smp_mass(hh_smp_weight(key, top, T)); };
+    const hh_smp_weights weights(top, p.temperature);
+    auto mass = [&](uint32_t key) { return hh_smp_mass(weights.of(key)); };
 
     // cut: tokens with larger keys are in, of those with this key the first `ties` by index
     uint32_t cut = HH_SMP_KEY_NINF;
@@ -193,8 +202,8 @@ HH_DEV void hh_sample_row(const hh_sample_args& a, hh_smp_lds& s) {
             ties = 1;
         }
     }
-    const double floor_w = !greedy && p.min_p > 0.f ? (double)p.min_p : 0.0;
-    auto heavy = [&](uint32_t key) { return key == top || hh_smp_weight(key, top, T) >= floor_w; };
+    const double floor_w = !greedy && p.min_p > 0.f ? (double)p.min_p * HH_SMP_ONE : 0.0;
+    auto heavy = [&](uint32_t key) { return key == top || weights.of(key) >= floor_w; };
     const bool only_top = greedy || cut == top;
     if (only_top && ties == 0) ties = 1;
 
@@ -232,7 +241,7 @@ HH_DEV void hh_sample_row(const hh_sample_args& a, hh_smp_lds& s) {
             if (run > want) {
                 a.ids[row] = (int32_t)i;
                 if (a.probs)
-                    a.probs[row] = greedy ? 1.f : (float)(hh_smp_weight(key, top, T) * HH_SMP_ONE / (double)total);
+                    a.probs[row] = greedy ? 1.f : (float)(weights.of(key) / (double)total);
                 break;
             }
         }
@@ -242,7 +251,8 @@ HH_DEV void hh_sample_row(const hh_sample_args& a, hh_smp_lds& s) {
 // ------------------------------------------------------------------ the four launches
 #define HH_SMP_CHUNK 512u    // tokens whose kept weight is one sum (4096 of them at most)
 #define HH_SMP_BINS 1024u
-#define HH_SMP_LIST 8192u
+#define HH_SMP_LIST 8192u    // tokens of a row's list, and of a part's before they join it
+#define HH_SMP_STAGE 2048u
 #define HH_SMP_THREADS 512u  // of the first three
 
 // What hh_sample_gather finds about a row, for hh_sample_pick.
@@ -256,16 +266,15 @@ struct hh_smp_cut {
 // are 31 temperatures below or more, which weighs less than 2^-42.
 struct hh_smp_bins {
     uint32_t top;
-    double value, scale;
+    float value, scale;
     HH_DEV hh_smp_bins(uint32_t top_, float temperature) : top(top_) {
-        value = (double)hh_smp_value(top_);
-        scale = 32.0 / (double)temperature;
+        value = hh_smp_value(top_);
+        scale = 32.f / temperature;
     }
     // rounding keeps the order: a lower logit never has a lower bin
     HH_DEV uint32_t of(uint32_t key) const {
-        if (key == top) return 0;
-        const double d = (value - (double)hh_smp_value(key)) * scale;
-        return d < 1023.0 ? (uint32_t)d : HH_SMP_BINS - 1;  // infinite or NaN (an infinite top): the last
+        const float d = fminf(value - hh_smp_value(key), 3.4028235e38f) * scale;  // (an infinite T: all in bin 0)
+        return key == top ? 0u : d < 1023.f ? (uint32_t)d : HH_SMP_BINS - 1;
     }
 };
 
@@ -369,11 +378,12 @@ HH_DEV void hh_sample_hist(const hh_sample_args& a) {
     uint32_t lo, hi;
     hh_smp_part(a, lo, hi);
     const bool weigh = p.top_p < 1.f;
+    const hh_smp_weights weights(top, p.temperature);
     hh_smp_each<F>((const typename F::E*)a.x + row * a.stride, lo, hi, HH_SMP_THREADS, tid, [&](uint32_t key, uint32_t) {
         const uint32_t b = bins.of(key);
         if (key <= HH_SMP_KEY_NINF || b == HH_SMP_BINS - 1) return;
         atomicAdd(&count[b], 1u);
-        if (weigh) atomicAdd(&mass[b], (unsigned long long)hh_smp_mass(hh_smp_weight(key, top, p.temperature)));
+        if (weigh) atomicAdd(&mass[b], (unsigned long long)hh_smp_mass(weights.of(key)));
     });
     __syncthreads();
     for (uint32_t i = tid; i < HH_SMP_BINS; i += HH_SMP_THREADS)
@@ -460,7 +470,8 @@ HH_DEV void hh_smp_find_cut(const hh_sample_args& a, uint32_t row, const hh_samp
 template <class F>
 HH_DEV void hh_sample_gather(const hh_sample_args& a) {
     __shared__ hh_smp_cut cut;
-    __shared__ uint64_t red[HH_SMP_THREADS / HH_WAVE];
+    __shared__ uint64_t red[HH_SMP_THREADS / HH_WAVE], stage[HH_SMP_STAGE];
+    __shared__ uint32_t found, base;
     const uint32_t row = blockIdx.y, tid = threadIdx.x;
     const hh_sample_row_params p = ((const hh_sample_row_params*)a.params)[row];
     if (!(p.temperature > 0.f)) return;
@@ -475,8 +486,11 @@ HH_DEV void hh_sample_gather(const hh_sample_args& a) {
     if (blockIdx.x == 0 && tid == 0) ((hh_smp_cut*)a.cut)[row] = cut;
     const uint32_t kbin = cut.kbin, plo = cut.plo, phi = cut.phi;
     const hh_smp_bins bins(top, p.temperature);
-    const double heavy = p.min_p > 0.f ? (double)p.min_p : 0.0;
+    const hh_smp_weights weights(top, p.temperature);
+    const double heavy = p.min_p > 0.f ? (double)p.min_p * HH_SMP_ONE : 0.0;
     uint64_t* list = a.list + (size_t)row * HH_SMP_LIST;
+    if (tid == 0) found = 0;
+    __syncthreads();
     uint32_t lo, hi;
     hh_smp_part(a, lo, hi);
     // a wave takes a chunk
@@ -487,17 +501,30 @@ HH_DEV void hh_sample_gather(const hh_sample_args& a) {
             if (key <= HH_SMP_KEY_NINF) return;
             const uint32_t b = bins.of(key);
             if (b < plo) {
-                const double w = hh_smp_weight(key, top, p.temperature);
+                const double w = weights.of(key);
                 if (w >= heavy || key == top) mine += hh_smp_mass(w);
             } else if (b <= phi || b == kbin) {
-                const uint32_t at = atomicAdd(&a.listed[row], 1u);
-                if (at < HH_SMP_LIST) list[at] = hh_smp_entry(key, i);
+                // into LDS first: a count on a device word takes microseconds
+                const uint32_t at = atomicAdd(&found, 1u);
+                if (at < HH_SMP_STAGE) {
+                    stage[at] = hh_smp_entry(key, i);
+                } else {
+                    const uint32_t to = atomicAdd(&a.listed[row], 1u);
+                    if (to < HH_SMP_LIST) list[to] = hh_smp_entry(key, i);
+                }
             }
         });
 #pragma unroll
         for (int off = 32; off; off >>= 1) mine += __shfl_xor(mine, off, HH_WAVE);
         if (tid % HH_WAVE == 0) a.sure[(size_t)row * a.chunks + c / HH_SMP_CHUNK] = mine;
     }
+    __syncthreads();
+    const uint32_t n = min(found, HH_SMP_STAGE);
+    if (n == 0) return;
+    if (tid == 0) base = atomicAdd(&a.listed[row], n);
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += HH_SMP_THREADS)
+        if (base + i < HH_SMP_LIST) list[base + i] = stage[i];
 }
 
 // The list's entries of a thread, 0: none.
@@ -582,6 +609,98 @@ HH_DEV uint64_t hh_smp_list_cut(const uint64_t (&v)[HH_SMP_EACH], double want, T
     return prefix;
 }
 
+// The last token of the row that the filters keep, from a list of more than HH_SMP_BLOCK.
+template <class Weigh>
+HH_DEV uint64_t hh_smp_end_select(const uint64_t* list, uint32_t n, const hh_sample_row_params& p, const hh_smp_cut& cut,
+                                  const hh_smp_bins& bins, Weigh weigh, hh_smp_lds& s) {
+    uint64_t v[HH_SMP_EACH], last = 0, before;
+#pragma unroll
+    for (uint32_t i = 0; i < HH_SMP_EACH; i++) {
+        const uint32_t at = i * HH_SMP_BLOCK + threadIdx.x;
+        v[i] = at < n ? list[at] : 0;
+    }
+    if (cut.kbin < HH_SMP_BINS) {
+        auto in_k = [&](uint64_t e) { return e && bins.of(hh_smp_entry_key(e)) == cut.kbin; };
+        last = hh_smp_list_cut(v, (double)cut.kneed, in_k, [](uint64_t) { return 1ull; }, s, before);
+    }
+    if (!(p.top_p < 1.f)) return last;
+    uint64_t kept = 0;  // of top-k's last bin
+    if (cut.kbin < HH_SMP_BINS) {
+#pragma unroll
+        for (uint32_t i = 0; i < HH_SMP_EACH; i++)
+            if (v[i] && v[i] >= last && bins.of(hh_smp_entry_key(v[i])) == cut.kbin) kept += weigh(v[i]);
+        kept = hh_smp_scan(kept, s);
+        __syncthreads();
+        if (threadIdx.x == HH_SMP_BLOCK - 1) s.found = kept;
+        __syncthreads();
+        kept = s.found;
+    }
+    const double want = (double)p.top_p * (double)(cut.kmass + kept);
+    const uint64_t klast = last;
+    auto in_p = [&](uint64_t e) { return e && e >= klast && bins.of(hh_smp_entry_key(e)) <= cut.phi; };
+    return hh_smp_list_cut(v, want - (double)cut.pmass, in_p, weigh, s, before);
+}
+
+// The same from a list that has a thread for each entry: sorted (a bitonic network over the power of two
+// that holds it, in shuffles where partners share a wave), its weights summed up once.
+template <class Weigh>
+HH_DEV uint64_t hh_smp_end_sorted(const uint64_t* list, uint32_t n, const hh_sample_row_params& p, const hh_smp_cut& cut,
+                                  const hh_smp_bins& bins, Weigh weigh, hh_smp_lds& s) {
+    const uint32_t tid = threadIdx.x;
+    uint64_t e = tid < n ? list[tid] : 0;
+    uint32_t size = 2;
+    while (size < n) size *= 2;
+    for (uint32_t k = 2; k <= size; k *= 2)
+        for (uint32_t j = k / 2; j > 0; j /= 2) {
+            uint64_t o;
+            if (j >= HH_WAVE) {
+                __syncthreads();
+                s.sort[tid] = e;
+                __syncthreads();
+                o = s.sort[tid ^ j];
+            } else {
+                o = __shfl_xor(e, (int)j, HH_WAVE);
+            }
+            const bool keep_large = ((tid & j) == 0) == ((tid & k) == 0);
+            e = (o > e) == keep_large ? o : e;
+        }
+    const uint64_t m = e ? weigh(e) : 0, run = hh_smp_scan(m, s);
+    const uint32_t bin = e ? bins.of(hh_smp_entry_key(e)) : HH_SMP_BINS;
+    // entries of kbin follow those of lower bins: its first entry, then the last that top-k keeps
+    __syncthreads();
+    s.sort[tid] = (uint64_t)bin;
+    if (tid == 0) {
+        s.digit = 0;
+        s.any = 0;
+        s.before = 0;
+        s.found = 0;
+    }
+    __syncthreads();
+    const bool topk = cut.kbin < HH_SMP_BINS;
+    if (topk && bin == cut.kbin && (tid == 0 || s.sort[tid - 1] != bin)) {
+        s.digit = tid;
+        s.before = run - m;
+    }
+    __syncthreads();
+    const uint32_t kend = topk ? s.digit + cut.kneed - 1 : HH_SMP_BLOCK;
+    if (topk && tid == kend) {
+        s.any = e;
+        s.found = run - s.before;  // kbin's weight that top-k keeps
+    }
+    __syncthreads();
+    uint64_t last = s.any;
+    if (p.top_p < 1.f) {
+        const double want = (double)p.top_p * (double)(cut.kmass + s.found);
+        const uint64_t before = cut.pmass + run - m;
+        __syncthreads();
+        if (e && bin <= cut.phi && tid <= kend && (before == 0 || (double)before < want) && (double)(before + m) >= want && m)
+            s.any = e;
+        __syncthreads();
+        last = s.any;
+    }
+    return last;
+}
+
 template <class F>
 HH_DEV void hh_sample_pick(const hh_sample_args& a) {
     __shared__ hh_smp_lds s;
@@ -600,45 +719,20 @@ HH_DEV void hh_sample_pick(const hh_sample_args& a) {
         return;
     }
     if (n > HH_SMP_LIST) return hh_sample_row<F>(a, s);
-    const float T = p.temperature;
     const hh_smp_cut cut = ((const hh_smp_cut*)a.cut)[row];
-    const hh_smp_bins bins(top, T);
-    auto weigh = [&](uint64_t e) { return hh_smp_mass(hh_smp_weight(hh_smp_entry_key(e), top, T)); };
-    uint64_t v[HH_SMP_EACH];
-#pragma unroll
-    for (uint32_t i = 0; i < HH_SMP_EACH; i++) {
-        const uint32_t at = i * HH_SMP_BLOCK + tid;
-        v[i] = at < n ? a.list[(size_t)row * HH_SMP_LIST + at] : 0;
-    }
+    const hh_smp_bins bins(top, p.temperature);
+    const hh_smp_weights weights(top, p.temperature);
+    auto weigh = [&](uint64_t e) { return hh_smp_mass(weights.of(hh_smp_entry_key(e))); };
+    const uint64_t* list = a.list + (size_t)row * HH_SMP_LIST;
     // tokens from `last` on are in
-    uint64_t last = 0, before;
-    if (cut.kbin < HH_SMP_BINS) {
-        auto in_k = [&](uint64_t e) { return e && bins.of(hh_smp_entry_key(e)) == cut.kbin; };
-        last = hh_smp_list_cut(v, (double)cut.kneed, in_k, [](uint64_t) { return 1ull; }, s, before);
-    }
-    if (p.top_p < 1.f && cut.plo < HH_SMP_BINS) {
-        uint64_t kept = 0;  // of top-k's last bin
-        if (cut.kbin < HH_SMP_BINS) {
-#pragma unroll
-            for (uint32_t i = 0; i < HH_SMP_EACH; i++)
-                if (v[i] && v[i] >= last && bins.of(hh_smp_entry_key(v[i])) == cut.kbin) kept += weigh(v[i]);
-            kept = hh_smp_scan(kept, s);
-            __syncthreads();
-            if (tid == HH_SMP_BLOCK - 1) s.found = kept;
-            __syncthreads();
-            kept = s.found;
-        }
-        const double want = (double)p.top_p * (double)(cut.kmass + kept);
-        const uint64_t klast = last;
-        auto in_p = [&](uint64_t e) { return e && e >= klast && bins.of(hh_smp_entry_key(e)) <= cut.phi; };
-        last = hh_smp_list_cut(v, want - (double)cut.pmass, in_p, weigh, s, before);
-    }
+    uint64_t last = 0;
+    if (n) last = n <= HH_SMP_BLOCK ? hh_smp_end_sorted(list, n, p, cut, bins, weigh, s) : hh_smp_end_select(list, n, p, cut, bins, weigh, s);
     if (p.min_p > 1.f) last = best;  // heavier than any token: the first alone
-    const double heavy = p.min_p > 0.f ? (double)p.min_p : 0.0;
+    const double heavy = p.min_p > 0.f ? (double)p.min_p * HH_SMP_ONE : 0.0;
     auto kept_mass = [&](uint64_t e) -> uint64_t {
         const uint32_t key = hh_smp_entry_key(e);
         if (e < last || key <= HH_SMP_KEY_NINF) return 0;
-        const double w = hh_smp_weight(key, top, T);
+        const double w = weights.of(key);
         return key == top || w >= heavy ? hh_smp_mass(w) : 0;
     };
     // the chunks' kept weight, four a thread: what is sure and the list's
@@ -652,10 +746,9 @@ HH_DEV void hh_sample_pick(const hh_sample_args& a) {
     if (p.min_p > 1.f) {
         if (tid == 0) mass[hh_smp_entry_index(best) / HH_SMP_CHUNK] = (unsigned long long)HH_SMP_ONE;
     } else {
-#pragma unroll
-        for (uint32_t i = 0; i < HH_SMP_EACH; i++) {
-            const uint64_t m = v[i] ? kept_mass(v[i]) : 0;
-            if (m) atomicAdd(&mass[hh_smp_entry_index(v[i]) / HH_SMP_CHUNK], (unsigned long long)m);
+        for (uint32_t i = tid; i < n; i += HH_SMP_BLOCK) {
+            const uint64_t e = list[i], m = kept_mass(e);
+            if (m) atomicAdd(&mass[hh_smp_entry_index(e) / HH_SMP_CHUNK], (unsigned long long)m);
         }
     }
     __syncthreads();
@@ -697,7 +790,7 @@ HH_DEV void hh_sample_pick(const hh_sample_args& a) {
     after = hh_smp_scan(m, s);
     if (after > want && after - m <= want) {
         a.ids[row] = (int32_t)i;
-        if (a.probs) a.probs[row] = (float)(hh_smp_weight(key, top, T) * HH_SMP_ONE / (double)total);
+        if (a.probs) a.probs[row] = (float)(weights.of(key) / (double)total);
     }
 }
 
