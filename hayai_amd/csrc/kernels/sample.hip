@@ -14,8 +14,8 @@
 //                     and the tokens of those bins into a list
 //   hh_sample_pick    one workgroup a row: where in the list the prefix ends (radix select), the
 //                     chunk at which the running weight passes u, the token in it
-// A row whose list passes 8192 tokens (nearly equal logits throughout) is done by one workgroup from
-// the logits (hh_sample_row).
+// A row whose list passes 8192 tokens (nearly equal logits throughout), whose largest logit is infinite or
+// whose T is past 1e30 is done by one workgroup from the logits (hh_sample_row).
 #include "act_types.h"
 
 struct hh_sample_row_params {
@@ -38,9 +38,9 @@ HH_DEV uint32_t hh_smp_key(float v) {
 #define HH_SMP_KEY_INF 0xff800000u   // of +inf
 HH_DEV float hh_smp_value(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu)); }
 
-// A row's weights, in units of 2^-42: 2^42 e^((logit - max) / T) is 2^(n + 42) times the Taylor polynomial
-// of e^(f ln 2), |f| <= 1/2, whose 12 terms leave 0.35^12 / 12! = 6e-15.  (T enters as log2 e / T: a
-// quotient an element would cost as much again.)
+// A row's weights, in units of 2^-42: 2^42 e^((logit - max) / T) is 2^(n + 42) 2^f, |f| <= 1/2, with 2^f
+// as the Taylor polynomial of e^(f ln 2), whose 12 terms leave 0.35^12 / 12! = 6e-15.  (T enters as
+// log2 e / T: a quotient an element would cost as much again.)
 struct hh_smp_weights {
     uint32_t top;
     double value, scale;
@@ -48,17 +48,22 @@ struct hh_smp_weights {
         value = (double)hh_smp_value(top_);
         scale = 1.4426950408889634074 / (double)temperature;
     }
-    HH_DEV double of(uint32_t key) const {
-        if (key <= HH_SMP_KEY_NINF || (top == HH_SMP_KEY_INF && key != top)) return 0.0;
-        if (key == top) return HH_SMP_ONE;
-        const double y = fmax(((double)hh_smp_value(key) - value) * scale, -1100.0), n = rint(y);
-        const double f = (y - n) * 0.69314718055994530942;
-        constexpr double c[11] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
-                                  1.0 / 362880, 1.0 / 3628800};
-        double p = 1.0 / 39916800;
+    HH_DEV static double pow2(double y) {  // 2^(y + 42)
+        constexpr double L = 0.69314718055994530942, L2 = L * L, L4 = L2 * L2, L8 = L4 * L4;
+        constexpr double c[11] = {1.0, L, L2 / 2, L2 * L / 6, L4 / 24, L4 * L / 120, L4 * L2 / 720, L4 * L2 * L / 5040,
+                                  L8 / 40320, L8 * L / 362880, L8 * L2 / 3628800};
+        const double n = rint(y), f = y - n;
+        double p = L8 * L2 * L / 39916800;
 #pragma unroll
         for (int i = 10; i >= 0; i--) p = fma(p, f, c[i]);
         return ldexp(p, (int)n + 42);
+    }
+    // of a logit within a few hundred temperatures of a finite largest
+    HH_DEV double near(float v) const { return pow2(((double)v - value) * scale); }
+    HH_DEV double of(uint32_t key) const {
+        if (key <= HH_SMP_KEY_NINF || (top == HH_SMP_KEY_INF && key != top)) return 0.0;
+        if (key == top) return HH_SMP_ONE;
+        return pow2(fmax(((double)hh_smp_value(key) - value) * scale, -1100.0));
     }
 };
 // The nearest whole number of a weight (below 2^43): the low bits of 2^52 + w.
@@ -262,20 +267,18 @@ struct hh_smp_cut {
     uint64_t kmass, pmass;    // weight of the bins before kbin (all: no such end), before plo
 };
 
-// A row's distance bins: 32 to a temperature; the largest key's is the first, the last one's tokens
-// are 31 temperatures below or more, which weighs less than 2^-42.
+// A row's distance bins: 32 to a temperature; the last one's tokens are 31 temperatures below the
+// largest or more, which weighs less than 2^-43, and -inf and NaN are among them.  For a finite largest logit
+// and T <= 1e30 (other rows are left to hh_sample_row).
 struct hh_smp_bins {
-    uint32_t top;
     float value, scale;
-    HH_DEV hh_smp_bins(uint32_t top_, float temperature) : top(top_) {
-        value = hh_smp_value(top_);
+    HH_DEV hh_smp_bins(uint32_t top, float temperature) {
+        value = hh_smp_value(top);
         scale = 32.f / temperature;
     }
-    // rounding keeps the order: a lower logit never has a lower bin
-    HH_DEV uint32_t of(uint32_t key) const {
-        const float d = fminf(value - hh_smp_value(key), 3.4028235e38f) * scale;  // (an infinite T: all in bin 0)
-        return key == top ? 0u : d < 1023.f ? (uint32_t)d : HH_SMP_BINS - 1;
-    }
+    HH_DEV static bool hold(uint32_t top, float temperature) { return top < HH_SMP_KEY_INF && temperature <= 1e30f; }
+    // rounding keeps the order: a lower logit never has a lower bin; fminf drops a NaN
+    HH_DEV uint32_t of(float v) const { return v == value ? 0u : (uint32_t)fminf((value - v) * scale, 1023.f); }
 };
 
 // A token as one number: the row's order is that of falling numbers.
@@ -312,20 +315,42 @@ HH_DEV void hh_smp_part(const hh_sample_args& a, uint32_t& lo, uint32_t& hi) {
     lo = min(a.vocab, blockIdx.x * per * HH_SMP_CHUNK);
     hi = min(a.vocab, lo + per * HH_SMP_CHUNK);
 }
-// f(key, index) for each token of [lo, hi) by `threads` threads, of which this is one.
+// f(eight logits, their indices) over the tokens of [lo, hi) by `threads` threads, of which this is one, the
+// next eight's loads ahead of them.  (-inf past hi.)
 template <class F, class Fn>
 HH_DEV void hh_smp_each(const typename F::E* x, uint32_t lo, uint32_t hi, uint32_t threads, uint32_t thread, Fn f) {
-    constexpr uint32_t VEC = F::VEC;
-    uint32_t i = lo + thread * VEC;
-#pragma unroll 2
-    for (; i + VEC <= hi; i += threads * VEC) {
-        typename F::E v[VEC];
-        hh_load_n(x + i, v);
+    constexpr uint32_t VEC = F::VEC, NV = 8 / VEC;
+    typename F::E now[NV][VEC], next[NV][VEC];
+    auto load = [&](uint32_t base, typename F::E (&v)[NV][VEC]) {
 #pragma unroll
-        for (uint32_t e = 0; e < VEC; e++) f(hh_smp_key(F::get(v[e])), i + e);
+        for (uint32_t j = 0; j < NV; j++) {
+            const uint32_t i = base + (j * threads + thread) * VEC;
+            if (i + VEC <= hi) {
+                hh_load_n(x + i, v[j]);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < VEC; e++) v[j][e] = i + e < hi ? x[i + e] : F::put(-__builtin_inff());
+            }
+        }
+    };
+    if (lo < hi) load(lo, next);
+    for (uint32_t base = lo; base < hi; base += threads * 8) {
+#pragma unroll
+        for (uint32_t j = 0; j < NV; j++)
+#pragma unroll
+            for (uint32_t e = 0; e < VEC; e++) now[j][e] = next[j][e];
+        if (base + threads * 8 < hi) load(base + threads * 8, next);
+        float v[8];
+        uint32_t at[8];
+#pragma unroll
+        for (uint32_t j = 0; j < NV; j++)
+#pragma unroll
+            for (uint32_t e = 0; e < VEC; e++) {
+                v[j * VEC + e] = F::get(now[j][e]);
+                at[j * VEC + e] = base + (j * threads + thread) * VEC + e;
+            }
+        f(v, at);
     }
-    if (i < hi)
-        for (uint32_t e = i; e < hi && e < i + VEC; e++) f(hh_smp_key(F::get(x[e])), e);
 }
 
 template <class F>
@@ -333,13 +358,30 @@ HH_DEV void hh_sample_max(const hh_sample_args& a) {
     __shared__ uint64_t red[HH_SMP_THREADS / HH_WAVE];
     const uint32_t row = blockIdx.y, tid = threadIdx.x;
     const typename F::E* x = (const typename F::E*)a.x + row * a.stride;
-    uint32_t lo, hi, key = 0, at = 0;
+    uint32_t lo, hi;
     hh_smp_part(a, lo, hi);
-    hh_smp_each<F>(x, lo, hi, HH_SMP_THREADS, tid, [&](uint32_t k, uint32_t i) {
-        at = k > key ? i : at;  // a thread's indices ascend
-        key = k > key ? k : key;
+    // the thread's first eight with its largest logit, then which of them it is
+    float most = -__builtin_inff(), eight[8];
+    uint32_t where[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) eight[e] = most, where[e] = 0;
+    hh_smp_each<F>(x, lo, hi, HH_SMP_THREADS, tid, [&](const float (&l)[8], const uint32_t (&at)[8]) {
+        float m = l[0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) m = fmaxf(m, l[e]);  // (drops NaN)
+        if (m > most) {
+            most = m;
+#pragma unroll
+            for (int e = 0; e < 8; e++) eight[e] = l[e], where[e] = at[e];
+        }
     });
-    uint64_t v = hh_smp_max64(hh_smp_entry(key, at));
+    uint64_t v = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const uint64_t o = hh_smp_entry(hh_smp_key(eight[e]), where[e]);
+        v = o > v ? o : v;
+    }
+    v = hh_smp_max64(v);
     if (tid % HH_WAVE == 0) red[tid / HH_WAVE] = v;
     __syncthreads();
     // this part's share of the row's bins and the list's length to zero, for the next launches
@@ -368,27 +410,31 @@ HH_DEV void hh_sample_hist(const hh_sample_args& a) {
     const hh_sample_row_params p = ((const hh_sample_row_params*)a.params)[row];
     if (!(p.temperature > 0.f) || !hh_smp_filters(p, a.vocab)) return;
     const uint32_t top = hh_smp_entry_key(hh_smp_top(a, row));
-    if (top <= HH_SMP_KEY_NINF) return;
+    if (top <= HH_SMP_KEY_NINF || !hh_smp_bins::hold(top, p.temperature)) return;
     for (uint32_t i = tid; i < HH_SMP_BINS; i += HH_SMP_THREADS) {
         mass[i] = 0;
         count[i] = 0;
     }
     __syncthreads();
     const hh_smp_bins bins(top, p.temperature);
+    const hh_smp_weights weights(top, p.temperature);
     uint32_t lo, hi;
     hh_smp_part(a, lo, hi);
-    const bool weigh = p.top_p < 1.f;
-    const hh_smp_weights weights(top, p.temperature);
-    hh_smp_each<F>((const typename F::E*)a.x + row * a.stride, lo, hi, HH_SMP_THREADS, tid, [&](uint32_t key, uint32_t) {
-        const uint32_t b = bins.of(key);
-        if (key <= HH_SMP_KEY_NINF || b == HH_SMP_BINS - 1) return;
-        atomicAdd(&count[b], 1u);
-        if (weigh) atomicAdd(&mass[b], (unsigned long long)hh_smp_mass(weights.of(key)));
+    const bool counts = p.top_k > 0 && (uint32_t)p.top_k < a.vocab, weigh = p.top_p < 1.f;
+    hh_smp_each<F>((const typename F::E*)a.x + row * a.stride, lo, hi, HH_SMP_THREADS, tid,
+                   [&](const float (&l)[8], const uint32_t (&)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t b = bins.of(l[e]);
+            if (b == HH_SMP_BINS - 1) continue;
+            if (counts) atomicAdd(&count[b], 1u);
+            if (weigh) atomicAdd(&mass[b], (unsigned long long)hh_smp_mass(weights.near(l[e])));
+        }
     });
     __syncthreads();
     for (uint32_t i = tid; i < HH_SMP_BINS; i += HH_SMP_THREADS)
-        if (count[i]) {
-            atomicAdd(&a.count[(size_t)row * HH_SMP_BINS + i], count[i]);
+        if (count[i] || mass[i]) {
+            if (counts) atomicAdd(&a.count[(size_t)row * HH_SMP_BINS + i], count[i]);
             if (weigh) atomicAdd((unsigned long long*)&a.mass[(size_t)row * HH_SMP_BINS + i], mass[i]);
         }
 }
@@ -445,14 +491,14 @@ HH_DEV void hh_smp_find_cut(const hh_sample_args& a, uint32_t row, const hh_samp
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < 2; q++) {
-            // the first bin with tokens at which the running weight reaches want
-            const uint64_t before = q ? mb + m0 : mb, here = q ? m1 : m0, n = q ? c1 : c0;
-            const bool first = n && (before == 0 || (double)before < want[0]);
-            if (first && (double)(before + here) >= want[0]) {
+            // the bin at which the running weight reaches want (0 and less: the first)
+            const uint64_t before = q ? mb + m0 : mb, here = q ? m1 : m0;
+            if (here && (before == 0 || (double)before < want[0]) && (double)(before + here) >= want[0]) {
                 cut.plo = 2 * tid + q;
                 cut.pmass = before;
             }
-            if (n && (before == 0 || (double)before < want[1]) && (double)(before + here) >= want[1]) cut.phi = 2 * tid + q;
+            if (here && (before == 0 || (double)before < want[1]) && (double)(before + here) >= want[1])
+                cut.phi = 2 * tid + q;
         }
         __syncthreads();
         if (tid == 0 && cut.plo > cut.kbin) {  // cannot be, but a bin past top-k's end is no end
@@ -477,6 +523,10 @@ HH_DEV void hh_sample_gather(const hh_sample_args& a) {
     if (!(p.temperature > 0.f)) return;
     const uint32_t top = hh_smp_entry_key(hh_smp_top(a, row));
     if (top <= HH_SMP_KEY_NINF) return;
+    if (!hh_smp_bins::hold(top, p.temperature)) {
+        if (blockIdx.x == 0 && tid == 0) a.listed[row] = HH_SMP_LIST + 1;
+        return;
+    }
     if (hh_smp_filters(p, a.vocab)) {
         hh_smp_find_cut(a, row, p, cut, red);
     } else {
@@ -484,7 +534,7 @@ HH_DEV void hh_sample_gather(const hh_sample_args& a) {
         __syncthreads();
     }
     if (blockIdx.x == 0 && tid == 0) ((hh_smp_cut*)a.cut)[row] = cut;
-    const uint32_t kbin = cut.kbin, plo = cut.plo, phi = cut.phi;
+    const uint32_t kbin = cut.kbin, plo = min(cut.plo, HH_SMP_BINS - 1), phi = cut.phi;
     const hh_smp_bins bins(top, p.temperature);
     const hh_smp_weights weights(top, p.temperature);
     const double heavy = p.min_p > 0.f ? (double)p.min_p * HH_SMP_ONE : 0.0;
@@ -493,31 +543,36 @@ HH_DEV void hh_sample_gather(const hh_sample_args& a) {
     __syncthreads();
     uint32_t lo, hi;
     hh_smp_part(a, lo, hi);
-    // a wave takes a chunk
-    for (uint32_t c = lo + tid / HH_WAVE * HH_SMP_CHUNK; c < hi; c += HH_SMP_THREADS / HH_WAVE * HH_SMP_CHUNK) {
+    // a wave takes a run of chunks, one chunk (eight tokens a lane) at a time
+    const uint32_t chunks = (hi - lo + HH_SMP_CHUNK - 1) / HH_SMP_CHUNK, waves = HH_SMP_THREADS / HH_WAVE;
+    const uint32_t per = (chunks + waves - 1) / waves * HH_SMP_CHUNK;
+    const uint32_t wlo = min(hi, lo + tid / HH_WAVE * per), whi = min(hi, wlo + per);
+    static_assert(HH_SMP_CHUNK == 8 * HH_WAVE, "a chunk is a wave's eight tokens a lane");
+    hh_smp_each<F>((const typename F::E*)a.x + row * a.stride, wlo, whi, HH_WAVE, tid % HH_WAVE,
+                   [&](const float (&l)[8], const uint32_t (&at)[8]) {
         uint64_t mine = 0;
-        hh_smp_each<F>((const typename F::E*)a.x + row * a.stride, c, min(hi, c + HH_SMP_CHUNK), HH_WAVE, tid % HH_WAVE,
-                       [&](uint32_t key, uint32_t i) {
-            if (key <= HH_SMP_KEY_NINF) return;
-            const uint32_t b = bins.of(key);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t b = bins.of(l[e]);
             if (b < plo) {
-                const double w = weights.of(key);
-                if (w >= heavy || key == top) mine += hh_smp_mass(w);
-            } else if (b <= phi || b == kbin) {
+                const double w = weights.near(l[e]);
+                if (w >= heavy) mine += hh_smp_mass(w);
+            } else if ((b <= phi && phi < HH_SMP_BINS) || b == kbin) {
                 // into LDS first: a count on a device word takes microseconds
-                const uint32_t at = atomicAdd(&found, 1u);
-                if (at < HH_SMP_STAGE) {
-                    stage[at] = hh_smp_entry(key, i);
+                const uint32_t to = atomicAdd(&found, 1u);
+                const uint64_t entry = hh_smp_entry(hh_smp_key(l[e]), at[e]);
+                if (to < HH_SMP_STAGE) {
+                    stage[to] = entry;
                 } else {
-                    const uint32_t to = atomicAdd(&a.listed[row], 1u);
-                    if (to < HH_SMP_LIST) list[to] = hh_smp_entry(key, i);
+                    const uint32_t past = atomicAdd(&a.listed[row], 1u);
+                    if (past < HH_SMP_LIST) list[past] = entry;
                 }
             }
-        });
+        }
 #pragma unroll
         for (int off = 32; off; off >>= 1) mine += __shfl_xor(mine, off, HH_WAVE);
-        if (tid % HH_WAVE == 0) a.sure[(size_t)row * a.chunks + c / HH_SMP_CHUNK] = mine;
-    }
+        if (tid % HH_WAVE == 0) a.sure[(size_t)row * a.chunks + at[0] / HH_SMP_CHUNK] = mine;
+    });
     __syncthreads();
     const uint32_t n = min(found, HH_SMP_STAGE);
     if (n == 0) return;
@@ -620,7 +675,7 @@ HH_DEV uint64_t hh_smp_end_select(const uint64_t* list, uint32_t n, const hh_sam
         v[i] = at < n ? list[at] : 0;
     }
     if (cut.kbin < HH_SMP_BINS) {
-        auto in_k = [&](uint64_t e) { return e && bins.of(hh_smp_entry_key(e)) == cut.kbin; };
+        auto in_k = [&](uint64_t e) { return e && bins.of(hh_smp_value(hh_smp_entry_key(e))) == cut.kbin; };
         last = hh_smp_list_cut(v, (double)cut.kneed, in_k, [](uint64_t) { return 1ull; }, s, before);
     }
     if (!(p.top_p < 1.f)) return last;
@@ -628,7 +683,7 @@ HH_DEV uint64_t hh_smp_end_select(const uint64_t* list, uint32_t n, const hh_sam
     if (cut.kbin < HH_SMP_BINS) {
 #pragma unroll
         for (uint32_t i = 0; i < HH_SMP_EACH; i++)
-            if (v[i] && v[i] >= last && bins.of(hh_smp_entry_key(v[i])) == cut.kbin) kept += weigh(v[i]);
+            if (v[i] && v[i] >= last && bins.of(hh_smp_value(hh_smp_entry_key(v[i]))) == cut.kbin) kept += weigh(v[i]);
         kept = hh_smp_scan(kept, s);
         __syncthreads();
         if (threadIdx.x == HH_SMP_BLOCK - 1) s.found = kept;
@@ -637,7 +692,7 @@ HH_DEV uint64_t hh_smp_end_select(const uint64_t* list, uint32_t n, const hh_sam
     }
     const double want = (double)p.top_p * (double)(cut.kmass + kept);
     const uint64_t klast = last;
-    auto in_p = [&](uint64_t e) { return e && e >= klast && bins.of(hh_smp_entry_key(e)) <= cut.phi; };
+    auto in_p = [&](uint64_t e) { return e && e >= klast && bins.of(hh_smp_value(hh_smp_entry_key(e))) <= cut.phi; };
     return hh_smp_list_cut(v, want - (double)cut.pmass, in_p, weigh, s, before);
 }
 
@@ -665,7 +720,7 @@ HH_DEV uint64_t hh_smp_end_sorted(const uint64_t* list, uint32_t n, const hh_sam
             e = (o > e) == keep_large ? o : e;
         }
     const uint64_t m = e ? weigh(e) : 0, run = hh_smp_scan(m, s);
-    const uint32_t bin = e ? bins.of(hh_smp_entry_key(e)) : HH_SMP_BINS;
+    const uint32_t bin = e ? bins.of(hh_smp_value(hh_smp_entry_key(e))) : HH_SMP_BINS;
     // entries of kbin follow those of lower bins: its first entry, then the last that top-k keeps
     __syncthreads();
     s.sort[tid] = (uint64_t)bin;

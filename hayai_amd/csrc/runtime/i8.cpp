@@ -139,7 +139,7 @@ hh_status hh_engine::enqueue_sample(int type, size_t rows, hh_sample_args a) {
     a.chunks = (uint32_t)((a.vocab + kSmpChunk - 1) / kSmpChunk);
     // parts of 4096 tokens or more, and no more than fill the chip twice
     a.parts = (uint32_t)std::max<size_t>(
-        1, std::min<size_t>((a.vocab + 4095) / 4096, (2 * (size_t)props.multiProcessorCount + pass - 1) / pass));
+        1, std::min<size_t>((a.vocab + 4095) / 4096, (4 * (size_t)props.multiProcessorCount + pass - 1) / pass));
     const size_t row_bytes = 8 * (a.parts + kSmpBins + a.chunks + kSmpList) + 4 * kSmpBins + kSmpCutBytes + 4;
     HH_TRY(grow(&ws_smp, &ws_smp_cap, pass * row_bytes));
     a.top = (uint64_t*)ws_smp;
