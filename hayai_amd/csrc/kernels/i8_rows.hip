@@ -15,50 +15,17 @@
 // One workgroup per row, the row in registers between the two phases (CH chunks of 16 bytes a
 // thread); rows of more than 2048 chunks are read twice (hh_i8_rows_<...>_loop).
 #include "act_types.h"
+#include "wave64.h"
 
-template <int CTRL, int ROWS = 0xf>
-HH_DEV uint64_t hh_i8_dpp64(uint64_t v) {
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, true);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, true);
-    return (uint64_t)hi << 32 | lo;
-}
-HH_DEV uint64_t hh_i8_lane64(uint64_t v, int lane) {
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
-    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
-    return (uint64_t)hi << 32 | lo;
-}
-struct hh_i8_max64 {
-    HH_DEV static uint64_t of(uint64_t a, uint64_t b) { return b > a ? b : a; }
-};
-struct hh_i8_add64 {
-    HH_DEV static uint64_t of(uint64_t a, uint64_t b) {
-        return (uint64_t)__double_as_longlong(__longlong_as_double((long long)a) + __longlong_as_double((long long)b));
-    }
-};
-// Op over each row of 16 lanes, then over the wave (in lane 63).  Zero is neutral to both.
-template <class Op>
-HH_DEV uint64_t hh_i8_row16(uint64_t v) {
-    v = Op::of(v, hh_i8_dpp64<0xB1>(v));
-    v = Op::of(v, hh_i8_dpp64<0x4E>(v));
-    v = Op::of(v, hh_i8_dpp64<0x124>(v));
-    return Op::of(v, hh_i8_dpp64<0x128>(v));
-}
-template <class Op>
-HH_DEV uint64_t hh_i8_wave64(uint64_t v) {
-    v = hh_i8_row16<Op>(v);
-    v = Op::of(v, hh_i8_dpp64<0x142, 0xa>(v));
-    v = Op::of(v, hh_i8_dpp64<0x143, 0xc>(v));
-    return hh_i8_lane64(v, 63);
-}
 // Op over the workgroup of up to 16 waves; red: 16 words of LDS not read since the last meeting.
 template <class Op>
 HH_DEV uint64_t hh_i8_block64(uint64_t v, uint64_t* red) {
-    v = hh_i8_wave64<Op>(v);
+    v = hh_wave64<Op>(v);
     const uint32_t waves = blockDim.x / HH_WAVE, lane = threadIdx.x % HH_WAVE;
     if (waves == 1) return v;
     if (lane == 0) red[threadIdx.x / HH_WAVE] = v;
     __syncthreads();
-    return hh_i8_lane64(hh_i8_row16<Op>(lane < waves ? red[lane] : 0), 0);
+    return hh_lane64(hh_row16<Op>(lane < waves ? red[lane] : 0), 0);
 }
 struct hh_i8_red {
     uint64_t top[16], ss[16];
@@ -69,14 +36,14 @@ struct hh_i8_red {
 template <bool SUM>
 HH_DEV void hh_i8_reduce(uint64_t& top, double& ss, hh_i8_red& red) {
     if (SUM) {
-        const uint64_t s = hh_i8_wave64<hh_i8_add64>((uint64_t)__double_as_longlong(ss));
+        const uint64_t s = hh_wave64<hh_addf64>((uint64_t)__double_as_longlong(ss));
         if (threadIdx.x % HH_WAVE == 0) red.ss[threadIdx.x / HH_WAVE] = s;
         ss = __longlong_as_double((long long)s);
     }
-    top = hh_i8_block64<hh_i8_max64>(top, red.top);  // meets
+    top = hh_i8_block64<hh_max64>(top, red.top);  // meets
     const uint32_t waves = blockDim.x / HH_WAVE, lane = threadIdx.x % HH_WAVE;
     if (SUM && waves > 1)
-        ss = __longlong_as_double((long long)hh_i8_lane64(hh_i8_row16<hh_i8_add64>(lane < waves ? red.ss[lane] : 0), 0));
+        ss = __longlong_as_double((long long)hh_lane64(hh_row16<hh_addf64>(lane < waves ? red.ss[lane] : 0), 0));
 }
 
 enum { HH_I8_PLAIN, HH_I8_ACT, HH_I8_NORM };
@@ -325,7 +292,7 @@ HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
         return hh_i8_act((double)F::get(row.x[e]), (double)F::get(row.b[e]), a.act);
     };
     // the 64-bit magnitude of whatever may be the largest: |h| (1 +- FAR) holds it
-    const float top32 = __uint_as_float((uint32_t)hh_i8_block64<hh_i8_max64>(seen, red[0]));
+    const float top32 = __uint_as_float((uint32_t)hh_i8_block64<hh_max64>(seen, red[0]));
     const bool wide = !(top32 >= 1e-25f && top32 <= 1e25f);
     const float least = top32 * (1.f - 2.f * FAR);
     uint32_t todo = far;
@@ -341,7 +308,7 @@ HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
         const uint64_t m = (uint64_t)__double_as_longlong(v) & 0x7fffffffffffffffull;
         bits = m > bits ? m : bits;
     }
-    bits = hh_i8_block64<hh_i8_max64>(bits, red[1]);
+    bits = hh_i8_block64<hh_max64>(bits, red[1]);
     double top, inv;
     const float scale = hh_i8_factors<HH_I8_ACT>(a, bits, 0.0, top, inv);
     const float inv32 = scale > 0.f && !wide ? (float)inv : 0.f;  // 0: codes 0 until recomputed

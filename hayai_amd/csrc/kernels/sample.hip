@@ -17,6 +17,7 @@
 // A row whose list passes 8192 tokens (nearly equal logits throughout), whose largest logit is infinite or
 // whose T is past 1e30 is done by one workgroup from the logits (hh_sample_row).
 #include "act_types.h"
+#include "wave64.h"
 
 struct hh_sample_row_params {
     float temperature;
@@ -80,20 +81,7 @@ struct hh_smp_lds {
     uint32_t digit, top;
 };
 
-// Inclusive sums over the workgroup's threads in thread order.
-HH_DEV uint64_t hh_smp_scan(uint64_t v, hh_smp_lds& s) {
-    const uint32_t lane = threadIdx.x % HH_WAVE, w = threadIdx.x / HH_WAVE;
-#pragma unroll
-    for (int off = 1; off < HH_WAVE; off <<= 1) {
-        const uint64_t o = __shfl_up(v, off, HH_WAVE);
-        if (lane >= (uint32_t)off) v += o;
-    }
-    __syncthreads();
-    if (lane == HH_WAVE - 1) s.wave[w] = v;
-    __syncthreads();
-    for (uint32_t i = 0; i < w; i++) v += s.wave[i];
-    return v;
-}
+HH_DEV uint64_t hh_smp_scan(uint64_t v, hh_smp_lds& s) { return hh_block_scan64(v, s.wave); }
 
 // The key at which the running amount, from the largest key down over keys > floor, first reaches
 // want: amount(key) a token.  before: the amount of the keys above it.  Returns 0 where the whole
@@ -292,14 +280,6 @@ HH_DEV uint32_t hh_smp_entry_index(uint64_t e) {
     return mask - ((uint32_t)e & mask);
 }
 
-HH_DEV uint64_t hh_smp_max64(uint64_t v) {
-#pragma unroll
-    for (int off = 32; off; off >>= 1) {
-        const uint64_t o = __shfl_xor(v, off, HH_WAVE);
-        v = o > v ? o : v;
-    }
-    return v;
-}
 // The row's first token, from the parts'.
 HH_DEV uint64_t hh_smp_top(const hh_sample_args& a, uint32_t row) {
     uint64_t v = 0;
@@ -307,7 +287,7 @@ HH_DEV uint64_t hh_smp_top(const hh_sample_args& a, uint32_t row) {
         const uint64_t o = a.top[(size_t)row * a.parts + i];
         v = o > v ? o : v;
     }
-    return hh_smp_max64(v);
+    return hh_wave64<hh_max64>(v);
 }
 // The tokens [lo, hi) of this workgroup's part.
 HH_DEV void hh_smp_part(const hh_sample_args& a, uint32_t& lo, uint32_t& hi) {
@@ -381,7 +361,7 @@ HH_DEV void hh_sample_max(const hh_sample_args& a) {
         const uint64_t o = hh_smp_entry(hh_smp_key(eight[e]), where[e]);
         v = o > v ? o : v;
     }
-    v = hh_smp_max64(v);
+    v = hh_wave64<hh_max64>(v);
     if (tid % HH_WAVE == 0) red[tid / HH_WAVE] = v;
     __syncthreads();
     // this part's share of the row's bins and the list's length to zero, for the next launches
@@ -439,21 +419,6 @@ HH_DEV void hh_sample_hist(const hh_sample_args& a) {
         }
 }
 
-// Inclusive sums over the workgroup's threads in thread order; red: a word a wave.
-HH_DEV uint64_t hh_smp_scan_block(uint64_t v, uint64_t* red) {
-    const uint32_t lane = threadIdx.x % HH_WAVE, w = threadIdx.x / HH_WAVE;
-#pragma unroll
-    for (int off = 1; off < HH_WAVE; off <<= 1) {
-        const uint64_t o = __shfl_up(v, off, HH_WAVE);
-        if (lane >= (uint32_t)off) v += o;
-    }
-    __syncthreads();
-    if (lane == HH_WAVE - 1) red[w] = v;
-    __syncthreads();
-    for (uint32_t i = 0; i < w; i++) v += red[i];
-    return v;
-}
-
 // The bins in which the filters end, from the row's sums: the same in every workgroup of the row.
 HH_DEV void hh_smp_find_cut(const hh_sample_args& a, uint32_t row, const hh_sample_row_params& p, hh_smp_cut& cut,
                             uint64_t* red) {
@@ -462,8 +427,8 @@ HH_DEV void hh_smp_find_cut(const hh_sample_args& a, uint32_t row, const hh_samp
     if (tid == 0) cut = hh_smp_cut{HH_SMP_BINS, HH_SMP_BINS, HH_SMP_BINS, 0, 0, 0};
     const size_t at = (size_t)row * HH_SMP_BINS + 2 * tid;
     const uint64_t c0 = a.count[at], c1 = a.count[at + 1], m0 = a.mass[at], m1 = a.mass[at + 1];
-    const uint64_t cs = hh_smp_scan_block(c0 + c1, red), cb = cs - c0 - c1;  // (meets: cut is set)
-    const uint64_t ms = hh_smp_scan_block(m0 + m1, red), mb = ms - m0 - m1;
+    const uint64_t cs = hh_block_scan64(c0 + c1, red), cb = cs - c0 - c1;  // (meets: cut is set)
+    const uint64_t ms = hh_block_scan64(m0 + m1, red), mb = ms - m0 - m1;
     const bool topk = p.top_k > 0 && (uint32_t)p.top_k < a.vocab;
     if (topk) {
         const uint64_t k = (uint32_t)p.top_k;
@@ -516,7 +481,7 @@ HH_DEV void hh_smp_find_cut(const hh_sample_args& a, uint32_t row, const hh_samp
 template <class F>
 HH_DEV void hh_sample_gather(const hh_sample_args& a) {
     __shared__ hh_smp_cut cut;
-    __shared__ uint64_t red[HH_SMP_THREADS / HH_WAVE], stage[HH_SMP_STAGE];
+    __shared__ uint64_t red[16], stage[HH_SMP_STAGE];
     __shared__ uint32_t found, base;
     const uint32_t row = blockIdx.y, tid = threadIdx.x;
     const hh_sample_row_params p = ((const hh_sample_row_params*)a.params)[row];
@@ -569,8 +534,7 @@ HH_DEV void hh_sample_gather(const hh_sample_args& a) {
                 }
             }
         }
-#pragma unroll
-        for (int off = 32; off; off >>= 1) mine += __shfl_xor(mine, off, HH_WAVE);
+        mine = hh_wave64<hh_addu64>(mine);
         if (tid % HH_WAVE == 0) a.sure[(size_t)row * a.chunks + at[0] / HH_SMP_CHUNK] = mine;
     });
     __syncthreads();
@@ -640,13 +604,7 @@ HH_DEV uint64_t hh_smp_list_cut(const uint64_t (&v)[HH_SMP_EACH], double want, T
             uint64_t h[4], sum = 0;
 #pragma unroll
             for (int q = 0; q < 4; q++) sum += h[q] = s.hist[d0 - q];
-            uint64_t run = sum;
-#pragma unroll
-            for (int off = 1; off < HH_WAVE; off <<= 1) {
-                const uint64_t o = __shfl_up(run, off, HH_WAVE);
-                if ((int)threadIdx.x >= off) run += o;
-            }
-            run += above - sum;
+            uint64_t run = hh_scan64(sum) + above - sum;
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 if (h[q] && (run == 0 || (double)run < want) && (double)(run + h[q]) >= want) {
