@@ -48,6 +48,14 @@ HH_DEV void hh_i8_reduce(uint64_t& top, double& ss, hh_i8_red& red) {
 
 enum { HH_I8_PLAIN, HH_I8_ACT, HH_I8_NORM };
 
+// How many of the elements e..e+VEC lie in the row (e + VEC stays under 2^32).  Neither difference can
+// wrap.  With e >= cols ? 0 : min(VEC, cols - e) the compiler computed cols - e in every lane as a
+// subtraction that does not wrap, concluded e <= cols, and dropped the tests that guard the stores.
+template <int VEC>
+HH_DEV uint32_t hh_i8_count(uint32_t e, uint32_t cols) {
+    return min(cols, e + VEC) - min(cols, e);
+}
+
 // SiLU(g) * u or tanh-GELU(g) * u; 1 + tanh(y) as 2 / (1 + exp(-2 y)).
 HH_DEV double hh_i8_act(double g, double u, int act) {
     if (act == HH_ACT_GELU_TANH) {
@@ -167,7 +175,7 @@ HH_DEV void hh_i8_rows_regs(const hh_i8_rows_args& a) {
 #pragma unroll
     for (int c = 0; c < CH; c++) {
         const uint32_t e = (c * blockDim.x + threadIdx.x) * VEC;
-        const uint32_t count = e >= a.cols ? 0u : min((uint32_t)VEC, a.cols - e);
+        const uint32_t count = hh_i8_count<VEC>(e, a.cols);
         double v[VEC];
         row.load(e, u[c], v, count);
         if (KIND == HH_I8_NORM && row.sum && count) row.store_sum(e, v, count);
@@ -186,8 +194,7 @@ HH_DEV void hh_i8_rows_regs(const hh_i8_rows_args& a) {
 #pragma unroll
     for (int c = 0; c < CH; c++) {
         const uint32_t e = (c * blockDim.x + threadIdx.x) * VEC;
-        const uint32_t count = e >= a.cols ? 0u : min((uint32_t)VEC, a.cols - e);
-        if (!count) break;
+        const uint32_t count = hh_i8_count<VEC>(e, a.cols);
         if (zero) {
 #pragma unroll
             for (int i = 0; i < VEC; i++) u[c][i] = 0.0;
@@ -253,8 +260,7 @@ HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
     __shared__ uint64_t red[2][16];
     const hh_i8_row<F, HH_I8_ACT> row(a, blockIdx.x);
     auto count = [&](int c) {
-        const uint32_t e = (c * blockDim.x + threadIdx.x) * VEC;
-        return e >= a.cols ? 0u : min((uint32_t)VEC, a.cols - e);
+        return hh_i8_count<VEC>((c * blockDim.x + threadIdx.x) * VEC, a.cols);
     };
     E g[CH][VEC];
     float h[CH][VEC];

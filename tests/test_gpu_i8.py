@@ -501,3 +501,46 @@ def test_wrapped_memory(engine):
                                 engine.alloc(64), 0)
     finally:
         other.close()
+
+
+# Rows enough to fill the chip twice: a workgroup of few threads with four chunks a thread, whose last
+# chunks lie partly or wholly past the row.  One element; inside, at and past a chunk of 64 threads; in
+# the third chunk; full; two waves.
+MANY = [1, 5, 89, 255, 257, 577, 1000, 1024, 1029, 2500, 4099]
+SLACK = 1 << 16
+
+
+@pytest.mark.parametrize("kind", ["plain", "act", "norm"])
+@pytest.mark.parametrize("ty", TYPES)
+def test_many_rows(engine, ty, kind):
+    rows = 2 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+    size = torch.empty(0, dtype=DT[ty]).element_size()
+    for k, cols in enumerate(MANY):
+        print(f"[case] many {kind} type={ty} {rows}x{cols}", flush=True)
+        wide = kind == "act"
+        x = normal(200 + k, rows, 2 * cols if wide else cols, scale=2.0).to(DT[ty])
+        w = (normal(300 + k, cols) + 1.0).float()
+        bx, bw = put(engine, x), put(engine, w)
+        q, s, v = engine.alloc(rows * cols + SLACK), engine.alloc(4 * rows), engine.alloc(4 * rows * cols + SLACK)
+        o = engine.alloc(rows * cols * size + SLACK)
+        for b in (q, s, v, o):
+            b.fill(0x5B)
+        u, unit = f64(x), 1.0
+        if kind == "norm":
+            d = engine.rms_norm_i8_desc(ty, rows, cols, EPS)
+            engine.rms_norm_i8_dev(d, bx, 0, bx, 0, bw, 0, o, 0, q, 0, s, 0, v, 0)
+            u = 2.0 * u
+            assert torch.equal(get(o, DT[ty], (rows, cols)), torch.from_numpy(u).to(DT[ty]))
+            unit = 1.0 / np.sqrt((u**2).mean(1, keepdims=True) + EPS)
+            u = u * f64(w)
+        elif wide:
+            d = engine.quant_i8_desc(ty, rows, cols, x_stride=2 * cols, up_stride=2 * cols)
+            engine.quant_i8_dev(d, bx, 0, bx, cols * size, q, 0, s, 0, v, 0)
+            u = act64(u[:, :cols], u[:, cols:], hayai_amd.ACT_SILU)
+        else:
+            engine.quant_i8_dev(engine.quant_i8_desc(ty, rows, cols), bx, 0, None, 0, q, 0, s, 0, v, 0)
+        check_codes(q.read(np.int8, rows * cols).reshape(rows, cols), s.read(np.float32, rows),
+                    v.read(np.float32, rows * cols).reshape(rows, cols), *codes_of(u, unit))
+        assert np.all(q.read(np.uint8, SLACK, rows * cols) == 0x5B)
+        assert np.all(v.read(np.uint8, SLACK, 4 * rows * cols) == 0x5B)
+        assert np.all(o.read(np.uint8, SLACK, rows * cols * size if kind == "norm" else 0) == 0x5B)
