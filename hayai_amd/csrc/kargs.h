@@ -95,10 +95,9 @@ struct hh_i8_rows_args {
     float* scale;
     float* values;
     uint64_t x_stride, b_stride, sum_stride, q_stride;
-    uint32_t cols;
+    uint32_t rows, cols;
     int32_t act;
     float eps;
-    uint32_t pad;
 };
 
 // y[t][r] = sum_k x[t][k] w[r][k] * xs[t] * ws[r] (+ res[t][r]) over codes (i8_gemm.hip);

@@ -37,7 +37,7 @@ template <bool SUM>
 HH_DEV void hh_i8_reduce(uint64_t& top, double& ss, hh_i8_red& red) {
     if (SUM) {
         const uint64_t s = hh_wave64<hh_addf64>((uint64_t)__double_as_longlong(ss));
-        if (threadIdx.x % HH_WAVE == 0) red.ss[threadIdx.x / HH_WAVE] = s;
+        if (threadIdx.x % HH_WAVE == 0 && blockDim.x > HH_WAVE) red.ss[threadIdx.x / HH_WAVE] = s;
         ss = __longlong_as_double((long long)s);
     }
     top = hh_i8_block64<hh_max64>(top, red.top);  // meets
@@ -165,11 +165,19 @@ HH_DEV float hh_i8_factors(const hh_i8_rows_args& a, uint64_t bits, double ss, d
     return scale;
 }
 
+// The row of this wave: a workgroup has blockDim.y rows where one wave holds a row, else one.
+HH_DEV bool hh_i8_my_row(const hh_i8_rows_args& a, uint32_t& r) {
+    r = blockIdx.x * blockDim.y + __builtin_amdgcn_readfirstlane(threadIdx.y);
+    return r < a.rows;
+}
+
 template <class F, int KIND, int CH>
 HH_DEV void hh_i8_rows_regs(const hh_i8_rows_args& a) {
+    uint32_t r;
+    if (!hh_i8_my_row(a, r)) return;
     constexpr int VEC = F::VEC;
     __shared__ hh_i8_red red;
-    const hh_i8_row<F, KIND> row(a, blockIdx.x);
+    const hh_i8_row<F, KIND> row(a, r);
     double u[CH][VEC], ss = 0.0;
     uint64_t bits = 0;
 #pragma unroll
@@ -190,7 +198,7 @@ HH_DEV void hh_i8_rows_regs(const hh_i8_rows_args& a) {
     double top, inv;
     const float scale = hh_i8_factors<KIND>(a, bits, ss, top, inv);
     const bool zero = !(scale > 0.f);
-    if (threadIdx.x == 0) a.scale[blockIdx.x] = scale;
+    if (threadIdx.x == 0) a.scale[r] = scale;
 #pragma unroll
     for (int c = 0; c < CH; c++) {
         const uint32_t e = (c * blockDim.x + threadIdx.x) * VEC;
@@ -253,12 +261,14 @@ HH_DEV float hh_i8_act32_error(float y) { return (8.f * fmaxf(-y, 0.f) + 36.f) *
 
 template <class F, int CH>
 HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
+    uint32_t r;
+    if (!hh_i8_my_row(a, r)) return;
     typedef typename F::E E;
     constexpr int VEC = F::VEC;
     static_assert(CH * VEC <= 32, "a bit for each element of a thread");
     constexpr float FAR = (8.f * 80.f + 36.f) * 0x1p-24f;  // the error bound at y = -80
     __shared__ uint64_t red[2][16];
-    const hh_i8_row<F, HH_I8_ACT> row(a, blockIdx.x);
+    const hh_i8_row<F, HH_I8_ACT> row(a, r);
     auto count = [&](int c) {
         return hh_i8_count<VEC>((c * blockDim.x + threadIdx.x) * VEC, a.cols);
     };
@@ -318,7 +328,7 @@ HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
     double top, inv;
     const float scale = hh_i8_factors<HH_I8_ACT>(a, bits, 0.0, top, inv);
     const float inv32 = scale > 0.f && !wide ? (float)inv : 0.f;  // 0: codes 0 until recomputed
-    if (threadIdx.x == 0) a.scale[blockIdx.x] = scale;
+    if (threadIdx.x == 0) a.scale[r] = scale;
     todo = far;
 #pragma unroll
     for (int c = 0; c < CH; c++) {

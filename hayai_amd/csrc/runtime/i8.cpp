@@ -27,18 +27,27 @@ void i8_kernels(std::vector<std::string>& k) {
 
 using namespace hh;
 
-hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_args& a) {
+hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, hh_i8_rows_args a) {
     const ActType* ty = act_type(type);
     const size_t chunks = (a.cols * ty->bytes + 15) / 16;
-    // Few rows: as many threads as chunks, for latency.  Rows enough to fill the chip twice: four chunks a
-    // thread, so that a CU holds more rows and asks for more of them at once.
+    // Few rows: as many threads as chunks, for latency.  Rows enough to fill the chip twice: up to four
+    // chunks a thread, so that a CU holds more rows and asks for more of them at once; and where one wave
+    // holds a row, four rows a workgroup (7178 rows of 208 f16: 8.2 us, one a workgroup with four chunks a
+    // thread 19.1, eight a workgroup 8.4; 13527 of 1076: 22.0, 32.1, 22.3).
     const bool many = rows >= 2 * (size_t)props.multiProcessorCount && chunks <= 2048;
     const size_t threads = std::min<size_t>(1024, ((many ? (chunks + 3) / 4 : chunks) + 63) / 64 * 64);
     const char* kind = a.norm ? "norm" : a.b ? "act" : "plain";
-    const char* v = many ? "c4" : chunks <= threads ? "c1" : chunks <= 2 * threads ? "c2" : "loop";
+    const size_t each = (chunks + threads - 1) / threads;
+    const char* v = each <= 1 ? "c1" : each <= 2 ? "c2" : many ? "c4" : "loop";
+    const size_t per = many && threads == 64 ? 4 : 1;
+    a.rows = (uint32_t)rows;
     hipFunction_t f;
     HH_TRY(kernel(std::string("hh_i8_rows_") + ty->name + "_" + kind + "_" + v, &f));
-    return launch(f, (uint32_t)rows, (uint32_t)threads, a);
+    void* params[] = {&a};
+    HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)((rows + per - 1) / per), 1, 1, (uint32_t)threads, (uint32_t)per, 1, 0,
+                                     stream, params, nullptr),
+               "hipModuleLaunchKernel(i8 rows)");
+    return HH_OK;
 }
 
 // Which form, by the weights' bytes, the tokens and the tiles (28672 x 4096, 4096 x 14336, 4096 x 4096,
@@ -48,7 +57,9 @@ hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_arg
 //     6.9; 32000 x 2048 15.8, 17.3; 4096 x 14336 14.3, 12.8); up to eight under 4 MB of weights
 //     (576 x 1536 4.0, 7.2; 4096 x 4096 8.4, 6.9)
 //   tiles of 32 x 32 to 32 tokens (28672 x 4096, 32 tokens: 29.4, of 64 x 64 30.9), and to 64 where 64-row
-//     tiles are few (4096 x 14336, 61 tokens: 15.0, 16.3; 28672 x 4096, 64 tokens: 40.8, 32.5)
+//     tiles are few (4096 x 14336, 61 tokens: 15.0, 16.3; 28672 x 4096, 64 tokens: 40.8, 32.5), and where
+//     64 x 64 tiles would not give every other CU one (1000 x 2048, 100 tokens: 5.7, 8.9; 512 x 4096, 200:
+//     8.0, 8.9; with 256 of them, 4096 x 4096, 200: 17.5, 10.3)
 //   past that the least of the estimates below.
 struct I8Big {
     const char* name;
@@ -81,7 +92,7 @@ hh_status hh_engine::enqueue_i8_gemm(int type, hh_i8_gemm_args a) {
     }
     auto tiles = [&](size_t tm, size_t tn) { return (a.m + tm - 1) / tm * ((a.t + tn - 1) / tn); };
     size_t tm = 64;  // the small tiles' side
-    if (a.t <= 32 || (a.t <= 64 && a.m < 8192)) tm = 32;
+    if (a.t <= 32 || (a.t <= 64 && a.m < 8192) || 2 * tiles(64, 64) <= cus) tm = 32;
     if (a.t > 64) {
         const I8Big* best = nullptr;
         double least = 6 + 0.27 * (double)(tiles(64, 64) * stages) / (double)cus;
@@ -107,11 +118,11 @@ hh_status hh_engine::enqueue_i8_gemm(int type, hh_i8_gemm_args a) {
     a.ttiles = (uint32_t)((a.t + tm - 1) / tm);
     const size_t n = (size_t)a.mtiles * a.ttiles, units = n * stages;
     if (n > UINT32_MAX / 2) return fail(HH_ERR_INVALID, "gemm_i8: %u x %u outputs are too many", a.t, a.m);
-    // workgroups, each at least a stage: two a CU where that cuts few tiles (28672 x 4096, 32 tokens, 896
+    // workgroups, each a tile or two stages at least: two a CU where that cuts few tiles (28672 x 4096, 32 tokens, 896
     // tiles: 29.4, one a CU 35.6; 4096 x 14336, 32 tokens, 128 tiles: 14.4, 13.2)
     size_t W = n >= (tm == 32 ? 1 : 2) * cus ? 2 * cus : cus;
-    W = std::max<size_t>(1, std::min(W, units / 2));
-    W = W >= 8 ? W / 8 * 8 : 1;
+    W = std::min(W, std::max(n, units / 2));
+    W = W >= 8 ? W / 8 * 8 : W;
     HH_TRY(grow(&ws_part, &ws_part_cap, W * 2 * tm * tm * sizeof(int)));
     if (ws_cnt_cap < n * sizeof(uint32_t)) {
         HH_TRY(grow(&ws_cnt, &ws_cnt_cap, n * sizeof(uint32_t)));

@@ -194,7 +194,8 @@ def codes(seed, rows, n, stride):
     return torch.from_numpy(c), c[:, :n].astype(np.int64)
 
 
-def run_gemm(engine, ty, m, n, t, wpad=0, xpad=0, ypad=0, res=False, in_place=False, seed=0, w=None, x=None):
+def run_gemm(engine, ty, m, n, t, wpad=0, xpad=0, ypad=0, res=False, in_place=False, seed=0, w=None, x=None,
+             behind=0):
     ws, xs = (n + 15) // 16 * 16 + wpad, (n + 15) // 16 * 16 + xpad
     wt, w64 = codes(seed, m, n, ws) if w is None else w
     xt, x64 = codes(seed + 1, t, n, xs) if x is None else x
@@ -202,12 +203,14 @@ def run_gemm(engine, ty, m, n, t, wpad=0, xpad=0, ypad=0, res=False, in_place=Fa
     sx = (normal(seed + 3, t).abs() * 0.01 + 1e-3).float()
     ys = m + ypad
     r = (normal(seed + 4, t, ys) * np.sqrt(n) * 0.5).to(DT[ty])
-    y0 = r if in_place else torch.full((t, ys), 7.0, dtype=DT[ty])
+    y0 = r if in_place else torch.full((t + behind, ys), 7.0, dtype=DT[ty])
     by = put(engine, y0)
     br = by if in_place else put(engine, r) if res else None
     d = engine.gemm_i8_desc(ty, m, n, t, w_stride=ws, x_stride=xs, res_stride=ys, y_stride=ys)
     engine.gemm_i8_dev(d, put(engine, wt), 0, put(engine, sw), 0, put(engine, xt), 0, put(engine, sx), 0, br, 0, by, 0)
-    got = get(by, DT[ty], (t, ys))
+    got = get(by, DT[ty], (t + behind, ys))
+    assert torch.equal(got[t:], y0[t:])  # rows behind the last token's are left as they were
+    got, y0 = got[:t], y0[:t]
     assert torch.equal(got[:, m:], y0[:, m:])
     # whole numbers below 2^53 in float64: exact
     prod = (x64.astype(np.float64) @ w64.astype(np.float64).T) * f64(sx)[:, None] * f64(sw)
@@ -544,3 +547,22 @@ def test_many_rows(engine, ty, kind):
         assert np.all(q.read(np.uint8, SLACK, rows * cols) == 0x5B)
         assert np.all(v.read(np.uint8, SLACK, 4 * rows * cols) == 0x5B)
         assert np.all(o.read(np.uint8, SLACK, rows * cols * size if kind == "norm" else 0) == 0x5B)
+
+
+@pytest.mark.parametrize("ty", TYPES)
+def test_gemm_leaves_rows_behind(engine, ty):
+    """Each small form, with an output that goes on behind the last token; a tile cut into one to many
+    workgroups; fewer tiles than workgroups of an XCD."""
+    for k, (m, n, t) in enumerate([(100, 1000, 1), (9, 40, 3), (1001, 577, 7), (33, 16327, 9), (102, 16327, 64),
+                                   (40, 131071, 17), (71, 93, 185), (300, 300, 300), (1667, 1040, 515)]):
+        print(f"[case] behind type={ty} m={m} n={n} t={t}", flush=True)
+        run_gemm(engine, ty, m, n, t, xpad=16 * (k % 2), ypad=k % 3, res=k % 2 == 1, seed=700 + 10 * k, behind=300)
+
+
+# Each form of whole tiles (128x128, 128x256, 192x256, 256x256) with ragged edges, then several tiles a
+# workgroup one after the other.
+@pytest.mark.parametrize("ty,m,n,t", [(BF16, 11657, 1040, 515), (F16, 4997, 577, 1500), (F32, 7661, 577, 1500),
+                                      (BF16, 9993, 577, 1501), (F16, 23457, 1040, 600), (BF16, 5991, 577, 4003),
+                                      (F32, 20462, 577, 1500), (F16, 20462, 577, 1500)])
+def test_gemm_large(engine, ty, m, n, t):
+    run_gemm(engine, ty, m, n, t, wpad=16, ypad=1, res=ty == BF16, seed=m, behind=260)
