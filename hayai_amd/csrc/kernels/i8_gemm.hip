@@ -399,7 +399,7 @@ HH_DEV void hh_i8_big(const hh_i8_gemm_args& a) {
     if (tile >= tiles) return;
 
     const uint32_t lrow = lane / 8, c0 = ((lane % 8) ^ (lane / 16)) * 16;
-    uint32_t woff[LW], xoff[LX];
+    uint32_t woff[LW], xoff[LX];  // 255 strides of 2^24 and a row of codes stay below 2^32
     const int8_t *wbase, *xbase;
     uint32_t m0, t0;
     auto place = [&]() {

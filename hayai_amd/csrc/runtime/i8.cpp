@@ -93,7 +93,8 @@ hh_status hh_engine::enqueue_i8_gemm(int type, hh_i8_gemm_args a) {
     auto tiles = [&](size_t tm, size_t tn) { return (a.m + tm - 1) / tm * ((a.t + tn - 1) / tn); };
     size_t tm = 64;  // the small tiles' side
     if (a.t <= 32 || (a.t <= 64 && a.m < 8192) || 2 * tiles(64, 64) <= cus) tm = 32;
-    if (a.t > 64) {
+    // whole tiles hold the offsets of up to 256 rows in 32 bits
+    if (a.t > 64 && std::max(a.w_stride, a.x_stride) <= (1u << 24)) {
         const I8Big* best = nullptr;
         double least = 6 + 0.27 * (double)(tiles(64, 64) * stages) / (double)cus;
         for (const I8Big& b : kI8Big) {
@@ -108,7 +109,7 @@ hh_status hh_engine::enqueue_i8_gemm(int type, hh_i8_gemm_args a) {
         if (best) {
             a.mtiles = (uint32_t)((a.m + best->tm - 1) / best->tm);
             a.ttiles = (uint32_t)((a.t + best->tn - 1) / best->tn);
-            const size_t n = (size_t)a.mtiles * a.ttiles, grid = std::min(cus * best->per_cu, (n + 7) / 8 * 8);
+            const size_t n = (size_t)a.mtiles * a.ttiles, grid = std::min(std::max<size_t>(cus * best->per_cu / 8, 1) * 8, (n + 7) / 8 * 8);
             if (n > UINT32_MAX / 2) return fail(HH_ERR_INVALID, "gemm_i8: %u x %u outputs are too many", a.t, a.m);
             HH_TRY(kernel(std::string("hh_i8_big_") + best->name + "_" + ty, &f));
             return launch(f, (uint32_t)grid, (uint32_t)best->threads, a);

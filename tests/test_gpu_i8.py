@@ -566,3 +566,24 @@ def test_gemm_leaves_rows_behind(engine, ty):
                                       (F32, 20462, 577, 1500), (F16, 20462, 577, 1500)])
 def test_gemm_large(engine, ty, m, n, t):
     run_gemm(engine, ty, m, n, t, wpad=16, ypad=1, res=ty == BF16, seed=m, behind=260)
+
+
+@pytest.mark.parametrize("far", ["w", "x"])
+def test_gemm_rows_far_apart(engine, far):
+    """Rows of codes more than 16 MB apart: 256 of them pass 32 bits of offset."""
+    m, n, t = (11657, 1040, 515) if far == "x" else (515, 1040, 11657)
+    stride, packed = (1 << 24) + 16, 1040
+    w, w64 = codes(1, m, n, packed)
+    x, x64 = codes(2, t, n, packed)
+    apart = engine.alloc(515 * stride)
+    for i, row in enumerate((w if far == "w" else x).numpy()):
+        apart.write(row, i * stride)
+    bw, bx = (apart, put(engine, x)) if far == "w" else (put(engine, w), apart)
+    one = put(engine, torch.ones(max(m, t), dtype=torch.float32))
+    y = engine.alloc(4 * t * m)
+    d = engine.gemm_i8_desc(F32, m, n, t, w_stride=stride if far == "w" else packed,
+                            x_stride=stride if far == "x" else packed)
+    engine.gemm_i8_dev(d, bw, 0, one, 0, bx, 0, one, 0, None, 0, y, 0)
+    # whole numbers below 127^2 * 1040 < 2^24: exact in f32
+    want = x64.astype(np.float32) @ w64.astype(np.float32).T
+    assert np.array_equal(y.read(np.float32, t * m).reshape(t, m), want)
