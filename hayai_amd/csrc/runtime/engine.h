@@ -342,7 +342,7 @@ struct hh_engine {
     hh_status enqueue_lut(size_t m, size_t n, const uint8_t* w, const float* lut, const float* x, float* y);
     // The 8-bit path (i8.cpp); device pointers, strides resolved (elements for activations, bytes
     // for codes).  b: up (norm null, act) or the residual (norm given); null: none.
-    hh_status enqueue_i8_rows(int type, size_t rows, hh_i8_rows_args a);
+    hh_status enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_args& a);
     hh_status enqueue_i8_gemm(int type, hh_i8_gemm_args a);
     hh_status enqueue_sample(int type, size_t rows, hh_sample_args a);
     // Reports (and clears) a grid-barrier timeout recorded by a fused kernel.  Syncs.

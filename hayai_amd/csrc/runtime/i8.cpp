@@ -27,7 +27,7 @@ void i8_kernels(std::vector<std::string>& k) {
 
 using namespace hh;
 
-hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, hh_i8_rows_args a) {
+hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_args& a) {
     const ActType* ty = act_type(type);
     const size_t chunks = (a.cols * ty->bytes + 15) / 16;
     // Few rows: as many threads as chunks, for latency.  Rows enough to fill the chip twice: up to four
@@ -40,13 +40,24 @@ hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, hh_i8_rows_args a) {
     const size_t each = (chunks + threads - 1) / threads;
     const char* v = each <= 1 ? "c1" : each <= 2 ? "c2" : many ? "c4" : "loop";
     const size_t per = many && threads == 64 ? 4 : 1;
-    a.rows = (uint32_t)rows;
     hipFunction_t f;
     HH_TRY(kernel(std::string("hh_i8_rows_") + ty->name + "_" + kind + "_" + v, &f));
-    void* params[] = {&a};
-    HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)((rows + per - 1) / per), 1, 1, (uint32_t)threads, (uint32_t)per, 1, 0,
-                                     stream, params, nullptr),
-               "hipModuleLaunchKernel(i8 rows)");
+    // a grid has fewer than 2^32 threads: 2^21 rows at a time
+    for (size_t r = 0; r < rows; r += (size_t)1 << 21) {
+        const size_t n = std::min(rows - r, (size_t)1 << 21);
+        hh_i8_rows_args p = a;
+        p.rows = (uint32_t)n;
+        p.x = (const char*)a.x + r * a.x_stride * ty->bytes;
+        p.b = a.b ? (const char*)a.b + r * a.b_stride * ty->bytes : nullptr;
+        p.sum = a.sum ? (char*)a.sum + r * a.sum_stride * ty->bytes : nullptr;
+        p.q = a.q + r * a.q_stride;
+        p.scale = a.scale + r;
+        p.values = a.values ? a.values + r * a.cols : nullptr;
+        void* params[] = {&p};
+        HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)((n + per - 1) / per), 1, 1, (uint32_t)threads, (uint32_t)per, 1, 0,
+                                         stream, params, nullptr),
+                   "hipModuleLaunchKernel(i8 rows)");
+    }
     return HH_OK;
 }
 

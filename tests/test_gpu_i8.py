@@ -587,3 +587,32 @@ def test_gemm_rows_far_apart(engine, far):
     # whole numbers below 127^2 * 1040 < 2^24: exact in f32
     want = x64.astype(np.float32) @ w64.astype(np.float32).T
     assert np.array_equal(y.read(np.float32, t * m).reshape(t, m), want)
+
+
+def test_more_rows_than_a_grid(engine):
+    rows, cols = (1 << 22) + 5, 3
+    for kind in ("plain", "act", "norm"):
+        print(f"[case] grid {kind}", flush=True)
+        x, up = normal(1, rows, cols).half(), normal(2, rows, cols).half()
+        w = (normal(3, cols) + 1.0).float()
+        bx, bu, bw = put(engine, x), put(engine, up), put(engine, w)
+        q, s, v = engine.alloc(rows * cols + SLACK), engine.alloc(4 * rows + SLACK), engine.alloc(4 * rows * cols + SLACK)
+        o = engine.alloc(rows * cols * 2)
+        for b in (q, s, v):
+            b.fill(0x5B)
+        u, unit = f64(x), 1.0
+        if kind == "norm":
+            engine.rms_norm_i8_dev(engine.rms_norm_i8_desc(F16, rows, cols, EPS), bx, 0, bu, 0, bw, 0, o, 0, q, 0, s, 0, v, 0)
+            u = u + f64(up)
+            assert torch.equal(get(o, torch.float16, (rows, cols)), torch.from_numpy(u).float().half())
+            unit = 1.0 / np.sqrt((u**2).mean(1, keepdims=True) + EPS)
+            u = u * f64(w)
+        elif kind == "act":
+            engine.quant_i8_dev(engine.quant_i8_desc(F16, rows, cols), bx, 0, bu, 0, q, 0, s, 0, v, 0)
+            u = act64(u, f64(up), hayai_amd.ACT_SILU)
+        else:
+            engine.quant_i8_dev(engine.quant_i8_desc(F16, rows, cols), bx, 0, None, 0, q, 0, s, 0, v, 0)
+        check_codes(q.read(np.int8, rows * cols).reshape(rows, cols), s.read(np.float32, rows),
+                    v.read(np.float32, rows * cols).reshape(rows, cols), *codes_of(u, unit))
+        for b, n in ((q, rows * cols), (s, 4 * rows), (v, 4 * rows * cols)):
+            assert np.all(b.read(np.uint8, SLACK, n) == 0x5B)
