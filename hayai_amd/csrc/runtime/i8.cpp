@@ -77,11 +77,12 @@ struct I8Big {
     size_t tm, tn, threads, per_cu;
     double first, round, stage;  // us: once, per round of tiles, per stage of 128 codes and round
 };
-// 28672 x 4096 and 4096 x 14336 at 128 to 4096 tokens: estimates within 15% of most, and the choice
-// within 10% of the best
+// Fitted to all forms' times at 20 shapes of 128 to 14336 codes, 159 to 49152 rows and 100 to 4096 tokens: the
+// choice is within 1% of the best on average and 6% at most (4751 x 467, 612 tokens: 128x128 9.1,
+// 64 x 64 16.2; 4096 x 4096, 256: 20.2, 9.8; 14336 x 4096, 200: 27.9, 38.6; 28672 x 4096, 2048: 256x256 234).
 static const I8Big kI8Big[] = {
-    {"128x128", 128, 128, 256, 2, 2, 10, 1.04},  // one a CU: 0.67 a stage
-    {"128x256", 128, 256, 512, 1, 3, 8, 0.98},
+    {"128x128", 128, 128, 256, 2, 2, 6, 1.04},  // one a CU: 3 a round, 0.67 a stage
+    {"128x256", 128, 256, 512, 1, 2, 7, 0.92},
     {"192x256", 192, 256, 512, 1, 5, 10, 1.2},
     {"256x256", 256, 256, 512, 1, 5, 13, 1.45},
 };
@@ -104,14 +105,17 @@ hh_status hh_engine::enqueue_i8_gemm(int type, hh_i8_gemm_args a) {
     auto tiles = [&](size_t tm, size_t tn) { return (a.m + tm - 1) / tm * ((a.t + tn - 1) / tn); };
     size_t tm = 64;  // the small tiles' side
     if (a.t <= 32 || (a.t <= 64 && a.m < 8192) || 2 * tiles(64, 64) <= cus) tm = 32;
+    const size_t n = tiles(tm, tm), whole = n >= 2 * cus ? 2 * cus : cus;  // (workgroups: below)
     // whole tiles hold the offsets of up to 256 rows in 32 bits
-    if (a.t > 64 && std::max(a.w_stride, a.x_stride) <= (1u << 24)) {
+    if (tm == 64 && std::max(a.w_stride, a.x_stride) <= (1u << 24)) {
         const I8Big* best = nullptr;
-        double least = 6 + 0.27 * (double)(tiles(64, 64) * stages) / (double)cus;
+        // small tiles: each one, its stages, and the exchange unless the workgroups get whole ones
+        double least = 3 + (1.3 + 0.208 * (double)stages) * (double)n / (double)cus + (n % whole ? 8 : 0);
         for (const I8Big& b : kI8Big) {
-            const size_t n = tiles(b.tm, b.tn), slots = cus * b.per_cu;
-            const double stage = b.per_cu > 1 && n <= cus ? 0.67 : b.stage;
-            const double t = b.first + (double)((n + slots - 1) / slots) * (b.round + stage * (double)stages);
+            const size_t k = tiles(b.tm, b.tn), slots = cus * b.per_cu;
+            const bool one = b.per_cu > 1 && k <= cus;
+            const double t = b.first + (double)((k + slots - 1) / slots) *
+                                           ((one ? 3 : b.round) + (one ? 0.67 : b.stage) * (double)stages);
             if (t < least) {
                 least = t;
                 best = &b;
@@ -120,15 +124,16 @@ hh_status hh_engine::enqueue_i8_gemm(int type, hh_i8_gemm_args a) {
         if (best) {
             a.mtiles = (uint32_t)((a.m + best->tm - 1) / best->tm);
             a.ttiles = (uint32_t)((a.t + best->tn - 1) / best->tn);
-            const size_t n = (size_t)a.mtiles * a.ttiles, grid = std::min(std::max<size_t>(cus * best->per_cu / 8, 1) * 8, (n + 7) / 8 * 8);
-            if (n > UINT32_MAX / 2) return fail(HH_ERR_INVALID, "gemm_i8: %u x %u outputs are too many", a.t, a.m);
+            const size_t k = (size_t)a.mtiles * a.ttiles;
+            const size_t grid = std::min(std::max<size_t>(cus * best->per_cu / 8, 1) * 8, (k + 7) / 8 * 8);
+            if (k > UINT32_MAX / 2) return fail(HH_ERR_INVALID, "gemm_i8: %u x %u outputs are too many", a.t, a.m);
             HH_TRY(kernel(std::string("hh_i8_big_") + best->name + "_" + ty, &f));
             return launch(f, (uint32_t)grid, (uint32_t)best->threads, a);
         }
     }
     a.mtiles = (uint32_t)((a.m + tm - 1) / tm);
     a.ttiles = (uint32_t)((a.t + tm - 1) / tm);
-    const size_t n = (size_t)a.mtiles * a.ttiles, units = n * stages;
+    const size_t units = n * stages;
     if (n > UINT32_MAX / 2) return fail(HH_ERR_INVALID, "gemm_i8: %u x %u outputs are too many", a.t, a.m);
     // workgroups, each a tile or two stages at least: two a CU where that cuts few tiles (28672 x 4096, 32 tokens, 896
     // tiles: 29.4, one a CU 35.6; 4096 x 14336, 32 tokens, 128 tiles: 14.4, 13.2)

@@ -616,3 +616,12 @@ def test_more_rows_than_a_grid(engine):
                     v.read(np.float32, rows * cols).reshape(rows, cols), *codes_of(u, unit))
         for b, n in ((q, rows * cols), (s, 4 * rows), (v, 4 * rows * cols)):
             assert np.all(b.read(np.uint8, SLACK, n) == 0x5B)
+
+
+@pytest.mark.parametrize("ty", TYPES)
+def test_gemm_mid(engine, ty):
+    """64 x 64 tiles cut between workgroups and whole, then each form of whole tiles at few tokens."""
+    for k, (m, n, t) in enumerate([(2999, 2100, 131), (4096, 512, 256), (8200, 100, 40), (2999, 130, 130),
+                                   (16653, 1040, 130), (21979, 131, 300), (24645, 1040, 300)]):
+        print(f"[case] mid type={ty} m={m} n={n} t={t}", flush=True)
+        run_gemm(engine, ty, m, n, t, ypad=k % 2, res=k % 2 == 0, in_place=k == 3, seed=900 + 10 * k, behind=0 if k == 3 else 256)
