@@ -30,8 +30,7 @@ HH_DEV float hh_i8_value(int sum, float xs, float ws) { return (float)sum * xs *
 // multiplies them with the tokens' same columns from LDS; v_dot4_i32_i8 sums stay in the lane until
 // the rows' end, then one DPP sum a row and token.  Rows go round over the grid's waves, so at any
 // moment the requests lie next to each other.  Bound by HBM: 28672 x 4096, one token, 22 us = 5.3
-// TB/s (v_mfma_i32_16x16x64_i8 straight from memory, 16 rows x 64 bytes a load: 28 us); 128256 x
-// 4096, 8 tokens, 106 us.
+// TB/s (v_mfma_i32_16x16x64_i8 straight from memory, 16 rows x 64 bytes a load: 28 us).
 #define HH_I8_RD_R 2
 #define HH_I8_RD_D 4
 
@@ -142,7 +141,9 @@ HH_DEV void hh_i8_rowdot(const hh_i8_gemm_args& a) {
 // The tiles' stages, tile after tile, are cut into W equal runs, one a workgroup, so all finish
 // together whatever the shape.  A tile cut between workgroups is summed by the last of them to
 // arrive: the others leave their sums in a workspace (stores and loads at device scope, then a count
-// on a device word; the count returns to zero) and nobody waits.
+// on a device word; the count returns to zero) and nobody waits.  Bound by HBM to 64 tokens: 128256 x
+// 4096, 8 tokens, 106 us = 5.0 TB/s; 4096 x 14336, 61 tokens, 15.3 us = 3.9 TB/s (256 tiles, each
+// cut in two: an exchange at every end).
 template <int B, int BYTES>
 HH_DEV int8_t* hh_i8_lds() {
     __shared__ __attribute__((aligned(128))) int8_t buf[BYTES];
@@ -380,7 +381,8 @@ HH_DEV void hh_i8_tile(const hh_i8_gemm_args& a) {
 // second half's operands are read while the first half multiplies, the next stage's first half's
 // while the second does (sched_group_barrier: one LDS read to PER products), and the next tile's
 // first stages are asked for before this one's outputs are written.  Cut tiles cost more here than
-// idle CUs: 28672 x 4096, 512 tokens, 224 tiles of 256 x 256: 67 us, cut into 256 runs 106.
+// idle CUs: 28672 x 4096, 512 tokens, 224 tiles of 256 x 256: 67 us, cut into 256 runs 106.  Bound by
+// power: 28672 x 4096, 2048 tokens, 235 us = 2.04 POP/s at a clock of 1.65 to 1.95 GHz.
 template <class F, int TM, int TN, int WM, int WN>
 HH_DEV void hh_i8_big(const hh_i8_gemm_args& a) {
     constexpr int WAVES = WM * WN, HALF = (TM + TN) * 128;

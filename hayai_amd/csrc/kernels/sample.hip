@@ -14,6 +14,9 @@
 //                     and the tokens of those bins into a list
 //   hh_sample_pick    one workgroup a row: where in the list the prefix ends (radix select), the
 //                     chunk at which the running weight passes u, the token in it
+// 128256 f32 logits, a row: 20 us, near all of it the chain of four launches (3, 5, 6 and 7 us); 64 rows: 57 us,
+// of which max 7.5 (at the memory's rate), hist 15 and gather 20 (both the weights, about 45 operations a token) and
+// pick 15 (sorts and scans one after the other).
 // A row whose list passes 8192 tokens (nearly equal logits throughout), whose largest logit is infinite or
 // whose T is past 1e30 is done by one workgroup from the logits (hh_sample_row).
 #include "act_types.h"

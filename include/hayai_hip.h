@@ -473,8 +473,8 @@ hh_status hh_gemm_i8_dev(hh_engine* e, const hh_gemm_i8_desc* d, const hh_buf* w
  * first token with probability 1.  A NaN logit counts as -inf; where the largest is +inf those
  * tokens have weight 1 and the others 0.  A row without a token above -inf gets id -1 and
  * probability 0.  u outside [0, 1) is taken to its nearest end (NaN: 0).  Weights are held as
- * whole multiples of 2^-42 (lighter tokens are never drawn), so a row's answer depends on nothing
- * but the row.  vocab <= HH_SAMPLE_MAX_VOCAB. */
+ * the nearest whole multiples of 2^-42 (tokens lighter than 2^-43 are never drawn), so a row's answer
+ * depends on nothing but the row.  vocab <= HH_SAMPLE_MAX_VOCAB. */
 #define HH_SAMPLE_MAX_VOCAB 2097152u
 typedef struct hh_sample_params {
     float temperature;
