@@ -6,6 +6,8 @@ rounding (2^-24 relative) of the 64-bit value.  A product's sum is exact; its co
 two scales and the residual round once each (2^-24 of the product, of the result), then the output
 type (eps / 2).
 """
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 import torch
@@ -625,3 +627,40 @@ def test_gemm_mid(engine, ty):
                                    (16653, 1040, 130), (21979, 131, 300), (24645, 1040, 300)]):
         print(f"[case] mid type={ty} m={m} n={n} t={t}", flush=True)
         run_gemm(engine, ty, m, n, t, ypad=k % 2, res=k % 2 == 0, in_place=k == 3, seed=900 + 10 * k, behind=0 if k == 3 else 256)
+
+
+def test_workspaces_grow_after_a_capture():
+    """A captured step keeps its workspaces when a larger eager one makes the engine's grow."""
+    with hayai_amd.HipEngine(0) as e:
+        L = Layer(e, F16, 20, 256, 704, 5000, 30)
+        L.step()
+        want = L.outputs()
+        g = e.capture(L.step)
+        big = Layer(e, F16, 260, 576, 1536, 30000, 31)
+        big.step()
+        want_big = big.outputs()
+        for k in range(3):
+            print(f"[case] replay after growth {k}", flush=True)
+            for b in (L.r2, L.logits, L.ids, L.probs):
+                b.fill(0xFF)
+            g.launch()
+            big.step()
+            assert all(torch.equal(a, b) for a, b in zip(L.outputs(), want))
+            assert all(torch.equal(a, b) for a, b in zip(big.outputs(), want_big))
+        g.close()
+
+
+def test_two_engines(engine):
+    """Two engines on one GPU, each from a thread of its own, disturb nothing of each other."""
+    with hayai_amd.HipEngine(0) as other:
+        layers = [Layer(engine, BF16, 17, 512, 1408, 9000, 40), Layer(other, BF16, 70, 512, 1408, 9000, 41)]
+        want = []
+        for L in layers:
+            L.step()
+            want.append(L.outputs())
+        with ThreadPoolExecutor(2) as pool:
+            for f in [pool.submit(lambda L: [L.step() for _ in range(20)], L) for L in layers]:
+                f.result()
+        for L, w in zip(layers, want):
+            assert all(torch.equal(a, b) for a, b in zip(L.outputs(), w))
+        del layers, L
