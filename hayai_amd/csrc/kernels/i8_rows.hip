@@ -13,7 +13,7 @@
 // vector rate equals the 32-bit one on this chip.
 //
 // One workgroup per row (many short rows: four, a wave each), the row in registers between the two phases
-// (CH chunks of 16 bytes a thread); rows of more than 2048 chunks are read twice (hh_i8_rows_<...>_loop).
+// (CH chunks of 16 bytes a thread); rows of more than 4096 chunks are read twice (hh_i8_rows_<...>_loop).
 // Bound by HBM where there are many rows: 14336 x 4096 f32 with values 92.7 us = 5.7 TB/s; 2048 x 4096 f32 with
 // residual, sum and values 32.8 us = 4.3 TB/s; 509 x 14336 bf16 gated 20.7 us = 3.2 TB/s (with 64-bit act 27).
 // By latency where there are few: 64 x 8192 bf16 with residual 5.9 us, 576 f32 4.5 us.
@@ -368,14 +368,14 @@ HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
 }
 
 #define HH_I8_ROWS_KIND(T, F, NAME, KIND)                                                                           \
-    HH_I8_ROWS_CH(T, F, NAME, KIND, 1, 1024)                                                                        \
-    HH_I8_ROWS_CH(T, F, NAME, KIND, 2, 1024)                                                                        \
-    HH_I8_ROWS_CH(T, F, NAME, KIND, 4, 512)                                                                         \
+    HH_I8_ROWS_CH(T, F, NAME, KIND, 1)                                                                              \
+    HH_I8_ROWS_CH(T, F, NAME, KIND, 2)                                                                              \
+    HH_I8_ROWS_CH(T, F, NAME, KIND, 4)                                                                              \
     extern "C" __global__ void __launch_bounds__(1024) hh_i8_rows_##T##_##NAME##_loop(const hh_i8_rows_args a) {   \
         hh_i8_rows_loop<F, KIND>(a);                                                                                \
     }
-#define HH_I8_ROWS_CH(T, F, NAME, KIND, CH, MAX)                                                                    \
-    extern "C" __global__ void __launch_bounds__(MAX) hh_i8_rows_##T##_##NAME##_c##CH(const hh_i8_rows_args a) {   \
+#define HH_I8_ROWS_CH(T, F, NAME, KIND, CH)                                                                         \
+    extern "C" __global__ void __launch_bounds__(1024) hh_i8_rows_##T##_##NAME##_c##CH(const hh_i8_rows_args a) {   \
         if constexpr (KIND == HH_I8_ACT)                                                                            \
             hh_i8_act_rows<F, CH>(a);                                                                               \
         else                                                                                                        \

@@ -34,11 +34,11 @@ hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_arg
     // chunks a thread, so that a CU holds more rows and asks for more of them at once; and where one wave
     // holds a row, four rows a workgroup (7178 rows of 208 f16: 8.2 us, one a workgroup with four chunks a
     // thread 19.1, eight a workgroup 8.4; 13527 of 1076: 22.0, 32.1, 22.3).
-    const bool many = rows >= 2 * (size_t)props.multiProcessorCount && chunks <= 2048;
+    const bool many = rows >= 2 * (size_t)props.multiProcessorCount && chunks <= 4096;
     const size_t threads = std::min<size_t>(1024, ((many ? (chunks + 3) / 4 : chunks) + 63) / 64 * 64);
     const char* kind = a.norm ? "norm" : a.b ? "act" : "plain";
     const size_t each = (chunks + threads - 1) / threads;
-    const char* v = each <= 1 ? "c1" : each <= 2 ? "c2" : many ? "c4" : "loop";
+    const char* v = each <= 1 ? "c1" : each <= 2 ? "c2" : each <= 4 ? "c4" : "loop";
     const size_t per = many && threads == 64 ? 4 : 1;
     hipFunction_t f;
     HH_TRY(kernel(std::string("hh_i8_rows_") + ty->name + "_" + kind + "_" + v, &f));

@@ -510,8 +510,8 @@ def test_wrapped_memory(engine):
 
 # Rows enough to fill the chip twice: a workgroup of few threads with four chunks a thread, whose last
 # chunks lie partly or wholly past the row.  One element; inside, at and past a chunk of 64 threads; in
-# the third chunk; full; two waves.
-MANY = [1, 5, 89, 255, 257, 577, 1000, 1024, 1029, 2500, 4099]
+# the third chunk; full; two waves; twelve or six.
+MANY = [1, 5, 89, 255, 257, 577, 1000, 1024, 1029, 2500, 4099, 12001]
 SLACK = 1 << 16
 
 
