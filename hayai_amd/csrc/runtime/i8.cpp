@@ -30,11 +30,12 @@ using namespace hh;
 hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_args& a) {
     const ActType* ty = act_type(type);
     const size_t chunks = (a.cols * ty->bytes + 15) / 16;
-    // Few rows: as many threads as chunks, for latency.  Rows enough to fill the chip twice: up to four
-    // chunks a thread, so that a CU holds more rows and asks for more of them at once; and where one wave
-    // holds a row, four rows a workgroup (7178 rows of 208 f16: 8.2 us, one a workgroup with four chunks a
-    // thread 19.1, eight a workgroup 8.4; 13527 of 1076: 22.0, 32.1, 22.3).
-    const bool many = rows >= 2 * (size_t)props.multiProcessorCount && chunks <= 4096;
+    // Few rows: as many threads as chunks, for latency.  More rows than CUs: up to four chunks a thread, so
+    // that a CU holds several rows and asks for more of them at once (400 x 4096 f32 normalised: 6.0 us, one
+    // chunk a thread 6.9; 300 x 16384 bf16: 12.2, 13.0); and where one wave holds a row, four rows a
+    // workgroup (7178 rows of 208 f16: 8.2 us, one a workgroup with four chunks a thread 19.1, eight a
+    // workgroup 8.4; 13527 of 1076: 22.0, 32.1, 22.3).
+    const bool many = rows > (size_t)props.multiProcessorCount && chunks <= 4096;
     const size_t threads = std::min<size_t>(1024, ((many ? (chunks + 3) / 4 : chunks) + 63) / 64 * 64);
     const char* kind = a.norm ? "norm" : a.b ? "act" : "plain";
     const size_t each = (chunks + threads - 1) / threads;
