@@ -252,13 +252,17 @@ HH_DEV void hh_i8_rows_loop(const hh_i8_rows_args& a) {
 // is twice the memory's time (509 x 14336 bf16: 27 us).  h = act(g) u is computed in f32 with a bound e
 // on its relative error: the exponent y is within 8 2^-24 |y| (GELU's polynomial, log2 e; it counts
 // where y < 0, as exp(-y) / (1 + exp(-y)) of it reaches h), v_exp_f32 and v_rcp_f32 are within 2^-23,
-// and the products, the sum and 127 / a add at most 2^-24 each.  A code whose t lies within e |t| of
+// and the products, the sum and 127 / a add at most 2^-24 each.  The product g u comes first: the factor
+// 1 / (1 + exp(-y)) is at most 1, so a product that leaves f32's normal range below is of an h under 2^-126,
+// whose code is 0 beside a largest of 1e-25 or more however it is rounded, and one that leaves it above
+// makes the row's largest infinite or NaN.  (act(g) first: the half of a subnormal g is off by up to itself,
+// and a large u makes an ordinary h of it.)  A code whose t lies within e |t| of
 // a border, every element that may be the row's largest, and all with y < -80, are recomputed in 64
 // bits from memory, one by one (about one element in 4000).  Rows whose largest element is outside
 // 1e-25..1e25 (or NaN) are recomputed whole.
 HH_DEV float hh_i8_act32(float g, float u, int act, float& y) {
     y = act == HH_ACT_GELU_TANH ? 1.5957691216f * (g + 0.044715f * g * g * g) : g;
-    return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y * -1.4426950409f)) * u;
+    return g * u * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y * -1.4426950409f));
 }
 HH_DEV float hh_i8_act32_error(float y) { return (8.f * fmaxf(-y, 0.f) + 36.f) * 0x1p-24f; }
 
@@ -269,7 +273,7 @@ HH_DEV void hh_i8_act_rows(const hh_i8_rows_args& a) {
     typedef typename F::E E;
     constexpr int VEC = F::VEC;
     static_assert(CH * VEC <= 32, "a bit for each element of a thread");
-    constexpr float FAR = (8.f * 80.f + 36.f) * 0x1p-24f;  // the error bound at y = -80
+    constexpr float FAR = (8.f * 89.f + 36.f) * 0x1p-24f;  // the error bound at y = -89, past which h is 0
     __shared__ uint64_t red[2][16];
     const hh_i8_row<F, HH_I8_ACT> row(a, r);
     auto count = [&](int c) {

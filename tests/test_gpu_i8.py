@@ -664,3 +664,46 @@ def test_two_engines(engine):
         for L, w in zip(layers, want):
             assert all(torch.equal(a, b) for a, b in zip(L.outputs(), w))
         del layers, L
+
+
+# --------------------------------------------------------------- gated rows, special values
+
+
+def gated(engine, ty, act, gate, up):
+    """(codes, scale, values) of act(gate) * up, and what they have to be."""
+    rows, cols = gate.shape
+    q, s, v = engine.alloc(rows * cols), engine.alloc(4 * rows), engine.alloc(4 * rows * cols)
+    engine.quant_i8_dev(engine.quant_i8_desc(ty, rows, cols, act=act), put(engine, gate), 0, put(engine, up), 0, q, 0, s, 0, v, 0)
+    with np.errstate(all="ignore"):
+        want = codes_of(act64(f64(gate), f64(up), act))
+    return (q.read(np.int8, rows * cols).reshape(rows, cols), s.read(np.float32, rows),
+            v.read(np.float32, rows * cols).reshape(rows, cols)), want
+
+
+def many_rows():
+    return 2 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+
+
+@pytest.mark.parametrize("act", [hayai_amd.ACT_SILU, hayai_amd.ACT_GELU_TANH])
+@pytest.mark.parametrize("ty", TYPES)
+def test_gated_rows_of_subnormal_gates(engine, ty, act):
+    """Gates below or just above the type's normal range, whose products with up are ordinary numbers."""
+    fi = torch.finfo(DT[ty])
+    least = fi.smallest_normal * fi.eps
+    # the row's largest from the smallest gate, beside an ordinary pair; neighbours among the smallest gates
+    some = torch.tensor([[least, 1e-3], [3 * least, 4 * least], [-least, 2 * least]], dtype=torch.float64)
+    up = torch.tensor([[0.9 * fi.max, 1e-6], [0.33 * fi.max, 0.3 * fi.max], [0.5 * fi.max, 0.2 * fi.max]], dtype=torch.float64)
+    got, want = gated(engine, ty, act, some.to(DT[ty]), up.to(DT[ty]))
+    check_codes(*got, *want)
+    for rows in (7, many_rows()):
+        for cols in (5, 300, 1029, 4099):
+            print(f"[case] subnormal gates type={ty} act={act} {rows}x{cols}", flush=True)
+            rng = np.random.default_rng(cols + rows)
+            # gates of a row around one magnitude in or near the subnormals, up's from 1 to the type's largest
+            low = np.exp2(rng.uniform(np.log2(least) + 1, np.log2(fi.smallest_normal) + 6, (rows, 1)))
+            high = np.exp2(rng.uniform(0.0, np.log2(fi.max) - 4, (rows, 1)))
+            gate, up = low * rng.standard_normal((rows, cols)), high * rng.standard_normal((rows, cols))
+            ordinary = rng.random((rows, cols)) < 0.3  # some of ordinary gates with the same products
+            gate, up = np.where(ordinary, gate / low, gate), np.where(ordinary, up * low, up)
+            got, want = gated(engine, ty, act, torch.from_numpy(gate).to(DT[ty]), torch.from_numpy(up).to(DT[ty]))
+            check_codes(*got, *want)
