@@ -707,3 +707,79 @@ def test_gated_rows_of_subnormal_gates(engine, ty, act):
             gate, up = np.where(ordinary, gate / low, gate), np.where(ordinary, up * low, up)
             got, want = gated(engine, ty, act, torch.from_numpy(gate).to(DT[ty]), torch.from_numpy(up).to(DT[ty]))
             check_codes(*got, *want)
+
+
+def special_rows(ty, act, cols, seed):
+    """One row for each thing that the gated form decides apart from ordinary elements."""
+    rng = np.random.default_rng(seed)
+    big = torch.finfo(DT[ty]).max
+    inf, nan = float("inf"), float("nan")
+    at = int(rng.integers(0, cols))
+    # exp(-80) in front of up: SiLU's gate there, and tanh-GELU's, whose exponent is 1.6 (g + 0.045 g^3)
+    edge = -80.0 if act == hayai_amd.ACT_SILU else -9.673
+    out = []
+
+    def row(gate=None, up=None, at_gate=None, at_up=None):
+        g = 2.0 * rng.standard_normal(cols) if gate is None else np.broadcast_to(gate, cols).copy()
+        u = 2.0 * rng.standard_normal(cols) if up is None else np.broadcast_to(up, cols).copy()
+        if at_gate is not None:
+            g[at] = at_gate
+        if at_up is not None:
+            u[at] = at_up
+        out.append((g, u))
+
+    row()
+    row(gate=0.0)
+    row(up=0.0)
+    row(gate=-0.0, at_up=-3.0)
+    row(at_gate=nan)
+    row(at_up=nan)
+    for v in (inf, -inf):
+        row(at_gate=v)
+        row(at_gate=v, at_up=0.0)
+        row(at_up=v)
+        row(at_up=v, at_gate=0.0)
+        row(at_up=v, at_gate=edge * 4)
+    row(gate=edge * (1.0 + 0.02 * rng.standard_normal(cols)))                 # on both sides of the edge, alone
+    mixed = rng.random(cols) < 0.5                                            # and among ordinary gates
+    row(gate=np.where(mixed, edge * (1.0 + 0.02 * rng.standard_normal(cols)), rng.standard_normal(cols)))
+    row(gate=np.where(mixed, edge * 1.02, rng.standard_normal(cols)), up=np.where(mixed, 0.3 * big, 1e-3))
+    row(gate=1e-2 * rng.standard_normal(cols), up=1e-7, at_gate=edge * 1.03, at_up=0.5 * big)  # the largest there
+    row(gate=-1000.0)
+    row(gate=edge * 9.0)
+    # the largest outside 1e-25..1e25, and at either end of it, as far as the type goes
+    for power in (-44, -40, -30, -25, -24, -12, 0, 4, 12, 24, 25, 30, 36):
+        half = 10.0 ** (power / 2)
+        if half < 0.5 * big:
+            row(gate=half * np.abs(rng.standard_normal(cols)), up=half * rng.standard_normal(cols))
+    # products past f32, of an element that is small all the same
+    row(gate=np.where(mixed, edge * 0.9, 1.0), up=np.where(mixed, 0.9 * big, 1e-2))
+    row(gate=np.where(mixed, -big, 1.0))
+    row(gate=1.0, up=0.25 * big * np.where(rng.random(cols) < 0.5, 1.0, 0.3))
+    gate, up = (torch.from_numpy(np.stack(v)).to(DT[ty]) for v in zip(*out))
+    return gate, up
+
+
+@pytest.mark.parametrize("act", [hayai_amd.ACT_SILU, hayai_amd.ACT_GELU_TANH])
+@pytest.mark.parametrize("ty", TYPES)
+def test_gated_special_rows(engine, ty, act):
+    """Zero rows, NaN, infinities, gates where exp(-y) is large, largest values near the ends of f32: by
+    each form of a row (one to four chunks a thread, read twice), few and many."""
+    for many, columns in ((False, (1, 7, 300, 1029, 4099, 12001, 20003, 33001)), (True, (5, 300, 1029, 4099))):
+        for cols in columns:
+            print(f"[case] special rows type={ty} act={act} many={many} {cols}", flush=True)
+            gate, up = special_rows(ty, act, cols, cols)
+            if many:
+                times = -(-many_rows() // len(gate))
+                gate, up = gate.repeat(times, 1), up.repeat(times, 1)
+            got, want = gated(engine, ty, act, gate, up)
+            check_codes(*got, *want)
+
+
+@pytest.mark.parametrize("ty", TYPES)
+def test_gated_many_rows_gelu(engine, ty):
+    for k, cols in enumerate(MANY):
+        print(f"[case] many gelu type={ty} {cols}", flush=True)
+        gate, up = (normal(400 + 50 * i + k, many_rows(), cols, scale=2.0).to(DT[ty]) for i in range(2))
+        got, want = gated(engine, ty, hayai_amd.ACT_GELU_TANH, gate, up)
+        check_codes(*got, *want)
