@@ -213,3 +213,20 @@ def test_refusals(engine):
         with pytest.raises(hayai_amd.HipError) as err:
             call(**kw)
         assert err.value.status_name == status and word in str(err.value), (kw, err.value)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+def test_lists_past_a_part(engine, ty):
+    """Rows whose filters end among 1025 to 8192 tokens of one part: equal logits, and logits a little
+    apart, alone and above a body of others."""
+    rng = np.random.default_rng(12)
+    for vocab, rows in ((1500, 12), (2500, 12), (4096, 12), (8000, 512), (8192, 512), (8193, 512)):
+        print(f"[case] lists type={ty} {rows}x{vocab}", flush=True)
+        flat = np.zeros(vocab)
+        near = rng.standard_normal(vocab) * 1e-3 - 1e-2
+        body = np.where(rng.random(vocab) < 0.9, -0.004 * rng.random(vocab), -3.0 - rng.random(vocab))
+        params = [(1.0, vocab // 2, 1.0, 0.0), (1.0, 0, 0.83, 0.0), (1.0, vocab * 2 // 3, 0.6, 0.0), (0.5, 1100, 0.999, 0.001)]
+        x = np.stack([(flat, near, body)[i % 3] for i in range(rows)])
+        p = [params[i // 3 % 4] for i in range(rows)]
+        check(engine, ty, torch.from_numpy(x).to(DT[ty]), engine.sample_params(*[np.array(c) for c in zip(*p)]),
+              rng.random(rows))
