@@ -224,7 +224,7 @@ HH_DEV void hh_sample_row(const hh_sample_args& a, hh_smp_lds& s) {
     const uint64_t total = s.found;
     double u = (double)a.u[row];
     if (!(u > 0.0)) u = 0.0;
-    uint64_t want = (uint64_t)(u * (double)total);
+    uint64_t want = u < 1.0 ? (uint64_t)(u * (double)total) : total - 1;
     if (want >= total) want = total - 1;
     // the token at which the running weight first exceeds `want`
     if (after > want && after - sum <= want) {

@@ -230,3 +230,22 @@ def test_lists_past_a_part(engine, ty):
         p = [params[i // 3 % 4] for i in range(rows)]
         check(engine, ty, torch.from_numpy(x).to(DT[ty]), engine.sample_params(*[np.array(c) for c in zip(*p)]),
               rng.random(rows))
+
+
+def test_ends_of_u_in_rows_of_one_workgroup(engine):
+    """Rows that one workgroup does (all tokens nearly equal under top-p, an infinite temperature, an
+    infinite largest logit), with u at and past its ends."""
+    vocab = 20011
+    flat = -np.arange(vocab) * 1e-7
+    tall = np.where(np.arange(vocab) % 9973 == 5, np.inf, flat)
+    us = [0.0, -1.0, float("nan"), np.nextafter(np.float32(1), np.float32(0)), 1.0, 7.0, 1e30, 3e38, float("inf"), -float("inf")]
+    cases = [(x, t, k, p, u) for x, t, k, p in [(flat, 1.0, 0, 0.9), (flat, 1.0, 9000, 1.0), (flat, float("inf"), 0, 1.0),
+                                                (flat, 2e30, 9000, 0.7), (tall, 1.0, 0, 1.0), (tall, 1.0, 2, 0.5)]
+             for u in us]
+    x, t, k, p, u = (np.array(c) for c in zip(*cases))
+    logits, params, n = torch.from_numpy(x).float(), engine.sample_params(t, k, p, 0.0), len(cases) - len(us)
+    check(engine, F32, logits[:n], params[:n], u[:n])
+    # the last ten: two tokens of weight 1 and half of their weight wanted.  The weight before the second is 1 and
+    # the weight wanted 0.5 * 2 = 1, whole numbers on either side: not below it, so the first alone is kept.
+    ids, probs = sample(engine, F32, logits[n:], params[n:], u[n:])
+    assert np.all(ids == 5) and np.all(probs == 1.0)
