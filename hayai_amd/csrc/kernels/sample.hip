@@ -81,7 +81,7 @@ struct hh_smp_lds {
     uint64_t before, found;
     unsigned long long any, all;
     uint64_t sort[HH_SMP_BLOCK];
-    uint32_t digit, top;
+    uint32_t digit;
 };
 
 HH_DEV uint64_t hh_smp_scan(uint64_t v, hh_smp_lds& s) { return hh_block_scan64(v, s.wave); }
@@ -126,82 +126,57 @@ HH_DEV uint32_t hh_smp_select(const typename F::E* x, uint32_t n, uint32_t floor
     return prefix;
 }
 
-// A whole row by one workgroup of 1024.
+// A whole row by one workgroup of 1024: its largest key is `top`, above -inf's, and its temperature above 0.
 template <class F>
-HH_DEV void hh_sample_row(const hh_sample_args& a, hh_smp_lds& s) {
+HH_DEV void hh_sample_row(const hh_sample_args& a, uint32_t top, hh_smp_lds& s) {
     const uint32_t row = blockIdx.x, n = a.vocab, tid = threadIdx.x;
     const typename F::E* x = (const typename F::E*)a.x + row * a.stride;
     const hh_sample_row_params p = ((const hh_sample_row_params*)a.params)[row];
-    const bool greedy = !(p.temperature > 0.f);
-
-    // the largest key
-    uint32_t top = 0;
-    for (uint32_t i = tid; i < n; i += HH_SMP_BLOCK) top = max(top, hh_smp_key(F::get(x[i])));
-    if (tid == 0) s.top = 0;
-    __syncthreads();
-    atomicMax(&s.top, top);
-    __syncthreads();
-    top = s.top;
-    if (top <= HH_SMP_KEY_NINF) {
-        if (tid == 0) {
-            a.ids[row] = -1;
-            if (a.probs) a.probs[row] = 0.f;
-        }
-        return;
-    }
     const hh_smp_weights weights(top, p.temperature);
     auto mass = [&](uint32_t key) { return hh_smp_mass(weights.of(key)); };
 
     // cut: tokens with larger keys are in, of those with this key the first `ties` by index
     uint32_t cut = HH_SMP_KEY_NINF;
-    uint64_t ties = 0;
-    if (greedy) {
-        cut = top;
-        ties = 1;
-    } else {
-        uint64_t before;
-        if (p.top_k > 0 && (uint32_t)p.top_k < n) {
-            const uint32_t key =
-                hh_smp_select<F>(x, n, HH_SMP_KEY_NINF, (double)p.top_k, [](uint32_t) { return 1ull; }, s, before);
-            if (key) {
-                cut = key;
-                ties = (uint64_t)p.top_k - before;
-            }
-        }
-        if (p.top_p < 1.f) {
-            // the weight top-k left, then the key at which the share is reached
-            const uint64_t at_cut = ties ? ties * mass(cut) : 0;
-            uint64_t sum = 0;
-            for (uint32_t i = tid; i < n; i += HH_SMP_BLOCK) {
-                const uint32_t key = hh_smp_key(F::get(x[i]));
-                if (key > cut) sum += mass(key);
-            }
-            sum = hh_smp_scan(sum, s);
-            __syncthreads();
-            if (tid == HH_SMP_BLOCK - 1) s.found = sum;
-            __syncthreads();
-            const double want = (double)p.top_p * (double)(s.found + at_cut);
-            const uint32_t key = hh_smp_select<F>(x, n, cut, want, mass, s, before);
-            // a tie is in while the weight before it is below what is wanted
-            const uint32_t at = key ? key : cut;
-            if (key || ties) {
-                const double left = (want - (double)before) / (double)mass(at);
-                uint64_t c = left > 0.0 ? (uint64_t)ceil(left < 4e9 ? left : 4e9) : 0;
-                if (at == top && c == 0) c = 1;
-                if (!key && c > ties) c = ties;
-                cut = at;
-                ties = c;
-            }
-        }
-        if (p.min_p > 1.f) {  // heavier than any token: the first alone
-            cut = top;
-            ties = 1;
+    uint64_t ties = 0, before;
+    if (p.top_k > 0 && (uint32_t)p.top_k < n) {
+        const uint32_t key =
+            hh_smp_select<F>(x, n, HH_SMP_KEY_NINF, (double)p.top_k, [](uint32_t) { return 1ull; }, s, before);
+        if (key) {
+            cut = key;
+            ties = (uint64_t)p.top_k - before;
         }
     }
-    const double floor_w = !greedy && p.min_p > 0.f ? (double)p.min_p * HH_SMP_ONE : 0.0;
+    if (p.top_p < 1.f) {
+        // the weight top-k left, then the key at which the share is reached
+        const uint64_t at_cut = ties ? ties * mass(cut) : 0;
+        uint64_t sum = 0;
+        for (uint32_t i = tid; i < n; i += HH_SMP_BLOCK) {
+            const uint32_t key = hh_smp_key(F::get(x[i]));
+            if (key > cut) sum += mass(key);
+        }
+        sum = hh_smp_scan(sum, s);
+        __syncthreads();
+        if (tid == HH_SMP_BLOCK - 1) s.found = sum;
+        __syncthreads();
+        const double want = (double)p.top_p * (double)(s.found + at_cut);
+        const uint32_t key = hh_smp_select<F>(x, n, cut, want, mass, s, before);
+        // a tie is in while the weight before it is below what is wanted
+        const uint32_t at = key ? key : cut;
+        if (key || ties) {
+            const double left = (want - (double)before) / (double)mass(at);
+            uint64_t c = left > 0.0 ? (uint64_t)ceil(left < 4e9 ? left : 4e9) : 0;
+            if (at == top && c == 0) c = 1;
+            if (!key && c > ties) c = ties;
+            cut = at;
+            ties = c;
+        }
+    }
+    if (p.min_p > 1.f) {  // heavier than any token: the first alone
+        cut = top;
+        ties = 1;
+    }
+    const double floor_w = p.min_p > 0.f ? (double)p.min_p * HH_SMP_ONE : 0.0;
     auto heavy = [&](uint32_t key) { return key == top || weights.of(key) >= floor_w; };
-    const bool only_top = greedy || cut == top;
-    if (only_top && ties == 0) ties = 1;
 
     // each thread takes a run of indices: how many ties precede it, then the kept weight
     const uint32_t per = (n + HH_SMP_BLOCK - 1) / HH_SMP_BLOCK;
@@ -212,7 +187,6 @@ HH_DEV void hh_sample_row(const hh_sample_args& a, hh_smp_lds& s) {
     auto kept_mass = [&](uint32_t key, uint64_t& rank) -> uint64_t {
         if (key < cut || key <= HH_SMP_KEY_NINF) return 0;
         if (key == cut && rank++ >= ties) return 0;
-        if (greedy) return 1;
         return heavy(key) ? mass(key) : 0;
     };
     uint64_t rank = rank0, sum = 0;
@@ -236,8 +210,7 @@ HH_DEV void hh_sample_row(const hh_sample_args& a, hh_smp_lds& s) {
             run += m;
             if (run > want) {
                 a.ids[row] = (int32_t)i;
-                if (a.probs)
-                    a.probs[row] = greedy ? 1.f : (float)(weights.of(key) / (double)total);
+                if (a.probs) a.probs[row] = (float)(weights.of(key) / (double)total);
                 break;
             }
         }
@@ -448,7 +421,8 @@ HH_DEV void hh_smp_find_cut(const hh_sample_args& a, uint32_t row, const hh_samp
     __syncthreads();
     if (tid == HH_SMP_THREADS - 1 && cut.kbin == HH_SMP_BINS) cut.kmass = ms;
     if (p.top_p < 1.f) {
-        // between what top-k keeps at least and at most
+        // between what top-k keeps at least and at most: less than the weight through kbin, so plo and phi are
+        // kbin at most
         __shared__ double want[2];
         const uint32_t kbin = cut.kbin;
         if (tid == HH_SMP_THREADS - 1 && kbin == HH_SMP_BINS) want[0] = want[1] = (double)p.top_p * (double)ms;
@@ -468,12 +442,6 @@ HH_DEV void hh_smp_find_cut(const hh_sample_args& a, uint32_t row, const hh_samp
             if (here && (before == 0 || (double)before < want[1]) && (double)(before + here) >= want[1])
                 cut.phi = 2 * tid + q;
         }
-        __syncthreads();
-        if (tid == 0 && cut.plo > cut.kbin) {  // cannot be, but a bin past top-k's end is no end
-            cut.plo = cut.kbin;
-            cut.pmass = cut.kmass;
-        }
-        if (tid == 0) cut.phi = min(cut.phi, cut.kbin);
     } else if (tid == 0) {
         cut.plo = cut.phi = cut.kbin;
         cut.pmass = cut.kmass;
@@ -734,7 +702,7 @@ HH_DEV void hh_sample_pick(const hh_sample_args& a) {
         }
         return;
     }
-    if (n > HH_SMP_LIST) return hh_sample_row<F>(a, s);
+    if (n > HH_SMP_LIST) return hh_sample_row<F>(a, top, s);
     const hh_smp_cut cut = ((const hh_smp_cut*)a.cut)[row];
     const hh_smp_bins bins(top, p.temperature);
     const hh_smp_weights weights(top, p.temperature);
