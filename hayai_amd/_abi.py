@@ -208,6 +208,7 @@ SIGNATURES = {
     "hh_engine_destroy": (None, [P]),
     "hh_engine_info": (ST, [P, C.POINTER(DeviceInfo)]),
     "hh_engine_sync": (ST, [P]),
+    "hh_engine_stream": (ST, [P, PP]),
     "hh_engine_ffn_calls": (C.c_uint64, [P]),
     "hh_buf_alloc": (ST, [P, SZ, I, PP]),
     "hh_buf_wrap": (ST, [P, P, SZ, PP]),

@@ -119,6 +119,14 @@ hh_status hh_engine_sync(hh_engine* e) {
     return e->check_device_error();
 }
 
+hh_status hh_engine_stream(hh_engine* e, void** stream) {
+    HH_NOT_NULL(stream, "stream");
+    *stream = nullptr;
+    HH_NOT_NULL(e, "engine");
+    *stream = e->stream;
+    return HH_OK;
+}
+
 uint64_t hh_engine_ffn_calls(const hh_engine* e) { return e ? e->ffn_calls.load() : 0; }
 
 // ---------------------------------------------------------------- buffers ------------

@@ -377,6 +377,14 @@ class HipEngine:
     def sync(self) -> None:
         _check(self.lib.hh_engine_sync(self.handle))
 
+    @property
+    def stream(self) -> int:
+        """The compute stream's hipStream_t, for work and events of another library that shares memory
+        with this engine (torch.cuda.ExternalStream(engine.stream), say)."""
+        s = C.c_void_p()
+        _check(self.lib.hh_engine_stream(self.handle, C.byref(s)))
+        return int(s.value)
+
     # ---------------------------------------------------------------- buffers
     def alloc(self, nbytes: int, kind: int = BUF_DEVICE) -> DeviceBuffer:
         return DeviceBuffer(self, nbytes, kind)
@@ -389,7 +397,8 @@ class HipEngine:
 
     def wrap(self, address: int, nbytes: int) -> BorrowedBuffer:
         """A buffer over device memory of the caller's (a torch tensor's data_ptr(), say), which has
-        to outlive it; work on other streams is the caller's to order (hh_buf_wrap)."""
+        to outlive it; work on other streams is the caller's to order, by synchronizations or by events
+        on `stream` (hh_buf_wrap)."""
         return BorrowedBuffer(self, address, nbytes)
 
     def event(self) -> Event:

@@ -127,6 +127,12 @@ void hh_engine_destroy(hh_engine* e);
 hh_status hh_engine_info(const hh_engine* e, hh_device_info* out);
 /* Wait for all work on both engine streams. */
 hh_status hh_engine_sync(hh_engine* e);
+/* No counterpart in the reference.  The engine's compute stream as a hipStream_t, for a caller that
+ * shares device memory with another library (hh_buf_wrap): record and wait for events on it, or queue the
+ * other library's work on it.  It does not synchronise with the default stream, belongs to the engine and is
+ * valid until hh_engine_destroy; leave it alone between hh_graph_begin and hh_graph_end.  It is a handle
+ * of the HIP runtime that this library is loaded with: the other library has to use the same one. */
+hh_status hh_engine_stream(hh_engine* e, void** stream);
 /* Count of FFN GEMVs dispatched (the ffn_calls counter, context.rs:64-65). */
 uint64_t hh_engine_ffn_calls(const hh_engine* e);
 
@@ -142,7 +148,8 @@ int hh_buf_kind(const hh_buf* b);
  * another library, say): `bytes` bytes at `ptr`, which must lie inside one device allocation of
  * this engine's GPU (HH_ERR_INVALID otherwise).  hh_buf_free drops the handle after the engine's
  * queued work and leaves the memory alone.  The engine's stream knows nothing of other streams:
- * the caller orders work on the memory between them. */
+ * the caller orders work on the memory between them, by a synchronization on the host before the
+ * engine's call and hh_engine_sync after it, or by events on hh_engine_stream. */
 hh_status hh_buf_wrap(hh_engine* e, void* ptr, size_t bytes, hh_buf** out);
 /* Host address of a pinned buffer (NULL for device buffers). */
 void* hh_buf_host_ptr(hh_buf* b);

@@ -783,3 +783,41 @@ def test_gated_many_rows_gelu(engine, ty):
         gate, up = (normal(400 + 50 * i + k, many_rows(), cols, scale=2.0).to(DT[ty]) for i in range(2))
         got, want = gated(engine, ty, hayai_amd.ACT_GELU_TANH, gate, up)
         check_codes(*got, *want)
+
+
+@pytest.mark.parametrize("how", ["one stream", "events"])
+def test_shared_tensors_without_a_host_synchronization(engine, how):
+    """Another library's long work before the engine's calls and its reads after them, ordered by the
+    engine's stream alone."""
+    rows, cols = 64, 4096
+    own = torch.cuda.ExternalStream(engine.stream)
+    other = own if how == "one stream" else torch.cuda.Stream()
+    a = torch.randn(4096, 4096, device="cuda") / 64.0
+    x, first = torch.zeros(rows, cols, device="cuda"), torch.randn(rows, 4096, device="cuda")
+    q, s = torch.zeros(rows, cols, device="cuda", dtype=torch.int8), torch.zeros(rows, device="cuda")
+    bx, bq, bs = (engine.wrap(v.data_ptr(), v.numel() * v.element_size()) for v in (x, q, s))
+    d = engine.quant_i8_desc(F32, rows, cols)
+    want = []
+    with torch.cuda.stream(other):
+        torch.mm(first, a)  # (the library's first product sets it up)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(other):
+            v = first
+            for _ in range(60):
+                v = torch.mm(v, a)
+                v = v / v.abs().amax()
+            x.copy_(v)
+            first = v + 0.25
+        if other is not own:
+            own.wait_stream(other)
+        engine.quant_i8_dev(d, bx, 0, None, 0, bq, 0, bs, 0)
+        if other is not own:
+            other.wait_stream(own)
+        with torch.cuda.stream(other):
+            want.append((x.clone(), q.clone(), s.clone()))
+            q.zero_()
+            s.zero_()
+    torch.cuda.synchronize()
+    for x, q, s in want:
+        check_codes(q.cpu().numpy(), s.cpu().numpy(), None, *codes_of(f64(x.cpu())))

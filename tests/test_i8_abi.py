@@ -31,3 +31,11 @@ def test_sample_params_table():
     assert np.all(p["temperature"] == np.float32(0.5)) and np.all(p["min_p"] == 0)
     assert hayai_amd.HipEngine.sample_params(rows=4).shape == (4,)
     assert hayai_amd.HipEngine.sample_params().tobytes() == np.array([(1.0, 0, 1.0, 0.0)], p.dtype).tobytes()
+
+
+def test_engine_stream_rejects_null():
+    lib = _abi.load()
+    out = C.c_void_p(1)
+    assert lib.hh_engine_stream(None, C.byref(out)) == 2 and b"engine is NULL" in lib.hh_last_error()
+    assert out.value is None
+    assert lib.hh_engine_stream(None, None) == 2
