@@ -7,7 +7,8 @@ for each token and each row of weights (gemm); and the choice of a token from th
 temperature, top-k, top-p and min-p and a given random number (sample).
 
 Where `own` is false, run() computes them from elementary torch operations; where it is true it
-calls HipEngine on the same tensors' memory.  Codes are returned as the values they stand for.
+calls HipEngine on the same tensors' memory; its outputs are whole, to other streams than the engine's,
+after a synchronization of the device.  Codes are returned as the values they stand for.
 """
 import math
 
@@ -250,6 +251,8 @@ def _buffers(state):
         h["desc"] = e.gemm_i8_desc(ty, case["m"], case["n"], case["tokens"], w_stride=wide, x_stride=wide)
     else:
         h["desc"] = e.sample_desc(ty, case["rows"], case["vocab"])
+    # the engine's stream does not wait for torch's: the inputs are whole before its first call
+    torch.cuda.synchronize()
     return h
 
 
