@@ -422,9 +422,10 @@ hh_status hh_moe_dev(hh_engine* e, const hh_moe_desc* d, const hh_buf* experts, 
 
 /* Rows into codes: of x itself, or of the gated intermediate u = act(x) * up.  For each row,
  * with a = max |u|:  q = rint(127 u / a) (ties to even, decided as in 64-bit arithmetic, in -127..127)
- * and scale = a / 127.  A row of zeros has scale 0 and codes 0; a row holding a NaN or an infinity
- * has scale NaN and codes 0.  values (or NULL): rows of `cols` f32, packed, q * scale as the codes
- * stand for them, for consumers that stay in float and must see the same numbers. */
+ * and scale = a / 127, rounded to f32.  A row of zeros, or whose scale rounds to 0, has scale 0 and
+ * codes 0; a row holding a NaN or an infinity has scale NaN and codes 0; one of finite u whose scale
+ * passes f32 has scale infinity and its codes.  values (or NULL): rows of `cols` f32, packed, q * scale as
+ * the codes stand for them, for consumers that stay in float and must see the same numbers. */
 typedef struct hh_quant_i8_desc {
     int type;          /* of x and up */
     int act;           /* HH_ACT_*, with up */
@@ -439,7 +440,7 @@ hh_status hh_quant_i8_dev(hh_engine* e, const hh_quant_i8_desc* d, const hh_buf*
 /* The RMS norm of x, or of x + res, into codes: v = x (+ res), u = v * norm with norm `cols`
  * f32, codes of u as above, scale = a / (127 sqrt(mean(v^2) + eps)): what q * scale stands for is
  * v * norm / sqrt(mean(v^2) + eps).  With res, sum receives v rounded to `type` (the new residual
- * stream) and may be res or x; the codes are of v before that rounding.  res and sum: both or
+ * stream) and may be res or x (same offset and stride); the codes are of v before that rounding.  res and sum: both or
  * neither. */
 typedef struct hh_rms_norm_i8_desc {
     int type;          /* of x, res and sum */

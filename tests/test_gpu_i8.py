@@ -821,3 +821,11 @@ def test_shared_tensors_without_a_host_synchronization(engine, how):
     torch.cuda.synchronize()
     for x, q, s in want:
         check_codes(q.cpu().numpy(), s.cpu().numpy(), None, *codes_of(f64(x.cpu())))
+
+
+def test_gated_rows_whose_scale_passes_f32(engine):
+    """Finite u, a / 127 past f32: codes as ever, scale infinity."""
+    gate, up = torch.tensor([[1e30, 5e29, 1.0, -1e30]]).repeat(2, 1), torch.tensor([[1e30, -1e30, 1.0, 1e30]]).repeat(2, 1)
+    got, want = gated(engine, F32, hayai_amd.ACT_SILU, gate, up)
+    assert want[0].tolist() == [[127, -64, 0, 0]] * 2  # (-63.5 to even; the last gate's act is 0)
+    assert np.array_equal(got[0], want[0]) and np.all(got[1] == np.inf)
