@@ -829,3 +829,26 @@ def test_gated_rows_whose_scale_passes_f32(engine):
     got, want = gated(engine, F32, hayai_amd.ACT_SILU, gate, up)
     assert want[0].tolist() == [[127, -64, 0, 0]] * 2  # (-63.5 to even; the last gate's act is 0)
     assert np.array_equal(got[0], want[0]) and np.all(got[1] == np.inf)
+
+
+@pytest.mark.parametrize("t", [hayai_amd.Q4_0, hayai_amd.Q8_0, hayai_amd.Q4_K, hayai_amd.Q6_K, hayai_amd.IQ2_XXS,
+                               hayai_amd.IQ3_XXS])
+def test_codes_from_packed_weights(engine, t):
+    """A GGUF matrix into codes on the device, and a product with them."""
+    from hayai_amd import synth
+    import oracle
+    rows, cols, tokens = 300, 768, 5
+    packed = synth.matrix(t, rows, cols, 77)
+    f, q, s = engine.alloc(4 * rows * cols), engine.alloc(rows * cols), engine.alloc(4 * rows)
+    engine.dequant_dev(t, engine.upload(packed), 0, rows * cols, f)
+    engine.quant_i8_dev(engine.quant_i8_desc(F32, rows, cols), f, 0, None, 0, q, 0, s, 0)
+    w = oracle.dequant(t, packed, rows * cols).reshape(rows, cols).astype(np.float64)
+    want_q, want_s = codes_of(w)
+    got_q, got_s = q.read(np.int8, rows * cols).reshape(rows, cols), s.read(np.float32, rows)
+    check_codes(got_q, got_s, None, want_q, want_s)
+    x, x64 = codes(3, tokens, cols, cols)
+    y, one = engine.alloc(4 * tokens * rows), put(engine, torch.ones(tokens))
+    engine.gemm_i8_dev(engine.gemm_i8_desc(F32, rows, cols, tokens), q, 0, s, 0, put(engine, x), 0, one, 0, None, 0, y, 0)
+    want = (x64 @ got_q.astype(np.int64).T).astype(np.float64) * got_s.astype(np.float64)
+    # the sum to f32 and its product with the scale: two roundings
+    assert np.all(np.abs(y.read(np.float32, tokens * rows).reshape(tokens, rows) - want) <= np.abs(want) * 2.0**-23 * (1 + 1e-6))
