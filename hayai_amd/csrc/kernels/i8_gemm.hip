@@ -142,8 +142,8 @@ HH_DEV void hh_i8_rowdot(const hh_i8_gemm_args& a) {
 // together whatever the shape.  A tile cut between workgroups is summed by the last of them to
 // arrive: the others leave their sums in a workspace (stores and loads at device scope, then a count
 // on a device word; the count returns to zero) and nobody waits.  Bound by HBM to 64 tokens: 128256 x
-// 4096, 8 tokens, 106 us = 5.0 TB/s; 4096 x 14336, 61 tokens, 15.3 us = 3.9 TB/s (256 tiles, each
-// cut in two: an exchange at every end).
+// 4096, 8 tokens, 106 us = 5.0 TB/s; 4096 x 14336, 61 tokens, 23.5 us = 2.6 TB/s, 15.4 where the weights lie in
+// the memory-side cache (256 tiles, each cut in two: an exchange at every end).
 template <int B, int BYTES>
 HH_DEV int8_t* hh_i8_lds() {
     __shared__ __attribute__((aligned(128))) int8_t buf[BYTES];
@@ -382,7 +382,7 @@ HH_DEV void hh_i8_tile(const hh_i8_gemm_args& a) {
 // while the second does (sched_group_barrier: one LDS read to PER products), and the next tile's
 // first stages are asked for before this one's outputs are written.  Cut tiles cost more here than
 // idle CUs: 28672 x 4096, 512 tokens, 224 tiles of 256 x 256: 67 us, cut into 256 runs 106.  Bound by
-// power: 28672 x 4096, 2048 tokens, 235 us = 2.04 POP/s at a clock of 1.65 to 1.95 GHz.
+// power: 28672 x 4096, 2048 tokens, 242 us = 1.99 POP/s at a clock of 1.65 to 1.95 GHz.
 template <class F, int TM, int TN, int WM, int WN>
 HH_DEV void hh_i8_big(const hh_i8_gemm_args& a) {
     constexpr int WAVES = WM * WN, HALF = (TM + TN) * 128;

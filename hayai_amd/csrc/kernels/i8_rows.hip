@@ -14,9 +14,11 @@
 //
 // One workgroup per row (many short rows: four, a wave each), the row in registers between the two phases
 // (CH chunks of 16 bytes a thread); rows of more than 4096 chunks are read twice (hh_i8_rows_<...>_loop).
-// Bound by HBM where there are many rows: 14336 x 4096 f32 with values 90.7 us = 5.8 TB/s; 2048 x 4096 f32 with
-// residual, sum and values 31.4 us = 4.5 TB/s; 509 x 14336 bf16 gated 19.5 us = 3.4 TB/s (with 64-bit act 27).
-// By latency where there are few: 64 x 8192 bf16 with residual 5.9 us, 576 f32 4.5 us.
+// Bound by HBM where there are many rows: 14336 x 4096 f32 with values 92.7 us = 5.7 TB/s; 2048 x 4096 f32 with
+// residual, sum and values 32.9 us = 4.3 TB/s (without values 27.9 = 3.9); 509 x 14336 bf16 gated 22.6 us = 2.9
+// TB/s, 19.5 over three sets of tensors in turn, which the memory-side cache holds in part (with 64-bit act 27;
+// without values 19.7 and 17.5).  By latency where there are few: 64 x 8192 bf16 with residual 7.2 us, 5.9 over
+// three sets, 576 f32 4.0 to 4.6 us.
 #include "act_types.h"
 #include "wave64.h"
 

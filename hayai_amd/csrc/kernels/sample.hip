@@ -17,8 +17,11 @@
 // 128256 f32 logits, a row: 20 us, near all of it the chain of four launches (3, 5, 6 and 7 us); 64 rows: 57 us,
 // of which max 7.5 (at the memory's rate), hist 15 and gather 20 (both the weights, about 45 operations a token) and
 // pick 15 (sorts and scans one after the other).
-// A row whose list passes 8192 tokens (nearly equal logits throughout), whose largest logit is infinite or
-// whose T is past 1e30 is done by one workgroup from the logits (hh_sample_row).
+// A row whose list passes 8192 tokens, whose largest logit is infinite or whose T is past 1e30 is done by one
+// workgroup from the logits (hh_sample_row): about a dozen reads of the row with atomics on few bins.  A list
+// passes where a filter ends among more than 8192 tokens within T / 32 of each other: 128256 logits of deviation 2
+// from T = 11 on at a top-p of 0.5, from 35 to 40 on at 0.95; equal logits at any T.  128256 f32 logits: 450 us a
+// row at an infinite T, 640 to 705 where all are equal; 64 such rows 580 and 1290 to 1400.
 #include "act_types.h"
 #include "wave64.h"
 

@@ -62,25 +62,29 @@ hh_status hh_engine::enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_arg
     return HH_OK;
 }
 
-// Which form, by the weights' bytes, the tokens and the tiles (28672 x 4096, 4096 x 14336, 4096 x 4096,
-// 128256 x 4096, 32000 x 2048 and 576 x 1536, weights from HBM; us):
-//   rows by v_dot4: one or two tokens (28672 x 4096: 22.0 and 23.8, small tiles 26.6; 4096 x 14336:
-//     11.3 and 12.3, 12.8); up to four where their codes take 32 KB of LDS or less (4096 x 4096 6.6,
-//     6.9; 32000 x 2048 15.8, 17.3; 4096 x 14336 14.3, 12.8); up to eight under 4 MB of weights
-//     (576 x 1536 4.0, 7.2; 4096 x 4096 8.4, 6.9)
-//   tiles of 32 x 32 to 32 tokens (28672 x 4096, 32 tokens: 29.4, of 64 x 64 30.9), and to 64 where 64-row
-//     tiles are few (4096 x 14336, 61 tokens: 15.0, 16.3; 28672 x 4096, 64 tokens: 40.8, 32.5), and where
-//     64 x 64 tiles would not give every other CU one (1000 x 2048, 100 tokens: 5.7, 8.9; 512 x 4096, 200:
-//     8.0, 8.9; with 256 of them, 4096 x 4096, 200: 17.5, 10.3)
+// Which form, by the weights' bytes, the tokens and the tiles.  Measured (us) over three sets of tensors in
+// turn / over 1 GB of them: three sets of up to 85 MB stay in the 256 MB memory-side cache.
+//   rows by v_dot4: one or two tokens (28672 x 4096: 22.4 / 22.6 and 23.6 / 23.8, small tiles 27.1 / 27.1 and
+//     27.2 / 27.4; 4096 x 14336: 11.3 / 13.2 and 12.2 / 14.1, 12.9 / 18.4); up to four where their codes take
+//     32 KB of LDS or less (4096 x 4096: 7.0 / 7.8, 7.3 / 8.9; 32000 x 2048: 15.0 / 17.3, 16.2 / 20.6; past it
+//     4096 x 14336: 14.5 / 16.8, 12.8 / 18.6); up to eight under 4 MB of weights (576 x 1536: 5.3 / 5.7,
+//     6.1 / 6.8; past it 4096 x 4096: 8.9 / 10.0, 7.2 / 9.1)
+//   tiles of 32 x 32 to 32 tokens (28672 x 4096, 32 tokens: 31.0 / 31.3, of 64 x 64 31.4 / 32.2), and to 64 where
+//     64-row tiles are few (4096 x 14336, 61 tokens: 15.4 / 23.2, 15.9 / 18.5, so the side that the cache favours;
+//     28672 x 4096, 64 tokens: 40.5 / 41.5, 33.7 / 34.5), and where 64 x 64 tiles would not give every other CU
+//     one (1000 x 2048, 100 tokens: 5.7 / 6.9, 8.7 / 9.4; 512 x 4096, 200: 7.6 / 9.7, 8.7 / 9.6; with 256 of
+//     them, 4096 x 4096, 200: 17.3 / 20.9, 9.8 / 13.0)
 //   past that the least of the estimates below.
 struct I8Big {
     const char* name;
     size_t tm, tn, threads, per_cu;
     double first, round, stage;  // us: once, per round of tiles, per stage of 128 codes and round
 };
-// Fitted to all forms' times at 20 shapes of 128 to 14336 codes, 159 to 49152 rows and 100 to 4096 tokens: the
-// choice is within 1% of the best on average and 6% at most (4751 x 467, 612 tokens: 128x128 9.1,
-// 64 x 64 16.2; 4096 x 4096, 256: 20.2, 9.8; 14336 x 4096, 200: 27.9, 38.6; 28672 x 4096, 2048: 256x256 234).
+// Fitted to all forms' times, three sets in turn, at 20 shapes of 128 to 14336 codes, 159 to 49152 rows and 100 to
+// 4096 tokens: there the choice is within 1% of the best on average and 6% at most; of nine more shapes it is
+// 10% off at one (28672 x 4096, 256 tokens: 128x256 54.6 / 57.1, 128x128 49.8 / 49.4).  As above: 4751 x 467,
+// 612 tokens: 128x128 8.7 / 11.1, 64 x 64 15.7 / 17.1; 4096 x 4096, 256: 23.5 / 32.8, 10.2 / 13.7; 14336 x 4096, 200:
+// 25.9 / 34.7, 36.7 / 39.6; 28672 x 4096, 2048: 256x256 242, 192x256 250.
 static const I8Big kI8Big[] = {
     {"128x128", 128, 128, 256, 2, 2, 6, 1.04},  // one a CU: 3 a round, 0.67 a stage
     {"128x256", 128, 256, 512, 1, 2, 7, 0.92},
@@ -166,9 +170,9 @@ hh_status hh_engine::enqueue_sample(int type, size_t rows, hh_sample_args a) {
     for (int i = 0; i < 4; i++) HH_TRY(kernel(std::string("hh_sample_") + names[i] + "_" + ty->name, &f[i]));
     const size_t pass = std::min(rows, kSmpRows);
     a.chunks = (uint32_t)((a.vocab + kSmpChunk - 1) / kSmpChunk);
-    // parts of 4096 tokens or more (of 8192: 23.0 us a row of 128256, 20.9), two a CU at most: each begins
-    // with the row's largest logit and bins (64 x 128256: 41.8 us, four a CU 43.3, one 45.9; 330 x 14006:
-    // 43.9, 51.8, 46.6)
+    // parts of 4096 tokens or more (of 8192: 23.6 us a row of 128256, 21.3), two a CU at most: each begins
+    // with the row's largest logit and bins (64 x 128256, a normal body and 40 likely tokens a row, eight requests'
+    // filters in turn: 56.6 us, four a CU 55.9, one 62.1; 330 x 14006: 48.1, 50.5, 53.6)
     a.parts = (uint32_t)std::max<size_t>(
         1, std::min<size_t>((a.vocab + 4095) / 4096, (2 * (size_t)props.multiProcessorCount + pass - 1) / pass));
     const size_t row_bytes = 8 * (a.parts + kSmpBins + a.chunks + kSmpList) + 4 * kSmpBins + kSmpCutBytes + 4;
