@@ -852,3 +852,71 @@ def test_codes_from_packed_weights(engine, t):
     want = (x64 @ got_q.astype(np.int64).T).astype(np.float64) * got_s.astype(np.float64)
     # the sum to f32 and its product with the scale: two roundings
     assert np.all(np.abs(y.read(np.float32, tokens * rows).reshape(tokens, rows) - want) <= np.abs(want) * 2.0**-23 * (1 + 1e-6))
+
+
+def test_rows_four_gigabytes_apart(engine):
+    """Strides and offsets past 32 bits in every operand that has rows of its own."""
+    cols, rows, far = 300, 3, (1 << 31) + 64  # f16 elements: 4 GB and a little
+    lead = 256
+    x, r = normal(1, rows, cols).half(), normal(2, rows, cols).half()
+    w = (normal(3, cols) + 1.0).float()
+    big = engine.alloc(lead + 2 * ((rows - 1) * far + 2 * cols) + 64)
+    big.fill(0x5B)
+    for i in range(rows):
+        big.write(x[i].view(torch.uint8).numpy(), lead + 2 * i * far)
+        big.write(r[i].view(torch.uint8).numpy(), lead + 2 * (i * far + cols))
+    qfar = (1 << 32) + 16
+    q, s, v = engine.alloc((rows - 1) * qfar + cols + 64), engine.alloc(4 * rows), engine.alloc(4 * rows * cols)
+    for i in range(rows):
+        q.fill(0x5B, cols + 64, i * qfar)
+
+    def codes_at(i):
+        got = q.read(np.int8, cols + 64, i * qfar)
+        assert np.all(got[cols:] == 0x5B)
+        return got[:cols]
+
+    d = engine.quant_i8_desc(F16, rows, cols, x_stride=far, up_stride=far, q_stride=qfar)
+    engine.quant_i8_dev(d, big, lead, big, lead + 2 * cols, q, 0, s, 0, v, 0)
+    check_codes(np.stack([codes_at(i) for i in range(rows)]), s.read(np.float32, rows),
+                v.read(np.float32, rows * cols).reshape(rows, cols), *codes_of(act64(f64(x), f64(r), hayai_amd.ACT_SILU)))
+    # the sum over the residual, in place
+    d = engine.rms_norm_i8_desc(F16, rows, cols, EPS, x_stride=far, res_stride=far, sum_stride=far, q_stride=qfar)
+    engine.rms_norm_i8_dev(d, big, lead, big, lead + 2 * cols, put(engine, w), 0, big, lead + 2 * cols, q, 0, s, 0, v, 0)
+    sum64 = f64(x) + f64(r)
+    check_codes(np.stack([codes_at(i) for i in range(rows)]), s.read(np.float32, rows),
+                v.read(np.float32, rows * cols).reshape(rows, cols),
+                *codes_of(sum64 * f64(w), 1.0 / np.sqrt((sum64**2).mean(1, keepdims=True) + EPS)))
+    for i in range(rows):
+        got = big.read(np.uint8, 4 * cols + 64, lead + 2 * i * far)
+        assert torch.equal(torch.from_numpy(got[2 * cols:4 * cols]).view(torch.float16), torch.from_numpy(sum64[i]).float().half())
+        assert np.array_equal(got[:2 * cols], x[i].view(torch.uint8).numpy()) and np.all(got[4 * cols:] == 0x5B)
+    del big
+    # a product with those codes, its rows as far apart: by rows of codes, and by tiles
+    m, n = 70, 288
+    for t, from_far in ((3, True), (40, False)):
+        w8, w64 = codes(5, m, n, n)
+        x8, x64 = codes(6, t, n, n)
+        if from_far:
+            x64 = np.stack([codes_at(i) for i in range(rows)])[:, :n].astype(np.int64)
+            bx, xstride = q, qfar
+        else:
+            bx, xstride = put(engine, x8), n
+        yfar = far if t == 3 else 1 << 26
+        y = engine.alloc(2 * ((t - 1) * yfar + m) + 64)
+        for i in range(t):
+            y.fill(0x5B, 2 * m + 64, 2 * i * yfar)
+        one = put(engine, torch.full((max(m, t),), 2.0**-4))
+        if from_far:  # the last row has its whole stride in the buffer
+            q2 = engine.alloc(rows * qfar)
+            for i in range(rows):
+                q2.copy_from(q, cols, i * qfar, i * qfar)
+            bx = q2
+        engine.gemm_i8_dev(engine.gemm_i8_desc(F16, m, n, t, x_stride=xstride, y_stride=yfar), put(engine, w8), 0, one, 0,
+                           bx, 0, one, 0, None, 0, y, 0)
+        want = (x64 @ w64.T).astype(np.float64) / 256.0
+        for i in range(t):
+            raw = y.read(np.uint8, 2 * m + 64, 2 * i * yfar)
+            got = torch.from_numpy(raw[:2 * m]).view(torch.float16).double().numpy()
+            # whole numbers below 2^24 and powers of two: one rounding, to f16
+            assert np.all(np.abs(got - want[i]) <= np.abs(want[i]) * 2.0**-11 + 2.0**-25) and np.all(raw[2 * m:] == 0x5B)
+        del y

@@ -249,3 +249,19 @@ def test_ends_of_u_in_rows_of_one_workgroup(engine):
     # the weight wanted 0.5 * 2 = 1, whole numbers on either side: not below it, so the first alone is kept.
     ids, probs = sample(engine, F32, logits[n:], params[n:], u[n:])
     assert np.all(ids == 5) and np.all(probs == 1.0)
+
+
+def test_rows_four_gigabytes_apart(engine):
+    vocab, far, rows = 5000, (1 << 31) + 8, 4
+    x = torch.from_numpy(2.0 * np.random.default_rng(13).standard_normal((rows, vocab))).half()
+    x[3] = 0.0
+    b = engine.alloc(2 * ((rows - 1) * far + vocab))
+    for i in range(rows):
+        b.write(x[i].view(torch.uint8).numpy(), 2 * i * far)
+    params, u = engine.sample_params([1.0, 0.0, 0.7, float("inf")], [0, 0, 40, 0], [0.9, 1.0, 0.9, 0.99]), [0.3, 0.5, 0.9, 0.77]
+    ids, pr = engine.alloc(4 * rows), engine.alloc(4 * rows)
+    engine.sample_dev(engine.sample_desc(F16, rows, vocab, far), b, 0, engine.upload(params), 0,
+                      engine.upload(np.asarray(u, np.float32)), 0, ids, 0, pr, 0)
+    want, probs = sample(engine, F16, x, params, u)
+    assert np.array_equal(ids.read(np.int32, rows), want) and np.array_equal(pr.read(np.float32, rows), probs)
+    check(engine, F16, x, params, u)
