@@ -20,6 +20,11 @@ from .engine import (  # noqa: F401
     Q4_K,
     Q6_K,
     Q8_0,
+    ROPE_BY_WAVELENGTH,
+    ROPE_HALVES,
+    ROPE_LINEAR,
+    ROPE_PAIRS,
+    ROPE_YARN,
     BorrowedBuffer,
     DeviceBuffer,
     HipEngine,
@@ -29,6 +34,7 @@ from .engine import (  # noqa: F401
     QuantMatrix,
     StreamingScratch,
     device_count,
+    rope_factors,
     row_bytes,
     validate_gemv_shape,
     validate_gemv_weights,

@@ -183,6 +183,33 @@ class SampleDesc(C.Structure):
     ]
 
 
+class KvDesc(C.Structure):
+    _fields_ = [
+        ("type", C.c_int),
+        ("kv_heads", C.c_size_t),
+        ("head_dim", C.c_size_t),
+        ("page_size", C.c_size_t),
+        ("n_pages", C.c_size_t),
+        ("page_stride", C.c_size_t),
+    ]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [
+        ("type", C.c_int),
+        ("layout", C.c_int),
+        ("tokens", C.c_size_t),
+        ("q_heads", C.c_size_t),
+        ("rot_dim", C.c_size_t),
+        ("base", C.c_double),
+        ("mscale", C.c_float),
+        ("q_stride", C.c_size_t),
+        ("k_stride", C.c_size_t),
+        ("v_stride", C.c_size_t),
+        ("out_stride", C.c_size_t),
+    ]
+
+
 SIGNATURES = {
     "hh_gguf_open": (ST, [C.c_char_p, PP]),
     "hh_gguf_close": (None, [P]),
@@ -251,6 +278,9 @@ SIGNATURES = {
     "hh_rms_norm_i8_dev": (ST, [P, C.POINTER(RmsNormI8Desc)] + [P, SZ] * 7),
     "hh_gemm_i8_dev": (ST, [P, C.POINTER(GemmI8Desc)] + [P, SZ] * 6),
     "hh_sample_dev": (ST, [P, C.POINTER(SampleDesc)] + [P, SZ] * 5),
+    "hh_rope_kv_dev": (ST, [P, C.POINTER(RopeDesc), C.POINTER(KvDesc)] + [P, SZ] * 8),
+    "hh_rope_factors": (ST, [I, SZ, C.c_double, C.c_double, C.c_double, P, P]),
+    "hh_kv_copy_dev": (ST, [P, C.POINTER(KvDesc), SZ, SZ, P, SZ, P, SZ, SZ]),
     "hh_streamer_create": (ST, [P, SZ, SZ, SZ, PP]),
     "hh_streamer_destroy": (None, [P]),
     "hh_streamer_slot_for": (ST, [P, SZ, C.POINTER(SZ)]),

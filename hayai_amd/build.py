@@ -1,11 +1,12 @@
 """Build the gfx950 code object and the C-ABI library ``libhayai_hip.so`` in-tree.
 
 Steps (all offline, no GPU needed):
-  1. hipcc --genco: every kernel source (one translation unit, csrc/kernels/all.hip) into
-     one gfx950 code object, with -ffp-contract=off and packed FP32 disabled.
-  2. An assembler stub .incbin's that code object into the library, so the engine loads it
-     with hipModuleLoadData and the .so is the only file a deployment needs (the engine
-     also accepts a code-object file via HAYAI_HIP_CODE_OBJECT, loaded with hipModuleLoad).
+  1. hipcc --genco: every kernel source into two gfx950 code objects, the attention operators'
+     (csrc/kernels/attn_all.hip) and all others' (csrc/kernels/all.hip), with
+     -ffp-contract=off and packed FP32 disabled.
+  2. An assembler stub .incbin's both code objects into the library, so the engine loads them
+     with hipModuleLoadData and the .so is the only file a deployment needs (the engine also
+     accepts a file in place of all.hip's via HAYAI_HIP_CODE_OBJECT, loaded with hipModuleLoad).
   3. g++ builds the host runtime (csrc/runtime/*.cpp) against the HIP runtime.
 
 Run ``python -m hayai_amd.build`` or call :func:`build`.
@@ -25,6 +26,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libhayai_hip.so")
 CODE_OBJECT = os.path.join(BUILD, "hayai_kernels_gfx950.hsaco")
+ATTN_CODE_OBJECT = os.path.join(BUILD, "hayai_attn_gfx950.hsaco")
 ARCH = "gfx950"
 
 KERNEL_FLAGS = [
@@ -57,14 +59,14 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(out)
 
 
-def build_kernels(verbose: bool = False) -> str:
+def build_kernels(verbose: bool = False, unit: str = "all.hip", out: str = CODE_OBJECT) -> str:
     os.makedirs(BUILD, exist_ok=True)
     hipcc = os.path.join(rocm_path(), "bin", "hipcc")
-    src = os.path.join(CSRC, "kernels", "all.hip")
-    tmp = CODE_OBJECT + ".tmp"
+    src = os.path.join(CSRC, "kernels", unit)
+    tmp = out + ".tmp"
     _run([hipcc, *KERNEL_FLAGS, "-o", tmp, src], verbose)
-    os.replace(tmp, CODE_OBJECT)
-    return CODE_OBJECT
+    os.replace(tmp, out)
+    return out
 
 
 def build_runtime(verbose: bool = False) -> list[str]:
@@ -72,7 +74,7 @@ def build_runtime(verbose: bool = False) -> list[str]:
     os.makedirs(BUILD, exist_ok=True)
     cxx = os.environ.get("CXX", "g++")
     objs = []
-    for name in ("engine.cpp", "i8.cpp", "capi.cpp", "streamer.cpp", "gguf.cpp"):
+    for name in ("engine.cpp", "i8.cpp", "attn.cpp", "capi.cpp", "streamer.cpp", "gguf.cpp"):
         src = os.path.join(CSRC, "runtime", name)
         obj = os.path.join(BUILD, name.replace(".cpp", ".o"))
         _run([cxx, "-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-parameter",
@@ -104,6 +106,9 @@ def link(objs: list[str], verbose: bool = False) -> str:
             "hh_kernels_blob:\n"
             f"\t.incbin \"{CODE_OBJECT}\"\n"
             "\t.global hh_kernels_blob_end\nhh_kernels_blob_end:\n\t.byte 0\n"
+            "\t.global hh_attn_blob\n\t.type hh_attn_blob, @object\n\t.balign 4096\n"
+            "hh_attn_blob:\n"
+            f"\t.incbin \"{ATTN_CODE_OBJECT}\"\n"
             "\t.section .note.GNU-stack,\"\",@progbits\n")
     blob_o = os.path.join(BUILD, "blob.o")
     _run(["gcc", "-c", blob_s, "-o", blob_o], verbose)
@@ -117,11 +122,13 @@ def link(objs: list[str], verbose: bool = False) -> str:
 def build(verbose: bool = False) -> str:
     """Compile everything; always rebuilds (this is the "does it build" check)."""
     t0 = time.time()
-    with ThreadPoolExecutor(max_workers=3) as ex:
+    with ThreadPoolExecutor(max_workers=4) as ex:
         fk = ex.submit(build_kernels, verbose)
+        fa = ex.submit(build_kernels, verbose, "attn_all.hip", ATTN_CODE_OBJECT)
         fr = ex.submit(build_runtime, verbose)
         fn = ex.submit(build_noalloc, verbose)
         fk.result()
+        fa.result()
         objs = fr.result() + [fn.result()]
     lib = link(objs, verbose)
     if verbose:

@@ -134,6 +134,38 @@ struct hh_sample_args {
     uint32_t vocab, parts, chunks, pad;
 };
 
+// Pages of keys and values (kv_pages.h): page p at base + p * stride bytes, its keys [heads][1 << shift][dim],
+// then its values [heads][dim][1 << shift].
+struct hh_kv_args {
+    uint8_t* base;
+    uint64_t stride;
+    uint32_t pages, shift, heads, dim;
+};
+
+// Rotated queries and keys, and the tokens' places in the cache (rope.hip); strides in elements.
+struct hh_rope_args {
+    hh_kv_args kv;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    const int32_t* positions;
+    const int32_t* slots;
+    const float* factors;  // null: all 1
+    uint64_t q_stride, k_stride, v_stride, out_stride;
+    double log2_base;
+    float mscale;
+    uint32_t heads, rot;
+};
+
+// Pages moves[i][0] -> moves[i][1] in each layer (kv_pages.hip); strides and sizes in bytes.
+struct hh_kv_copy_args {
+    hh_kv_args kv;
+    const int32_t* moves;
+    uint64_t layer_stride;
+    uint32_t n, chunks;  // moves, 16-byte chunks of a page
+};
+
 // Synthetic GGUF bytes: splitmix64 stream, then f16 scale fields drawn U(lo, hi).
 struct hh_synth_args {
     uint8_t* dst;

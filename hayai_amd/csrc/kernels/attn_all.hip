@@ -1,0 +1,4 @@
+// Translation unit of the attention operators' gfx950 code object, apart from all.hip's so that the two
+// compile at the same time.
+#include "rope.hip"
+#include "kv_pages.hip"

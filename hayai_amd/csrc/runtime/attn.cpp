@@ -1,0 +1,76 @@
+// Dispatch of the attention operators: rotary positions into the cache (rope.hip) and copies of its
+// pages (kv_pages.hip).
+#include <algorithm>
+
+#include "engine.h"
+
+namespace hh {
+
+std::string attn_types(int type, int kv_type) {
+    std::string s = act_type(type)->name;
+    return kv_type == type ? s : s + "_" + act_type(kv_type)->name;
+}
+
+static const int kAttnTypes[][2] = {{HH_TYPE_F32, HH_TYPE_F32}, {HH_TYPE_F16, HH_TYPE_F16}, {HH_TYPE_BF16, HH_TYPE_BF16},
+                                    {HH_TYPE_F32, HH_TYPE_F16}, {HH_TYPE_F32, HH_TYPE_BF16}};
+
+void attn_kernels(std::vector<std::string>& k) {
+    for (auto& t : kAttnTypes) {
+        const std::string ty = attn_types(t[0], t[1]);
+        for (const char* v : {"halves_", "pairs_"}) k.push_back(std::string("hh_rope_") + v + ty);
+    }
+    k.push_back("hh_kv_copy");
+}
+
+bool attn_kernel(const std::string& name) {
+    for (const char* stem : {"hh_rope_", "hh_kv_", "hh_attn_"})
+        if (name.rfind(stem, 0) == 0) return true;
+    return false;
+}
+
+}  // namespace hh
+
+using namespace hh;
+
+hh_status hh_engine::enqueue_rope(int type, int kv_type, int layout, size_t tokens, const hh_rope_args& a) {
+    hipFunction_t f;
+    HH_TRY(kernel(std::string("hh_rope_") + (layout == HH_ROPE_PAIRS ? "pairs_" : "halves_") + attn_types(type, kv_type), &f));
+    // a workgroup's 256 threads take a token's 16-byte pieces; of few tokens each is given to several
+    const size_t el = act_type(type)->bytes, cus = (size_t)props.multiProcessorCount;
+    const size_t pieces = (a.heads + 2 * (size_t)a.kv.heads) * ((a.kv.dim * el + 15) / 16);
+    const size_t parts = std::max<size_t>(1, std::min((pieces + 255) / 256, 2 * cus / tokens));
+    // a grid has fewer than 2^32 threads: 2^20 tokens at a time (parts are 1 there)
+    for (size_t t = 0; t < tokens; t += (size_t)1 << 20) {
+        const size_t n = std::min(tokens - t, (size_t)1 << 20);
+        hh_rope_args p = a;
+        p.q = (const char*)a.q + t * a.q_stride * el;
+        p.k = (const char*)a.k + t * a.k_stride * el;
+        p.v = (const char*)a.v + t * a.v_stride * el;
+        p.out = (char*)a.out + t * a.out_stride * el;
+        p.positions = a.positions + t;
+        p.slots = a.slots + t;
+        void* params[] = {&p};
+        HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)n, (uint32_t)parts, 1, 256, 1, 1, 0, stream, params, nullptr),
+                   "hipModuleLaunchKernel(rope)");
+    }
+    return HH_OK;
+}
+
+hh_status hh_engine::enqueue_kv_copy(size_t layers, const hh_kv_copy_args& a) {
+    hipFunction_t f;
+    HH_TRY(kernel("hh_kv_copy", &f));
+    const size_t cus = (size_t)props.multiProcessorCount, blocks = (a.chunks + 255) / 256;
+    // Moves are also split where the pages' pieces give fewer than eight workgroups a CU, and a bit for each page
+    // fits 32 KB of LDS.
+    size_t parts = 1, lds = 0;
+    if (a.kv.pages <= (1u << 18) && blocks * layers < 8 * cus) {
+        parts = std::min<size_t>((a.n + 7) / 8, 8 * cus / (blocks * layers));
+        if (parts > 1) lds = (a.kv.pages + 31) / 32 * 4;
+    }
+    hh_kv_copy_args p = a;
+    void* params[] = {&p};
+    HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)blocks, (uint32_t)layers, (uint32_t)std::max<size_t>(parts, 1), 256, 1, 1,
+                                     (unsigned)lds, stream, params, nullptr),
+               "hipModuleLaunchKernel(kv_copy)");
+    return HH_OK;
+}

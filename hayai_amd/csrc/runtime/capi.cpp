@@ -1,5 +1,6 @@
 // extern "C" surface declared in include/hayai_hip.h.
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -937,6 +938,159 @@ hh_status hh_sample_dev(hh_engine* e, const hh_sample_desc* d, const hh_buf* log
     try {
         std::lock_guard<std::mutex> lk(e->ws_mutex);
         return e->enqueue_sample(d->type, d->rows, a);
+    } catch (const std::bad_alloc&) {
+        return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
+}
+
+// ---------------------------------------------------------------- attention ----------
+
+// The cache's pages in a device-visible buffer of the engine, `layers` caches *layer_stride elements apart.
+static hh_status check_kv(hh_engine* e, const hh_kv_desc* kv, const hh_buf* cache, size_t off, size_t layers,
+                          size_t* layer_stride, hh_kv_args* out, const char* what) {
+    HH_NOT_NULL(kv, "kv desc");
+    HH_TRY(check_act_type(kv->type, what));
+    const size_t el = act_type(kv->type)->bytes;
+    if (kv->kv_heads < 1 || kv->kv_heads > 1024)
+        return fail(HH_ERR_INVALID, "%s: kv_heads=%zu outside 1..1024", what, kv->kv_heads);
+    if (kv->head_dim < 8 || kv->head_dim > 256 || kv->head_dim % 8)
+        return fail(HH_ERR_INVALID, "%s: head_dim=%zu is no multiple of 8 in 8..256", what, kv->head_dim);
+    if (kv->page_size < 16 || kv->page_size > 256 || (kv->page_size & (kv->page_size - 1)))
+        return fail(HH_ERR_INVALID, "%s: page_size=%zu is no power of two in 16..256", what, kv->page_size);
+    if (kv->n_pages < 1 || kv->n_pages > INT32_MAX / kv->page_size)
+        return fail(HH_ERR_INVALID, "%s: %zu pages of %zu tokens", what, kv->n_pages, kv->page_size);
+    const size_t page = 2 * kv->kv_heads * kv->head_dim * kv->page_size;
+    const size_t stride = kv->page_stride ? kv->page_stride : page;
+    if (stride < page) return fail(HH_ERR_INVALID, "%s: page_stride %zu < %zu elements of a page", what, stride, page);
+    if (stride > SIZE_MAX / el / kv->n_pages) return fail(HH_ERR_INVALID, "%s: size overflow", what);
+    if (*layer_stride == 0) *layer_stride = stride * kv->n_pages;
+    HH_TRY(check_engine(e, cache, what));
+    const size_t last = ((kv->n_pages - 1) * stride + page) * el;
+    if (layers > 1 && *layer_stride > (SIZE_MAX - last) / el / (layers - 1))
+        return fail(HH_ERR_INVALID, "%s: size overflow", what);
+    HH_TRY(check_range(cache, off, (layers - 1) * *layer_stride * el + last, what));
+    if ((((uintptr_t)cache->ptr + off) | stride * el | (layers > 1 ? *layer_stride * el : 0)) % 16)
+        return fail(HH_ERR_INVALID, "%s: pages must start on 16-byte boundaries (strides %zu, %zu)", what, stride,
+                    *layer_stride);
+    out->base = (uint8_t*)cache->ptr + off;
+    out->stride = stride * el;
+    out->pages = (uint32_t)kv->n_pages;
+    out->shift = (uint32_t)__builtin_ctzll(kv->page_size);
+    out->heads = (uint32_t)kv->kv_heads;
+    out->dim = (uint32_t)kv->head_dim;
+    return HH_OK;
+}
+
+static hh_status check_kv_type(int type, const hh_kv_desc* kv, const char* what) {
+    HH_NOT_NULL(kv, "kv desc");
+    HH_TRY(check_act_type(type, what));
+    HH_TRY(check_act_type(kv->type, what));
+    if (kv->type != type && type != HH_TYPE_F32)
+        return fail(HH_ERR_KERNEL_MISSING, "%s: no kernel for activations of GGML type %d over a cache of type %d", what,
+                    type, kv->type);
+    return HH_OK;
+}
+
+hh_status hh_rope_kv_dev(hh_engine* e, const hh_rope_desc* d, const hh_kv_desc* kv, const hh_buf* q, size_t q_off,
+                         const hh_buf* k, size_t k_off, const hh_buf* v, size_t v_off, const hh_buf* positions,
+                         size_t positions_off, const hh_buf* slots, size_t slots_off, const hh_buf* factors,
+                         size_t factors_off, hh_buf* out, size_t out_off, hh_buf* cache, size_t cache_off) {
+    HH_NOT_NULL(e, "engine");
+    HH_NOT_NULL(d, "rope desc");
+    HH_TRY(check_kv_type(d->type, kv, "rope_kv"));
+    hh_rope_args a{};
+    size_t layer = 0;
+    HH_TRY(check_kv(e, kv, cache, cache_off, 1, &layer, &a.kv, "rope_kv cache"));
+    if (d->layout != HH_ROPE_HALVES && d->layout != HH_ROPE_PAIRS)
+        return fail(HH_ERR_INVALID, "rope_kv: unknown layout %d", d->layout);
+    if (d->q_heads > 65535) return fail(HH_ERR_INVALID, "rope_kv: q_heads=%zu > 65535", d->q_heads);
+    if (d->rot_dim > kv->head_dim || d->rot_dim % 2)
+        return fail(HH_ERR_INVALID, "rope_kv: rot_dim=%zu is not even in 0..%zu", d->rot_dim, kv->head_dim);
+    if (!(d->base > 0) || !std::isfinite(d->base) || !std::isfinite(d->mscale))
+        return fail(HH_ERR_INVALID, "rope_kv: base=%g mscale=%g", d->base, (double)d->mscale);
+    const size_t el = act_type(d->type)->bytes, cols = kv->kv_heads * kv->head_dim, qcols = d->q_heads * kv->head_dim;
+    HH_TRY(check_sizes(d->tokens, cols, "rope_kv"));
+    size_t qs = d->q_stride, ks = d->k_stride, vs = d->v_stride, os = d->out_stride;
+    if (d->q_heads) {
+        HH_TRY(check_rows(e, q, q_off, d->tokens, qcols, el, &qs, "rope_kv q"));
+        HH_TRY(check_rows(e, out, out_off, d->tokens, qcols, el, &os, "rope_kv out"));
+    }
+    HH_TRY(check_rows(e, k, k_off, d->tokens, cols, el, &ks, "rope_kv k"));
+    HH_TRY(check_rows(e, v, v_off, d->tokens, cols, el, &vs, "rope_kv v"));
+    HH_TRY(check_vector(e, positions, positions_off, d->tokens, "rope_kv positions"));
+    HH_TRY(check_vector(e, slots, slots_off, d->tokens, "rope_kv slots"));
+    if (factors) HH_TRY(check_vector(e, factors, factors_off, d->rot_dim / 2, "rope_kv factors"));
+    if (d->tokens == 0) return HH_OK;
+    HH_TRY(e->select());
+    a.q = at(q, q_off);
+    a.k = at(k, k_off);
+    a.v = at(v, v_off);
+    a.out = at(out, out_off);
+    a.positions = (const int32_t*)at(positions, positions_off);
+    a.slots = (const int32_t*)at(slots, slots_off);
+    a.factors = (const float*)at(factors, factors_off);
+    a.q_stride = qs;
+    a.k_stride = ks;
+    a.v_stride = vs;
+    a.out_stride = os;
+    a.log2_base = std::log2(d->base);
+    a.mscale = d->mscale;
+    a.heads = (uint32_t)d->q_heads;
+    a.rot = (uint32_t)d->rot_dim;
+    try {
+        return e->enqueue_rope(d->type, kv->type, d->layout, d->tokens, a);
+    } catch (const std::bad_alloc&) {
+        return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
+}
+
+hh_status hh_rope_factors(int scaling, size_t rot_dim, double base, double scale, double trained, float* factors,
+                          float* mscale) {
+    HH_NOT_NULL(factors, "factors");
+    if (scaling != HH_ROPE_LINEAR && scaling != HH_ROPE_BY_WAVELENGTH && scaling != HH_ROPE_YARN)
+        return fail(HH_ERR_INVALID, "rope_factors: unknown scaling %d", scaling);
+    if (rot_dim < 2 || rot_dim > 256 || rot_dim % 2)
+        return fail(HH_ERR_INVALID, "rope_factors: rot_dim=%zu is not even in 2..256", rot_dim);
+    if (!(base > 1) || !std::isfinite(base) || !(scale >= 1) || !std::isfinite(scale) || !(trained >= 1) ||
+        !std::isfinite(trained))
+        return fail(HH_ERR_INVALID, "rope_factors: base=%g scale=%g trained=%g", base, scale, trained);
+    const double n = (double)(rot_dim / 2), tau = 6.283185307179586476925;
+    // the pair that turns `times` times over the trained length
+    auto pair_of = [&](double times) { return n * std::log(trained / (times * tau)) / std::log(base); };
+    const double lo = std::min(std::max(std::floor(pair_of(32)), 0.0), (double)rot_dim - 1);
+    const double hi = std::min(std::max(std::ceil(pair_of(1)), 0.0), (double)rot_dim - 1);
+    for (size_t i = 0; i < rot_dim / 2; i++) {
+        double f = scale;
+        if (scaling == HH_ROPE_BY_WAVELENGTH) {
+            const double turns = trained / (tau * std::pow(base, (double)i / n));
+            const double s = std::min(std::max((turns - 1) / 3, 0.0), 1.0);
+            f = 1 / ((1 - s) / scale + s);
+        } else if (scaling == HH_ROPE_YARN) {
+            const double r = std::min(std::max(((double)i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+            f = 1 / ((1 - r) + r / scale);
+        }
+        factors[i] = (float)f;
+    }
+    if (mscale) *mscale = scaling == HH_ROPE_YARN ? (float)(1 + 0.1 * std::log(scale)) : 1.f;
+    return HH_OK;
+}
+
+hh_status hh_kv_copy_dev(hh_engine* e, const hh_kv_desc* kv, size_t layers, size_t layer_stride, hh_buf* cache,
+                         size_t cache_off, const hh_buf* moves, size_t moves_off, size_t n) {
+    HH_NOT_NULL(e, "engine");
+    if (layers < 1 || layers > 65535) return fail(HH_ERR_INVALID, "kv_copy: layers=%zu outside 1..65535", layers);
+    hh_kv_copy_args a{};
+    HH_TRY(check_kv(e, kv, cache, cache_off, layers, &layer_stride, &a.kv, "kv_copy cache"));
+    if (n > INT32_MAX) return fail(HH_ERR_INVALID, "kv_copy: %zu moves exceed 31 bits", n);
+    HH_TRY(check_vector(e, moves, moves_off, 2 * n, "kv_copy moves"));
+    if (n == 0) return HH_OK;
+    HH_TRY(e->select());
+    a.moves = (const int32_t*)at(moves, moves_off);
+    a.layer_stride = layer_stride * act_type(kv->type)->bytes;
+    a.n = (uint32_t)n;
+    a.chunks = (uint32_t)(2 * kv->kv_heads * kv->head_dim * kv->page_size * act_type(kv->type)->bytes / 16);
+    try {
+        return e->enqueue_kv_copy(layers, a);
     } catch (const std::bad_alloc&) {
         return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
     }

@@ -11,6 +11,7 @@
 // gfx950 code object embedded by blob.S (.incbin of the --genco output).
 extern "C" const unsigned char hh_kernels_blob[];
 extern "C" const unsigned char hh_kernels_blob_end[];
+extern "C" const unsigned char hh_attn_blob[];
 
 namespace hh {
 
@@ -113,7 +114,7 @@ hh_status hh_engine::kernel(const std::string& name, hipFunction_t* out) {
         return HH_OK;
     }
     hipFunction_t f = nullptr;
-    hipError_t err = hipModuleGetFunction(&f, module, name.c_str());
+    hipError_t err = hipModuleGetFunction(&f, attn_kernel(name) ? attn_module : module, name.c_str());
     if (err != hipSuccess || !f)
         return fail(HH_ERR_KERNEL_MISSING, "kernel %s missing from the gfx950 code object", name.c_str());
     fns[name] = f;
@@ -2101,6 +2102,7 @@ static std::vector<std::string> required_kernels() {
     for (int t : {16, 32, 64})
         for (const char* kind : {"hh_moe_gateup_t", "hh_moe_down_t"}) k.push_back(std::string(kind) + std::to_string(t));
     i8_kernels(k);
+    attn_kernels(k);
     return k;
 }
 
@@ -2118,6 +2120,7 @@ hh_status engine_create(int device, hh_engine** out) {
         if (e->copy_stream) (void)hipStreamDestroy(e->copy_stream);
     if (e->copy_stream2) (void)hipStreamDestroy(e->copy_stream2);
         if (e->module) (void)hipModuleUnload(e->module);
+        if (e->attn_module) (void)hipModuleUnload(e->attn_module);
         delete e;
         return st;
     };
@@ -2132,6 +2135,7 @@ hh_status engine_create(int device, hh_engine** out) {
         err = hipModuleLoad(&e->module, path);
     else
         err = hipModuleLoadData(&e->module, hh_kernels_blob);
+    if (err == hipSuccess) err = hipModuleLoadData(&e->attn_module, hh_attn_blob);
     if (err != hipSuccess) return bail(hip_fail(err, "hipModuleLoad(gfx950 code object)"));
     err = hipStreamCreateWithFlags(&e->stream, hipStreamNonBlocking);
     if (err != hipSuccess) return bail(hip_fail(err, "hipStreamCreate(compute)"));
@@ -2192,5 +2196,6 @@ void engine_destroy(hh_engine* e) {
     if (e->copy_stream) (void)hipStreamDestroy(e->copy_stream);
     if (e->copy_stream2) (void)hipStreamDestroy(e->copy_stream2);
     if (e->module) (void)hipModuleUnload(e->module);
+    if (e->attn_module) (void)hipModuleUnload(e->attn_module);
     delete e;
 }

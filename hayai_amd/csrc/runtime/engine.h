@@ -66,6 +66,11 @@ struct ActType {
 const ActType* act_type(int ggml_type);
 // Names of the 8-bit path's kernels, for the check at engine creation.
 void i8_kernels(std::vector<std::string>& names);
+// The same of the attention operators, whether a name is one of theirs (they have a code object of their own),
+// and the kernel-name stem of a pair of activations' and cache's types.
+void attn_kernels(std::vector<std::string>& names);
+bool attn_kernel(const std::string& name);
+std::string attn_types(int type, int kv_type);
 
 // The device address of noalloc.hip's fixed scratch array on `device` (which must be the
 // current device): looked up once per device and kept.
@@ -103,6 +108,7 @@ struct hh_engine {
     int device = 0;
     hipDeviceProp_t props{};
     hipModule_t module = nullptr;
+    hipModule_t attn_module = nullptr;  // the attention operators' kernels
     hipStream_t stream = nullptr;       // compute stream (default priority)
     hipStream_t copy_stream = nullptr;  // side stream for host<->device DMA
     hipStream_t copy_stream2 = nullptr; // second DMA stream: large streamer copies split in two
@@ -345,6 +351,9 @@ struct hh_engine {
     hh_status enqueue_i8_rows(int type, size_t rows, const hh_i8_rows_args& a);
     hh_status enqueue_i8_gemm(int type, hh_i8_gemm_args a);
     hh_status enqueue_sample(int type, size_t rows, hh_sample_args a);
+    // Attention over pages (attn.cpp).
+    hh_status enqueue_rope(int type, int kv_type, int layout, size_t tokens, const hh_rope_args& a);
+    hh_status enqueue_kv_copy(size_t layers, const hh_kv_copy_args& a);
     // Reports (and clears) a grid-barrier timeout recorded by a fused kernel.  Syncs.
     hh_status check_device_error();
 };

@@ -24,8 +24,10 @@ import numpy as np
 from . import _abi
 
 F32, F16, Q4_0, Q8_0, Q4_K, Q6_K, IQ2_XXS, IQ3_XXS = 0, 1, 2, 8, 12, 14, 16, 18
-BF16 = 30  # activations of the 8-bit operators
+BF16 = 30  # activations of the 8-bit and attention operators
 ACT_SILU, ACT_GELU_TANH = 0, 1
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+ROPE_LINEAR, ROPE_BY_WAVELENGTH, ROPE_YARN = 0, 1, 2
 BUF_DEVICE, BUF_PINNED_HOST = 0, 1
 TYPE_NAMES = {F32: "f32", F16: "f16", Q4_0: "q4_0", Q8_0: "q8_0", Q4_K: "q4_k", Q6_K: "q6_k", IQ2_XXS: "iq2_xxs",
               IQ3_XXS: "iq3_xxs"}
@@ -71,6 +73,13 @@ def device_count() -> int:
     n = C.c_int(0)
     _check(_abi.load().hh_device_count(C.byref(n)))
     return n.value
+
+
+def rope_factors(scaling: int, rot_dim: int, base: float, scale: float, trained: float = 1.0) -> tuple[np.ndarray, float]:
+    """(factors, mscale) of a context `scale` times longer than the trained one (hh_rope_factors)."""
+    factors, mscale = np.empty(max(rot_dim // 2, 1), np.float32), C.c_float(0)
+    _check(_abi.load().hh_rope_factors(scaling, rot_dim, base, scale, trained, _ptr(factors), C.byref(mscale)))
+    return factors, mscale.value
 
 
 class DeviceBuffer:
@@ -731,6 +740,36 @@ class HipEngine:
         random number u): ids int32, probs f32.  Enqueue only."""
         _check(self.lib.hh_sample_dev(self.handle, C.byref(desc), logits.handle, logits_off, params.handle, params_off,
                                       u.handle, u_off, ids.handle, ids_off, _handle(probs), probs_off))
+
+    # ---------------------------------------------------------------- attention
+    # No counterpart in the reference's device runtime; the definitions stand in include/hayai_hip.h.
+    @staticmethod
+    def kv_desc(ggml_type: int, kv_heads: int, head_dim: int, page_size: int, n_pages: int,
+                page_stride: int = 0) -> _abi.KvDesc:
+        """A cache's pages: keys as [kv_heads][page_size][head_dim], then values as [kv_heads][head_dim][page_size]."""
+        return _abi.KvDesc(ggml_type, kv_heads, head_dim, page_size, n_pages, page_stride)
+
+    @staticmethod
+    def rope_desc(ggml_type: int, tokens: int, q_heads: int, rot_dim: int, base: float = 10000.0, q_stride: int = 0,
+                  k_stride: int = 0, v_stride: int = 0, out_stride: int = 0, layout: int = ROPE_HALVES,
+                  mscale: float = 1.0) -> _abi.RopeDesc:
+        return _abi.RopeDesc(ggml_type, layout, tokens, q_heads, rot_dim, base, mscale, q_stride, k_stride, v_stride,
+                             out_stride)
+
+    def rope_kv_dev(self, desc: _abi.RopeDesc, kv: _abi.KvDesc, q, q_off: int, k: DeviceBuffer, k_off: int,
+                    v: DeviceBuffer, v_off: int, positions: DeviceBuffer, positions_off: int, slots: DeviceBuffer,
+                    slots_off: int, factors, factors_off: int, out, out_off: int, cache: DeviceBuffer,
+                    cache_off: int) -> None:
+        """q (to out) and k turned by the tokens' positions, k and v into the cache's slots.  Enqueue only."""
+        _check(self.lib.hh_rope_kv_dev(self.handle, C.byref(desc), C.byref(kv), _handle(q), q_off, k.handle, k_off,
+                                       v.handle, v_off, positions.handle, positions_off, slots.handle, slots_off,
+                                       _handle(factors), factors_off, _handle(out), out_off, cache.handle, cache_off))
+
+    def kv_copy_dev(self, kv: _abi.KvDesc, cache: DeviceBuffer, cache_off: int, moves: DeviceBuffer, moves_off: int,
+                    n: int, layers: int = 1, layer_stride: int = 0) -> None:
+        """Pages moves[i] = (from, to) copied in each layer, as if one after another.  Enqueue only."""
+        _check(self.lib.hh_kv_copy_dev(self.handle, C.byref(kv), layers, layer_stride, cache.handle, cache_off,
+                                       moves.handle, moves_off, n))
 
     # ---------------------------------------------------------------- synthetic data
     def synth_weights_dev(self, ggml_type: int, dst: DeviceBuffer, off: int, n_blocks: int, seed: int,

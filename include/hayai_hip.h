@@ -63,7 +63,7 @@ enum {
     HH_TYPE_Q6_K = 14,
     HH_TYPE_IQ2_XXS = 16,
     HH_TYPE_IQ3_XXS = 18,
-    /* activations of the 8-bit operators only (no GEMV over BF16 weights) */
+    /* activations of the 8-bit and attention operators only (no GEMV over BF16 weights) */
     HH_TYPE_BF16 = 30
 };
 
@@ -117,7 +117,8 @@ hh_status hh_validate_gemv_weights(int ggml_type, size_t m, size_t n, size_t wei
 hh_status hh_device_count(int* count);
 
 /* Bring up one device: select it, load the gfx950 code object (embedded in this library,
- * or the file named by HAYAI_HIP_CODE_OBJECT) with hipModuleLoadData/hipModuleLoad,
+ * or the file named by HAYAI_HIP_CODE_OBJECT; the attention operators' own always the embedded one)
+ * with hipModuleLoadData/hipModuleLoad,
  * resolve every kernel, create the compute and copy streams.  Fails with
  * HH_ERR_UNSUPPORTED_DEVICE on a non-gfx950 device and HH_ERR_KERNEL_MISSING if a kernel
  * is absent from the code object.  Replaces OpenClEngine::init_device
@@ -499,6 +500,81 @@ typedef struct hh_sample_desc {
 hh_status hh_sample_dev(hh_engine* e, const hh_sample_desc* d, const hh_buf* logits, size_t logits_off,
                         const hh_buf* params, size_t params_off, const hh_buf* u, size_t u_off, hh_buf* ids,
                         size_t ids_off, hh_buf* probs, size_t probs_off);
+
+/* ------------------------------------------------------------------ attention ------- */
+
+/* No counterpart in the reference's device runtime (its attention runs on the CPU).  What a layer
+ * does between the products of its queries, keys and values and that of its output, over a cache of
+ * pages: hh_rope_kv_dev turns queries and keys by their positions and puts keys and values into the
+ * cache, hh_kv_copy_dev copies pages (forked sequences, a cache made dense again).
+ *
+ * Activations are of `type`, as in the 8-bit path (element-aligned byte offsets, rows `*_stride`
+ * elements apart, 0: packed); a row holds its token's heads one after another, kv.head_dim elements
+ * each.  The cache is of the same type, or of HH_TYPE_F16 or HH_TYPE_BF16 under HH_TYPE_F32
+ * activations; other pairs are HH_ERR_KERNEL_MISSING.  Page numbers, slots, positions and lengths are
+ * int32 on the device, read when the kernels run, so a captured graph follows what they hold at its
+ * replay; none of them can lead a kernel outside the buffers that were named.  All calls are
+ * enqueue-only and give the same bits every time.  Buffers of one call must not overlap except where
+ * said. */
+
+/* A cache of n_pages pages, page p `page_stride` elements after page p - 1 (0: packed).  A page has
+ * room for page_size tokens: their keys as [kv_heads][page_size][head_dim], then their values turned,
+ * as [kv_heads][head_dim][page_size].  The cache's offset and page_stride are multiples of 16 bytes.
+ * Token t of a sequence is in slot t % page_size of the page that entry t / page_size of its table
+ * names.  A larger page_stride lets the layers' pages lie next to each other. */
+typedef struct hh_kv_desc {
+    int type;           /* HH_TYPE_F32, HH_TYPE_F16 or HH_TYPE_BF16 */
+    size_t kv_heads;    /* 1..1024 */
+    size_t head_dim;    /* a multiple of 8, 8..256 */
+    size_t page_size;   /* 16, 32, 64, 128 or 256 */
+    size_t n_pages;     /* >= 1; n_pages * page_size < 2^31 */
+    size_t page_stride; /* elements, >= 2 * kv_heads * page_size * head_dim; 0: that */
+} hh_kv_desc;
+
+/* Which elements of a head turn together: x[i] with x[i + rot/2], or x[2i] with x[2i + 1]. */
+enum { HH_ROPE_HALVES = 0, HH_ROPE_PAIRS = 1 };
+
+/* Queries and keys turned: the first rot_dim elements of each head in pairs i < rot_dim / 2 by the
+ * angle position * base^(-2i / rot_dim) / factors[i] (taken in 64 bits), times mscale; the head's other
+ * elements go through.  out receives the queries (and may be q: same offset and stride), the cache's
+ * slot page * page_size + t receives the token's keys and values.  slots[token] outside the cache (-1,
+ * say) stores nothing.  Tokens of one call have different slots: of two with the same one either's
+ * elements may stay.  factors (rot_dim / 2 f32, or NULL: all 1): a model file's frequency factors, or
+ * hh_rope_factors'.  Positions may be negative. */
+typedef struct hh_rope_desc {
+    int type;          /* of q, k, v and out */
+    int layout;        /* HH_ROPE_* */
+    size_t tokens;
+    size_t q_heads;    /* 0..65535 */
+    size_t rot_dim;    /* even, 0..head_dim */
+    double base;       /* > 0, finite */
+    float mscale;      /* finite; 1 as a rule */
+    size_t q_stride, k_stride, v_stride, out_stride; /* elements */
+} hh_rope_desc;
+hh_status hh_rope_kv_dev(hh_engine* e, const hh_rope_desc* d, const hh_kv_desc* kv, const hh_buf* q, size_t q_off,
+                         const hh_buf* k, size_t k_off, const hh_buf* v, size_t v_off, const hh_buf* positions,
+                         size_t positions_off, const hh_buf* slots, size_t slots_off, const hh_buf* factors,
+                         size_t factors_off, hh_buf* out, size_t out_off, hh_buf* cache, size_t cache_off);
+
+/* Frequency factors and mscale of the usual ways to reach past the length a model was trained on
+ * (host memory, no device needed).  scale (>= 1): by how much; trained: that length; n = rot_dim / 2,
+ * w(i) = 2 pi base^(i / n) the wavelength of pair i.
+ *   HH_ROPE_LINEAR         factors = scale
+ *   HH_ROPE_BY_WAVELENGTH  1 where trained / w >= 4, scale where trained / w <= 1, between them
+ *                          1 / ((1 - s) / scale + s), s = (trained / w - 1) / 3
+ *   HH_ROPE_YARN           1 / ((1 - r) + r / scale), r = (i - lo) / max(hi - lo, 0.001) in 0..1, lo and hi the
+ *                          pairs (rounded down and up, in 0..rot_dim - 1) that turn 32 times and once over
+ *                          `trained`; mscale = 1 + 0.1 ln scale (else 1)
+ * factors: rot_dim / 2 floats; mscale may be NULL. */
+enum { HH_ROPE_LINEAR = 0, HH_ROPE_BY_WAVELENGTH = 1, HH_ROPE_YARN = 2 };
+hh_status hh_rope_factors(int scaling, size_t rot_dim, double base, double scale, double trained, float* factors,
+                          float* mscale);
+
+/* Pages copied in `layers` caches, `layer_stride` elements apart (a multiple of 16 bytes; 0: n_pages *
+ * page_stride): moves is int32[n][2], (from, to), taken as if one after another.  A move with a page outside [0, n_pages) does
+ * nothing, so lists may be padded with -1. */
+hh_status hh_kv_copy_dev(hh_engine* e, const hh_kv_desc* kv, size_t layers, size_t layer_stride, hh_buf* cache,
+                         size_t cache_off, const hh_buf* moves, size_t moves_off, size_t n);
 
 /* ------------------------------------------------------------------ streaming ------- */
 

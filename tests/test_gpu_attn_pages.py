@@ -1,0 +1,206 @@
+"""GPU tests of the cache's entry points: rotary positions into the cache (rope_kv) and copies of its
+pages (kv_copy), against their definitions in 64 bits.
+
+A turned element is a cos - b sin with cos and sin rounded to f32 once (2^-24 each, times mscale), one
+product, one fused multiply-add: off by less than (|a| + |b|) * 2^-24 * 4, then one rounding to the
+output's type (eps / 2 of the value).  What only goes through is rounded once.
+"""
+import numpy as np
+import pytest
+import torch
+
+import hayai_amd
+from hayai_amd import BF16, F16, F32, ROPE_HALVES, ROPE_PAIRS
+
+pytestmark = pytest.mark.gpu
+
+DT = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}
+TYPES = [(F32, F32), (F16, F16), (BF16, BF16), (F32, F16), (F32, BF16)]
+
+
+def normal(seed, *shape, scale=1.0):
+    return torch.from_numpy(np.random.default_rng(seed).standard_normal(shape) * scale)
+
+
+def put(engine, t, lead=0):
+    t = t.contiguous()
+    raw = t.view(torch.uint8).numpy().reshape(-1) if t.numel() else np.zeros(0, np.uint8)
+    b = engine.alloc(max(lead + raw.size, 1))
+    if raw.size:
+        b.write(raw, lead)
+    return b
+
+
+def ints(engine, values, lead=0):
+    return put(engine, torch.tensor(values, dtype=torch.int32), lead)
+
+
+def get(b, dtype, shape, lead=0):
+    n = int(np.prod(shape))
+    if n == 0:
+        return torch.empty(shape, dtype=dtype)
+    raw = b.read(np.uint8, n * torch.empty(0, dtype=dtype).element_size(), lead)
+    return torch.from_numpy(raw).view(dtype).reshape(shape)
+
+
+def turned(x, positions, rot, base, layout, factors, mscale):
+    """x: (tokens, heads, dim) in 64 bits."""
+    y = x.clone()
+    i = np.arange(rot // 2)
+    w = base ** (-2.0 * i / max(rot, 1))
+    if factors is not None:
+        w = w / factors.astype(np.float64)
+    angle = torch.from_numpy(np.outer(positions.astype(np.float64), w))[:, None, :]
+    c, s = torch.cos(angle) * mscale, torch.sin(angle) * mscale
+    a_at, b_at = (i, i + rot // 2) if layout == ROPE_HALVES else (2 * i, 2 * i + 1)
+    a, b = x[..., a_at], x[..., b_at]
+    y[..., a_at], y[..., b_at] = a * c - b * s, a * s + b * c
+    return y
+
+
+def near(got, want, dtype, slack):
+    err = (got.double() - want).abs()
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # a step below the normal range
+    bound = slack * (1 + torch.finfo(dtype).eps) + want.abs() * torch.finfo(dtype).eps / 2 + tiny
+    assert torch.all(err <= bound), (err / bound).max()
+
+
+# tokens, q heads, kv heads, dim, rot, page, strides beyond a row, byte lead
+SHAPES = [(1, 9, 3, 64, 64, 16, 0, 0), (1, 32, 8, 128, 128, 64, 0, 0), (5, 4, 4, 72, 36, 32, 3, 4), (3, 0, 1, 8, 0, 16, 0, 0),
+          (61, 8, 1, 128, 64, 64, 0, 0), (7, 3, 1, 80, 80, 256, 1, 8), (2, 2, 2, 256, 256, 128, 5, 4),
+          (300, 6, 2, 40, 2, 16, 0, 0), (2, 64, 8, 96, 18, 64, 0, 0)]
+
+
+@pytest.mark.parametrize("layout", [ROPE_HALVES, ROPE_PAIRS])
+@pytest.mark.parametrize("ty,cty", TYPES)
+def test_rope(engine, ty, cty, layout):
+    for case, (t, heads, kvh, dim, rot, page, pad, lead) in enumerate(SHAPES):
+        print(f"[case] rope {ty} {cty} {layout} {SHAPES[case]}", flush=True)
+        rng = np.random.default_rng(case)
+        el = torch.empty(0, dtype=DT[ty]).element_size()
+        lead = lead // el * el
+        cols, base, mscale = (heads + 2 * kvh) * dim, 10000.0, float(np.float32([1.0, 1.25][case % 2]))
+        x = normal(case, t, cols + pad, scale=2.0).to(DT[ty])
+        n_pages = t // page + 3
+        # far positions, negative ones, slots outside the cache
+        positions = rng.integers(-3, [200, 200000, 2**31 - 1][case % 3], t).astype(np.int32)
+        slots = rng.permutation(n_pages * page)[:t].astype(np.int32)
+        if t > 2:
+            slots[1], slots[2] = -1, n_pages * page
+        factors = (1 + 7 * rng.random(rot // 2)).astype(np.float32) if case % 2 and rot else None
+        per = 2 * kvh * page * dim
+        stride = per + (16 if case % 2 else 0)
+        cache = normal(case + 100, n_pages, stride).to(DT[cty])
+        xb, cb = put(engine, x, lead), put(engine, cache)
+        out = put(engine, torch.full((t, heads * dim + pad), 9.0).to(DT[ty]), lead)
+        pb, sb = ints(engine, positions.tolist(), 4), ints(engine, slots.tolist())
+        fb = None if factors is None else put(engine, torch.from_numpy(factors))
+        d = engine.rope_desc(ty, t, heads, rot, base, q_stride=cols + pad, k_stride=cols + pad, v_stride=cols + pad,
+                             out_stride=heads * dim + pad, layout=layout, mscale=mscale)
+        kv = engine.kv_desc(cty, kvh, dim, page, n_pages, stride if case % 2 else 0)
+        engine.rope_kv_dev(d, kv, xb if heads else None, lead, xb, lead + heads * dim * el, xb,
+                           lead + (heads + kvh) * dim * el, pb, 4, sb, 0, fb, 0, out if heads else None, lead, cb, 0)
+        x64 = x[:, :cols].double().reshape(t, heads + 2 * kvh, dim)
+        want = turned(x64[:, :heads + kvh], positions, rot, base, layout, factors, mscale)
+        # the two products' and their sum's roundings: |a| + |b| of a pair, at most sqrt(2) of its length
+        size = (x64[:, :heads + kvh] ** 2).sum(-1, keepdim=True).sqrt().expand_as(want) * 1.5 * mscale * 4 * 2.0**-24
+        size[..., rot:] = 0
+        got = get(out, DT[ty], (t, heads * dim + pad), lead)
+        near(got[:, :heads * dim].reshape(t, heads, dim), want[:, :heads], DT[ty], size[:, :heads])
+        assert torch.all(got[:, heads * dim:] == 9.0)
+        new = get(cb, DT[cty], (n_pages, stride))
+        expect, slack = cache.double().clone(), torch.zeros(n_pages, stride, dtype=torch.float64)
+        for i, slot in enumerate(slots.tolist()):
+            if not 0 <= slot < n_pages * page:
+                continue
+            p, at = divmod(slot, page)
+            expect[p, :per // 2].view(kvh, page, dim)[:, at] = want[i, heads:]
+            slack[p, :per // 2].view(kvh, page, dim)[:, at] = size[i, heads:]
+            expect[p, per // 2:per].view(kvh, dim, page)[:, :, at] = x64[i, heads + kvh:]
+        near(new, expect, DT[cty], slack)
+        untouched = torch.ones(n_pages, stride, dtype=torch.bool)
+        for slot in slots.tolist():
+            if 0 <= slot < n_pages * page:
+                p, at = divmod(slot, page)
+                untouched[p, :per // 2].view(kvh, page, dim)[:, at] = False
+                untouched[p, per // 2:per].view(kvh, dim, page)[:, :, at] = False
+        assert torch.equal(new[untouched], cache[untouched])
+
+
+def test_rope_in_place(engine):
+    t, heads, kvh, dim, page = 130, 12, 2, 128, 16
+    for layout in (ROPE_HALVES, ROPE_PAIRS):
+        x = normal(7, t, (heads + 2 * kvh) * dim).to(torch.bfloat16)
+        outs = []
+        for in_place in (False, True):
+            xb, cb = put(engine, x), engine.alloc(20 * 2 * kvh * page * dim * 2)
+            cb.fill(0)
+            out = xb if in_place else engine.alloc(x.numel() * 2)
+            wide = x.shape[1]
+            d = engine.rope_desc(BF16, t, heads, dim, q_stride=wide, k_stride=wide, v_stride=wide, out_stride=wide, layout=layout)
+            kv = engine.kv_desc(BF16, kvh, dim, page, 20)
+            engine.rope_kv_dev(d, kv, xb, 0, xb, heads * dim * 2, xb, (heads + kvh) * dim * 2, ints(engine, list(range(t))), 0,
+                               ints(engine, list(range(t))), 0, None, 0, out, 0, cb, 0)
+            outs.append((get(out, torch.bfloat16, (t, wide))[:, :heads * dim], get(cb, torch.bfloat16, (20, 2 * kvh * page * dim))))
+        assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+def copied(cache, moves, n_pages, per):
+    out = cache.copy()
+    for s, d in moves:
+        if 0 <= s < n_pages and 0 <= d < n_pages:
+            out[:, d, :per] = out[:, s, :per]
+    return out
+
+
+# heads, dim, page, pages, layers, moves: few and many, in layers enough to keep all in one part or not
+COPIES = [(1, 8, 16, 2, 1, 1), (3, 64, 16, 300, 1, 5), (8, 128, 64, 20, 2, 9), (2, 72, 32, 50, 3, 100), (1, 64, 16, 40, 5, 257),
+          (8, 256, 256, 6, 4, 3), (1, 8, 16, 300000, 1, 40)]
+
+
+@pytest.mark.parametrize("kind", ["forks", "holes", "chain", "any"])
+def test_kv_copy(engine, kind):
+    for case, (kvh, dim, page, n_pages, layers, n) in enumerate(COPIES):
+        print(f"[case] kv_copy {kind} {COPIES[case]}", flush=True)
+        rng = np.random.default_rng(case)
+        at = rng.permutation(n_pages)
+        if kind in ("forks", "holes"):
+            n = min(n, n_pages // 2)
+            source = at[rng.integers(0, max(1, n // 3), n)] if kind == "forks" else at[:n]
+            moves = np.stack([source, at[n_pages - n:]], 1)
+        elif kind == "chain":  # every page one down, the first to the end
+            n = min(n, n_pages - 1)
+            moves = np.stack([np.arange(1, n + 1), np.arange(n)], 1)
+        else:  # pages twice, pages outside, padding
+            moves = rng.integers(-2, min(n_pages, 12) + 2, (n, 2))
+            moves[moves >= min(n_pages, 12)] += n_pages
+            moves = np.concatenate([moves, [[-1, -1], [0, -1], [-1, 0]]])
+        per = 2 * kvh * dim * page
+        stride = per + 8 * (case % 3)
+        cache = rng.integers(0, 1 << 16, (layers, n_pages, stride), dtype=np.uint16)
+        b = engine.upload(cache)
+        kv = engine.kv_desc(F16, kvh, dim, page, n_pages, stride)
+        engine.kv_copy_dev(kv, b, 0, engine.upload(moves.astype(np.int32)), 0, len(moves), layers=layers)
+        assert np.array_equal(b.read(np.uint16, cache.size).reshape(cache.shape), copied(cache, moves.tolist(), n_pages, per))
+
+
+def test_kv_copy_layers_between_pages(engine):
+    """page_stride leaves room for the layers: layer l's pages begin one page further."""
+    kvh, dim, page, n_pages, layers = 2, 64, 16, 12, 3
+    per = 2 * kvh * dim * page
+    cache = np.random.default_rng(0).integers(0, 1 << 16, (n_pages, layers, per), dtype=np.uint16)
+    b = engine.upload(cache)
+    kv = engine.kv_desc(BF16, kvh, dim, page, n_pages, layers * per)
+    moves = [(3, 1), (1, 2), (11, 0)]
+    engine.kv_copy_dev(kv, b, 0, engine.upload(np.array(moves, np.int32)), 0, 3, layers=layers, layer_stride=per)
+    want = np.ascontiguousarray(copied(cache.transpose(1, 0, 2), moves, n_pages, per).transpose(1, 0, 2))
+    assert np.array_equal(b.read(np.uint16, cache.size).reshape(cache.shape), want)
+
+
+def test_no_tokens_no_moves(engine):
+    b = engine.alloc(1 << 16)
+    b.fill(0x5B)
+    kv = engine.kv_desc(F16, 1, 64, 16, 2)
+    engine.kv_copy_dev(kv, b, 0, b, 0, 0)
+    engine.rope_kv_dev(engine.rope_desc(F16, 0, 1, 64), kv, b, 0, b, 0, b, 0, b, 0, b, 0, None, 0, b, 0, b, 0)
+    assert np.all(b.read(np.uint8, 1 << 16) == 0x5B)
