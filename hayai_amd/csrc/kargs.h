@@ -166,6 +166,22 @@ struct hh_kv_copy_args {
     uint32_t n, chunks;  // moves, 16-byte chunks of a page
 };
 
+// Causal attention of packed prompts (attn_prompt.hip); strides in elements.  A tile is `tile_tokens` tokens'
+// `group` heads of one kv head; `slots` bounds the tiles of a kv head.
+struct hh_attn_prompt_args {
+    hh_kv_args kv;
+    const void* q;
+    void* out;
+    const int32_t* starts;  // seqs + 1
+    const int32_t* lens;    // seqs
+    const int32_t* tables;  // seqs rows of `entries`
+    float* part;            // keys in `splits` parts: 128 rows of sums a part of a tile
+    float* part_sum;        // their bases and sums of weights
+    uint64_t q_stride, out_stride;
+    uint32_t tokens, seqs, entries, group, tile_tokens, slots, splits;
+    float c;  // scale * log2(e)
+};
+
 // Synthetic GGUF bytes: splitmix64 stream, then f16 scale fields drawn U(lo, hi).
 struct hh_synth_args {
     uint8_t* dst;

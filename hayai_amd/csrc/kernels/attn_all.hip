@@ -2,3 +2,4 @@
 // compile at the same time.
 #include "rope.hip"
 #include "kv_pages.hip"
+#include "attn_prompt.hip"

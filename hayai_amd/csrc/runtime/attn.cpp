@@ -1,5 +1,5 @@
-// Dispatch of the attention operators: rotary positions into the cache (rope.hip) and copies of its
-// pages (kv_pages.hip).
+// Dispatch of the attention operators: rotary positions into the cache (rope.hip), copies of its
+// pages (kv_pages.hip), attention of prompts (attn_prompt.hip).
 #include <algorithm>
 
 #include "engine.h"
@@ -18,6 +18,10 @@ void attn_kernels(std::vector<std::string>& k) {
     for (auto& t : kAttnTypes) {
         const std::string ty = attn_types(t[0], t[1]);
         for (const char* v : {"halves_", "pairs_"}) k.push_back(std::string("hh_rope_") + v + ty);
+        for (const char* v : {"64_", "64_any_", "128_", "128_any_", "256_", "256_any_"})
+            k.push_back(std::string("hh_attn_prompt_") + v + ty);
+        for (const char* v : {"64_", "128_", "256_"})
+            if (t[0] == t[1]) k.push_back(std::string("hh_attn_prompt_join_") + v + ty);
     }
     k.push_back("hh_kv_copy");
 }
@@ -72,5 +76,38 @@ hh_status hh_engine::enqueue_kv_copy(size_t layers, const hh_kv_copy_args& a) {
     HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)blocks, (uint32_t)layers, (uint32_t)std::max<size_t>(parts, 1), 256, 1, 1,
                                      (unsigned)lds, stream, params, nullptr),
                "hipModuleLaunchKernel(kv_copy)");
+    return HH_OK;
+}
+
+// Kernels are made for heads of 64, 128 and 256 elements, whole or with the rest as zeros.
+static size_t padded_dim(size_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+static std::string dim_name(size_t dim) {
+    return std::to_string(padded_dim(dim)) + (dim == padded_dim(dim) ? "_" : "_any_");
+}
+
+hh_status hh_engine::enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_args a) {
+    hipFunction_t f, join;
+    const size_t dp = padded_dim(a.kv.dim), cus = (size_t)props.multiProcessorCount;
+    HH_TRY(kernel("hh_attn_prompt_" + dim_name(a.kv.dim) + attn_types(type, kv_type), &f));
+    HH_TRY(kernel("hh_attn_prompt_join_" + std::to_string(dp) + "_" + act_type(type)->name, &join));
+    a.tile_tokens = 128 / a.group;
+    a.slots = a.tokens / a.tile_tokens + a.seqs;
+    const size_t tiles = (size_t)a.slots * a.kv.heads;
+    if (tiles >= 1u << 24) return fail(HH_ERR_INVALID, "attn_prompt: %u tokens of %u sequences are too many", a.tokens, a.seqs);
+    // Few tiles: their keys are split, into parts of 256 keys or more, for two workgroups a CU.
+    const size_t keys = (size_t)a.entries << a.kv.shift;
+    a.splits = (uint32_t)std::max<size_t>(1, std::min({2 * cus / tiles, keys / 256, (size_t)64}));
+    if (a.splits > 1) {
+        const size_t rows = tiles * a.splits * 128;
+        HH_TRY(grow(&ws_attn, &ws_attn_cap, rows * (dp + 2) * sizeof(float)));
+        a.part = (float*)ws_attn;
+        a.part_sum = a.part + rows * dp;
+    }
+    void* params[] = {&a};
+    HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)tiles, a.splits, 1, 256, 1, 1, 0, stream, params, nullptr),
+               "hipModuleLaunchKernel(attn_prompt)");
+    if (a.splits > 1)
+        HH_TRY_HIP(hipModuleLaunchKernel(join, (uint32_t)tiles, (uint32_t)(128 * dp / 1024), 1, 256, 1, 1, 0, stream, params, nullptr),
+                   "hipModuleLaunchKernel(attn_prompt_join)");
     return HH_OK;
 }

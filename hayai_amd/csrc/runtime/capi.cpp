@@ -1096,6 +1096,60 @@ hh_status hh_kv_copy_dev(hh_engine* e, const hh_kv_desc* kv, size_t layers, size
     }
 }
 
+// What both attention calls check: heads, scale, activations, tables and lengths.
+static hh_status check_attn(hh_engine* e, int type, float scale, size_t rows, size_t seqs, size_t q_heads, size_t entries,
+                            const hh_kv_desc* kv, const hh_buf* q, size_t q_off, size_t* q_stride, const hh_buf* out,
+                            size_t out_off, size_t* out_stride, const hh_buf* lens, size_t lens_off, const hh_buf* tables,
+                            size_t tables_off, const char* what) {
+    if (!(scale > 0) || !std::isfinite(scale)) return fail(HH_ERR_INVALID, "%s: scale=%g", what, (double)scale);
+    if (q_heads < 1 || q_heads % kv->kv_heads || q_heads / kv->kv_heads > 64)
+        return fail(HH_ERR_INVALID, "%s: q_heads=%zu is not 1 to 64 times kv_heads=%zu", what, q_heads, kv->kv_heads);
+    const size_t el = act_type(type)->bytes, cols = q_heads * kv->head_dim;
+    HH_TRY(check_sizes(rows, cols, what));
+    HH_TRY(check_rows(e, q, q_off, rows, cols, el, q_stride, what));
+    HH_TRY(check_rows(e, out, out_off, rows, cols, el, out_stride, what));
+    HH_TRY(check_sizes(seqs, 1, what));
+    if (entries > INT32_MAX) return fail(HH_ERR_INVALID, "%s: table_stride=%zu exceeds 31 bits", what, entries);
+    HH_TRY(check_vector(e, lens, lens_off, seqs, what));
+    if (entries) HH_TRY(check_vector(e, tables, tables_off, seqs * entries, what));
+    return HH_OK;
+}
+
+hh_status hh_attn_prompt_dev(hh_engine* e, const hh_attn_prompt_desc* d, const hh_kv_desc* kv, const hh_buf* q,
+                             size_t q_off, const hh_buf* cache, size_t cache_off, const hh_buf* starts, size_t starts_off,
+                             const hh_buf* lens, size_t lens_off, const hh_buf* tables, size_t tables_off, hh_buf* out,
+                             size_t out_off) {
+    HH_NOT_NULL(e, "engine");
+    HH_NOT_NULL(d, "attn_prompt desc");
+    HH_TRY(check_kv_type(d->type, kv, "attn_prompt"));
+    hh_attn_prompt_args a{};
+    size_t layer = 0, qs = d->q_stride, os = d->out_stride;
+    HH_TRY(check_kv(e, kv, cache, cache_off, 1, &layer, &a.kv, "attn_prompt cache"));
+    HH_TRY(check_attn(e, d->type, d->scale, d->tokens, d->seqs, d->q_heads, d->table_stride, kv, q, q_off, &qs, out, out_off,
+                      &os, lens, lens_off, tables, tables_off, "attn_prompt"));
+    HH_TRY(check_vector(e, starts, starts_off, d->seqs + 1, "attn_prompt starts"));
+    if (d->tokens == 0 || d->seqs == 0) return HH_OK;
+    HH_TRY(e->select());
+    a.q = at(q, q_off);
+    a.out = at(out, out_off);
+    a.starts = (const int32_t*)at(starts, starts_off);
+    a.lens = (const int32_t*)at(lens, lens_off);
+    a.tables = (const int32_t*)at(tables, tables_off);
+    a.q_stride = qs;
+    a.out_stride = os;
+    a.tokens = (uint32_t)d->tokens;
+    a.seqs = (uint32_t)d->seqs;
+    a.entries = (uint32_t)d->table_stride;
+    a.group = (uint32_t)(d->q_heads / kv->kv_heads);
+    a.c = (float)((double)d->scale * 1.4426950408889634074);
+    try {
+        std::lock_guard<std::mutex> lk(e->ws_mutex);
+        return e->enqueue_attn_prompt(d->type, kv->type, a);
+    } catch (const std::bad_alloc&) {
+        return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
+}
+
 // ---------------------------------------------------------------- MoE ----------------
 
 static hh_status validate_moe_desc(const hh_moe_desc* d) {

@@ -179,6 +179,8 @@ struct hh_engine {
     size_t ws_stk_cap = 0;      // when allocated and after a device error
     void* ws_smp = nullptr;     // token choice: sums, lists (sample.hip)
     size_t ws_smp_cap = 0;
+    void* ws_attn = nullptr;    // attention whose keys are split: sums of the parts
+    size_t ws_attn_cap = 0;
     void* grid_sync = nullptr;  // grid-barrier state (counters, flags, error word, epochs)
     hh_ffn_desc ffn_stage{};    // FFN whose gate/up output is pending in ws_h (/ws_hq)
     bool ffn_stage_valid = false;
@@ -354,6 +356,7 @@ struct hh_engine {
     // Attention over pages (attn.cpp).
     hh_status enqueue_rope(int type, int kv_type, int layout, size_t tokens, const hh_rope_args& a);
     hh_status enqueue_kv_copy(size_t layers, const hh_kv_copy_args& a);
+    hh_status enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_args a);
     // Reports (and clears) a grid-barrier timeout recorded by a fused kernel.  Syncs.
     hh_status check_device_error();
 };

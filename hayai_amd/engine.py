@@ -771,6 +771,20 @@ class HipEngine:
         _check(self.lib.hh_kv_copy_dev(self.handle, C.byref(kv), layers, layer_stride, cache.handle, cache_off,
                                        moves.handle, moves_off, n))
 
+    @staticmethod
+    def attn_prompt_desc(ggml_type: int, tokens: int, seqs: int, q_heads: int, scale: float, table_stride: int,
+                         q_stride: int = 0, out_stride: int = 0) -> _abi.AttnPromptDesc:
+        return _abi.AttnPromptDesc(ggml_type, scale, tokens, seqs, q_heads, table_stride, q_stride, out_stride)
+
+    def attn_prompt_dev(self, desc: _abi.AttnPromptDesc, kv: _abi.KvDesc, q: DeviceBuffer, q_off: int, cache: DeviceBuffer,
+                        cache_off: int, starts: DeviceBuffer, starts_off: int, lens: DeviceBuffer, lens_off: int,
+                        tables: DeviceBuffer, tables_off: int, out: DeviceBuffer, out_off: int) -> None:
+        """Causal attention of packed sequences' new tokens (rows starts[s].. of q) over the lens[s] cached tokens
+        in the pages of tables[s].  Enqueue only."""
+        _check(self.lib.hh_attn_prompt_dev(self.handle, C.byref(desc), C.byref(kv), q.handle, q_off, cache.handle,
+                                           cache_off, starts.handle, starts_off, lens.handle, lens_off, tables.handle,
+                                           tables_off, out.handle, out_off))
+
     # ---------------------------------------------------------------- synthetic data
     def synth_weights_dev(self, ggml_type: int, dst: DeviceBuffer, off: int, n_blocks: int, seed: int,
                           lo: float, hi: float) -> None:

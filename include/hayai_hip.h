@@ -576,6 +576,30 @@ hh_status hh_rope_factors(int scaling, size_t rot_dim, double base, double scale
 hh_status hh_kv_copy_dev(hh_engine* e, const hh_kv_desc* kv, size_t layers, size_t layer_stride, hh_buf* cache,
                          size_t cache_off, const hh_buf* moves, size_t moves_off, size_t n);
 
+/* Causal attention of new tokens over their sequences' pages, after hh_rope_kv_dev has put their keys and
+ * values there.  Sequence s has rows starts[s] .. starts[s + 1] - 1 of q and out (starts: int32[seqs + 1],
+ * ascending, at most `tokens`) as the last of its lens[s] cached tokens, and its pages in row s of
+ * tables (int32[seqs][table_stride]).  The i-th of its n rows sees the first lens[s] - n + i + 1 tokens: a whole
+ * prompt has lens[s] = n, the next part of a longer one has more.  For each query head h (kv head h / (q_heads /
+ * kv_heads)):  out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j).
+ * A row that sees no token gets zeros.  Rows of no sequence stay as they were.  Lengths are taken to what the
+ * table has room for; an entry that is read and outside [0, n_pages) stands for a page of zeros.  What lies
+ * past a sequence's length, or past what a row sees, has no influence, NaN and infinities included.
+ * Scores, weights' sums and outputs are summed in f32; over a 16-bit cache the products' operands are of the
+ * cache's type: weights are rounded to it, and f32 queries too. */
+typedef struct hh_attn_prompt_desc {
+    int type;            /* of q and out */
+    float scale;         /* > 0, finite: 1 / sqrt(head_dim) as a rule */
+    size_t tokens, seqs;
+    size_t q_heads;      /* 1..64 times kv_heads */
+    size_t table_stride; /* pages a sequence can have */
+    size_t q_stride, out_stride; /* elements */
+} hh_attn_prompt_desc;
+hh_status hh_attn_prompt_dev(hh_engine* e, const hh_attn_prompt_desc* d, const hh_kv_desc* kv, const hh_buf* q,
+                             size_t q_off, const hh_buf* cache, size_t cache_off, const hh_buf* starts, size_t starts_off,
+                             const hh_buf* lens, size_t lens_off, const hh_buf* tables, size_t tables_off, hh_buf* out,
+                             size_t out_off);
+
 /* ------------------------------------------------------------------ streaming ------- */
 
 /* Pinned-host ping-pong weight streaming: StreamingScratch

@@ -204,3 +204,34 @@ def test_no_tokens_no_moves(engine):
     engine.kv_copy_dev(kv, b, 0, b, 0, 0)
     engine.rope_kv_dev(engine.rope_desc(F16, 0, 1, 64), kv, b, 0, b, 0, b, 0, b, 0, b, 0, None, 0, b, 0, b, 0)
     assert np.all(b.read(np.uint8, 1 << 16) == 0x5B)
+
+
+def test_refusals(engine):
+    b, small = engine.alloc(1 << 16), engine.alloc(8)
+    kv = engine.kv_desc(F16, 2, 64, 16, 2)
+    good = dict(ggml_type=F16, tokens=4, q_heads=4, rot_dim=64)
+
+    def rope(kv=kv, q=b, k=b, slots=b, factors=None, out=b, cache=b, cache_off=0, **changes):
+        engine.rope_kv_dev(engine.rope_desc(**{**good, **changes}), kv, q, 0, k, 0, b, 0, b, 0, slots, 0, factors, 0, out, 0, cache,
+                           cache_off)
+
+    rope()
+    for status, changes in [(3, dict(ggml_type=2)), (3, dict(ggml_type=BF16)), (3, dict(kv=engine.kv_desc(F32, 2, 64, 16, 1))),
+                            (2, dict(layout=2)), (2, dict(rot_dim=66)), (2, dict(rot_dim=3)), (2, dict(base=0.0)),
+                            (2, dict(base=float("inf"))), (2, dict(base=float("nan"))), (2, dict(mscale=float("inf"))),
+                            (2, dict(q_heads=65536)), (2, dict(tokens=1 << 40)), (2, dict(tokens=1 << 14)), (2, dict(q_stride=255)),
+                            (2, dict(k_stride=127)), (2, dict(v_stride=127)), (2, dict(out_stride=255)), (2, dict(q=None)),
+                            (2, dict(out=None)), (2, dict(k=small)), (2, dict(slots=small)), (2, dict(factors=small)),
+                            (2, dict(cache=small)), (2, dict(cache_off=2)), (2, dict(cache_off=1 << 16)),
+                            (2, dict(kv=engine.kv_desc(F16, 1025, 64, 16, 2)))]:
+        with pytest.raises(hayai_amd.HipError) as err:
+            rope(**changes)
+        assert err.value.status == status, changes
+    engine.kv_copy_dev(kv, b, 0, small, 0, 1)
+    for args, kw in [((kv, b, 0, small, 0, 2), {}), ((kv, b, 0, small, 0, 1), dict(layers=0)), ((kv, b, 0, small, 0, 1), dict(layers=1 << 16)),
+                     ((kv, b, 0, small, 0, 1), dict(layers=9)), ((kv, b, 0, small, 0, 1), dict(layers=2, layer_stride=4)),
+                     ((kv, b, 0, small, 0, 1), dict(layers=3, layer_stride=1 << 62)), ((kv, b, 0, small, 0, 1 << 40), {}),
+                     ((kv, b, 0, small, 2, 1), {}), ((kv, small, 0, b, 0, 1), {})]:
+        with pytest.raises(hayai_amd.HipError) as err:
+            engine.kv_copy_dev(*args, **kw)
+        assert err.value.status == 2, (args[2:], kw)

@@ -1,0 +1,235 @@
+"""GPU tests of causal attention over pages (attn_prompt) against its definition in 64 bits; the bounds'
+derivation stands in attn_reference.py."""
+import numpy as np
+import pytest
+import torch
+
+from attn_reference import DT, attend, check, gather, page_elements
+from hayai_amd import BF16, F16, F32, HipError
+from test_gpu_attn_pages import get, ints, normal, put
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [(F32, F32), (F16, F16), (BF16, BF16), (F32, F16), (F32, BF16)]
+
+
+class Problem:
+    """Packed sequences of (new, cached) tokens, their pages at random places."""
+
+    def __init__(self, ty, cty, seqs, heads, kvh, dim, page, seed=0, spare=2, pad=0, scale=None, width=None):
+        self.ty, self.cty, self.seqs, self.heads, self.kvh, self.dim, self.page, self.pad = ty, cty, seqs, heads, kvh, dim, page, pad
+        rng = np.random.default_rng(seed)
+        per = page_elements(kvh, dim, page)
+        need = [-(-max(length, 0) // page) for _, length in seqs]
+        self.n_pages = sum(need) + spare
+        ids = rng.permutation(self.n_pages)
+        self.width = max(need + [1]) if width is None else width
+        self.tables = np.full((len(seqs), self.width), -7, np.int32)
+        at = 0
+        for s, n in enumerate(need):
+            self.tables[s, :n] = ids[at:at + n]
+            at += n
+        self.cache = normal(seed + 1, self.n_pages, per).to(DT[cty])
+        self.starts = np.cumsum([0] + [n for n, _ in seqs]).astype(np.int32)
+        self.lens = np.array([length for _, length in seqs], np.int32)
+        self.tokens = int(self.starts[-1])
+        self.q = normal(seed + 2, self.tokens, heads * dim + pad).to(DT[ty])
+        self.scale = float(np.float32(dim**-0.5 if scale is None else scale))
+
+    def run(self, engine, tokens=None):
+        tokens = self.tokens if tokens is None else tokens
+        wide = self.heads * self.dim + self.pad
+        self.out = put(engine, torch.full((max(tokens, self.tokens), wide), 5.0).to(DT[self.ty]))
+        q = torch.zeros(max(tokens, len(self.q)), wide).to(DT[self.ty])
+        q[:len(self.q)] = self.q
+        d = engine.attn_prompt_desc(self.ty, tokens, len(self.seqs), self.heads, self.scale, self.width, wide, wide)
+        kv = engine.kv_desc(self.cty, self.kvh, self.dim, self.page, self.n_pages)
+        engine.attn_prompt_dev(d, kv, put(engine, q), 0, put(engine, self.cache), 0, ints(engine, self.starts.tolist()), 0,
+                               ints(engine, self.lens.tolist()), 0, ints(engine, self.tables.reshape(-1).tolist()), 0, self.out, 0)
+        return get(self.out, DT[self.ty], (max(tokens, self.tokens), wide))
+
+    def want(self, cache=None):
+        cache = self.cache if cache is None else cache
+        q = self.q[:, :self.heads * self.dim].double().numpy().reshape(-1, self.heads, self.dim)
+        out, bound = np.zeros_like(q), np.zeros_like(q)
+        for s, (n, length) in enumerate(self.seqs):
+            length = min(max(length, 0), self.width * self.page)
+            rows = slice(self.starts[s], self.starts[s] + n)
+            k, v = gather(cache, self.tables[s], length, self.kvh, self.dim, self.page)
+            out[rows], bound[rows] = attend(q[rows], k, v, length - n + 1 + np.arange(n), self.scale, self.ty, self.cty)
+        return out, bound
+
+    def check(self, engine, cache=None):
+        got = self.run(engine)
+        want, bound = self.want(cache)
+        check(got[:self.tokens, :self.heads * self.dim].reshape(want.shape), want, bound, self.ty)
+        assert torch.all(got[:, self.heads * self.dim:] == 5.0)
+        return got
+
+
+# sequences (new, cached), heads, kv heads, dim, page: one token, tiles' edges, ragged packs, empty sequences, rows
+# that see nothing (more new than cached tokens), parts of longer prompts, long ones whose keys are split, groups
+# of 1, 3, 7, 64 heads
+CASES = [([(1, 1)], 1, 1, 64, 16), ([(30, 30)], 9, 3, 64, 16), ([(33, 33), (1, 1), (0, 0), (70, 70)], 8, 2, 128, 32),
+         ([(5, 3), (4, 0), (2, 40)], 4, 4, 64, 64), ([(64, 64)], 2, 2, 128, 64), ([(65, 129), (3, 700)], 7, 1, 128, 128),
+         ([(17, 17)], 4, 1, 72, 16), ([(40, 101)], 3, 1, 256, 32), ([(3, 2500)], 8, 2, 128, 16), ([(1, 1300), (2, 15)], 64, 1, 64, 256),
+         ([(9, 650)], 2, 1, 8, 16), ([(21, 21), (22, 150)], 6, 2, 200, 64), ([(130, 130), (0, 64), (140, 141)], 5, 5, 96, 32)]
+
+
+@pytest.mark.parametrize("ty,cty", TYPES)
+def test_prompt(engine, ty, cty):
+    for i, (seqs, heads, kvh, dim, page) in enumerate(CASES):
+        print(f"[case] prompt {ty} {cty} {CASES[i]}", flush=True)
+        Problem(ty, cty, seqs, heads, kvh, dim, page, seed=i, pad=i % 3).check(engine)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+def test_rows_of_no_sequence_stay(engine, ty):
+    p = Problem(ty, ty, [(20, 20), (7, 31)], 4, 2, 64, 32)
+    got = p.run(engine, tokens=60)
+    want, bound = p.want()
+    check(got[:27].reshape(want.shape), want, bound, ty)
+    assert torch.all(got[27:] == 5.0)
+    # a first sequence that begins later
+    p.starts = p.starts + 5
+    p.q = torch.cat([torch.zeros_like(p.q[:5]), p.q])
+    got = p.run(engine, tokens=60)
+    check(got[5:32].reshape(want.shape), want, bound, ty)
+    assert torch.all(got[:5] == 5.0) and torch.all(got[32:] == 5.0)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_a_row_does_not_see(engine, ty, bad):
+    """Later tokens' keys and values, slots past the length and pages of no sequence hold no finite numbers."""
+    for seqs, page in [([(50, 50)], 16), ([(70, 400)], 64), ([(3, 1201)], 32)]:
+        p = Problem(ty, ty, seqs, 4, 2, 128, page, seed=3)
+        n, length = seqs[0]
+        want, bound = p.want()
+        per, kvh, dim = page_elements(2, 128, page), 2, 128
+        keys, values = p.cache[:, :per // 2].view(-1, kvh, page, dim), p.cache[:, per // 2:].view(-1, kvh, dim, page)
+        used = set(p.tables[0].tolist())
+        for other in range(p.n_pages):
+            if other not in used:
+                p.cache[other] = bad
+        for t in range(length - n // 2, -(-length // page) * page):  # later half of the new tokens, and past them
+            keys[p.tables[0, t // page], :, t % page] = bad
+            values[p.tables[0, t // page], :, :, t % page] = bad
+        got = p.run(engine).double().numpy().reshape(want.shape)
+        free = n - n // 2
+        check(torch.from_numpy(got[:free]), want[:free], bound[:free], ty)
+        assert not np.any(np.isfinite(got[free:]))
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+def test_infinite_value_is_seen(engine, ty):
+    """An infinite value decides that element of every row that sees it, and of no other."""
+    p = Problem(ty, ty, [(40, 90)], 2, 1, 64, 16, seed=5)
+    values = p.cache[:, 16 * 64:].view(-1, 1, 64, 16)
+    values[p.tables[0, 70 // 16], 0, 9, 70 % 16] = float("inf")
+    values[p.tables[0, 75 // 16], 0, 9, 75 % 16] = -float("inf")
+    got = p.run(engine).double().numpy().reshape(40, 2, 64)
+    assert np.all(np.isfinite(got[:20])) and np.all(np.isfinite(np.delete(got, 9, axis=2)))
+    assert np.all(got[20:25, :, 9] == np.inf) and np.all(np.isnan(got[25:, :, 9]))
+
+
+def test_entries_outside_the_cache_are_zeros(engine):
+    p = Problem(BF16, BF16, [(90, 90), (5, 200)], 4, 2, 128, 32, seed=8)
+    p.tables[0, 1], p.tables[1, 0], p.tables[1, 3] = -1, p.n_pages, 2**31 - 1
+    p.check(engine)
+
+
+def test_lengths_past_the_table(engine):
+    p = Problem(F16, F16, [(6, 64)], 4, 2, 64, 16, seed=9)
+    p.lens[0] = 2**31 - 1  # as 64
+    p.check(engine)
+    p.lens[0], p.seqs = -5, [(6, -5)]
+    got = p.run(engine)
+    assert torch.all(got == 0)
+    p.width, p.tables = 0, np.zeros((1, 0), np.int32)
+    p.lens[0] = 64
+    kv, wide = engine.kv_desc(F16, 2, 64, 16, p.n_pages), 256
+    out = put(engine, torch.full((6, wide), 5.0).half())
+    engine.attn_prompt_dev(engine.attn_prompt_desc(F16, 6, 1, 4, 0.125, 0), kv, put(engine, p.q), 0, put(engine, p.cache), 0,
+                           ints(engine, [0, 6]), 0, ints(engine, [64]), 0, out, 0, out, 0)
+    assert torch.all(get(out, torch.float16, (6, wide)) == 0)
+
+
+def test_starts_that_do_not_ascend(engine):
+    """Bad lists: no access outside, rows of no sequence stay, the good sequence is right where no other writes."""
+    p = Problem(F16, F16, [(20, 20), (20, 20)], 4, 2, 64, 16, seed=10)
+    want, bound = p.want()
+    p.starts = np.array([0, 20, -3], np.int32)  # the second one ends before it begins
+    got = p.run(engine, tokens=50)
+    check(got[:20].reshape(20, 4, 64), want[:20], bound[:20], F16)
+    assert torch.all(got[20:] == 5.0)
+    p.starts = np.array([0, 20, 2**31 - 1], np.int32)  # it ends with the rows
+    got = p.run(engine, tokens=50)
+    check(got[:20].reshape(20, 4, 64), want[:20], bound[:20], F16)
+
+
+def test_many_sequences(engine):
+    """More than the search takes at once, many of them empty."""
+    rng = np.random.default_rng(4)
+    seqs = [(int(n), int(n) + int(m)) for n, m in zip(rng.integers(0, 3, 300), rng.integers(0, 20, 300))]
+    Problem(F32, F32, seqs, 2, 1, 64, 16, seed=6).check(engine)
+
+
+def test_large_scores(engine):
+    """Scores far apart, growing along the keys: the running base has to follow."""
+    for ty in (F32, F16, BF16):
+        p = Problem(ty, ty, [(3, 900)], 2, 1, 64, 16, seed=11, scale=1.0)
+        keys = p.cache[:, :16 * 64].view(-1, 16, 64)
+        for t in range(900):
+            keys[p.tables[0, t // 16], t % 16] *= 0.2 + t / 150
+        p.check(engine)
+
+
+def test_far_pages(engine):
+    """Pages three gigabytes apart: offsets past 32 bits."""
+    kvh, dim, page, n_pages = 2, 128, 64, 4
+    per, stride = page_elements(kvh, dim, page), 3 << 29
+    p = Problem(BF16, BF16, [(40, 200)], 8, kvh, dim, page, seed=12, spare=0)
+    b = engine.alloc(((n_pages - 1) * stride + per) * 2)
+    for i in range(n_pages):
+        b.write(p.cache[i].view(torch.uint8).numpy(), i * stride * 2)
+    kv = engine.kv_desc(BF16, kvh, dim, page, n_pages, stride)
+    out = engine.alloc(40 * 1024 * 2)
+    engine.attn_prompt_dev(engine.attn_prompt_desc(BF16, 40, 1, 8, p.scale, p.width), kv, put(engine, p.q), 0, b, 0,
+                           ints(engine, [0, 40]), 0, ints(engine, [200]), 0, ints(engine, p.tables[0].tolist()), 0, out, 0)
+    want, bound = p.want()
+    check(get(out, torch.bfloat16, want.shape), want, bound, BF16)
+    b.free()
+
+
+def test_same_bits_every_time(engine):
+    p = Problem(BF16, BF16, [(5, 3000), (60, 60)], 8, 2, 128, 64, seed=13)
+    first = p.run(engine)
+    for _ in range(3):
+        assert torch.equal(first, p.run(engine))
+
+
+def test_refusals(engine):
+    b = engine.alloc(1 << 16)
+    kv = engine.kv_desc(F16, 2, 64, 16, 2)
+    good = dict(ggml_type=F16, tokens=4, seqs=1, q_heads=4, scale=0.125, table_stride=2)
+
+    def call(kv=kv, starts=b, **changes):
+        engine.attn_prompt_dev(engine.attn_prompt_desc(**{**good, **changes}), kv, b, 0, b, 0, starts, 0, b, 0, b, 0, b, 0)
+
+    small = engine.alloc(4)
+    for status, changes in [(3, dict(ggml_type=2)), (3, dict(ggml_type=BF16)), (2, dict(scale=0.0)), (2, dict(scale=float("nan"))),
+                            (2, dict(scale=float("inf"))), (2, dict(q_heads=3)), (2, dict(q_heads=0)), (2, dict(q_heads=130)),
+                            (2, dict(tokens=1 << 12)), (2, dict(q_stride=255)), (2, dict(out_stride=255)), (2, dict(seqs=1 << 20)),
+                            (2, dict(table_stride=1 << 33)), (2, dict(tokens=1 << 40)), (2, dict(starts=small)),
+                            (3, dict(kv=engine.kv_desc(8, 2, 64, 16, 2))), (2, dict(kv=engine.kv_desc(F16, 0, 64, 16, 2))),
+                            (2, dict(kv=engine.kv_desc(F16, 2, 63, 16, 2))), (2, dict(kv=engine.kv_desc(F16, 2, 264, 16, 2))),
+                            (2, dict(kv=engine.kv_desc(F16, 2, 64, 24, 2))), (2, dict(kv=engine.kv_desc(F16, 2, 64, 8, 2))),
+                            (2, dict(kv=engine.kv_desc(F16, 2, 64, 512, 2))), (2, dict(kv=engine.kv_desc(F16, 2, 64, 16, 0))),
+                            (2, dict(kv=engine.kv_desc(F16, 2, 64, 16, 1 << 28))), (2, dict(kv=engine.kv_desc(F16, 2, 64, 16, 9))),
+                            (2, dict(kv=engine.kv_desc(F16, 2, 64, 16, 2, 4095))), (2, dict(kv=engine.kv_desc(F16, 2, 64, 16, 2, 4100)))]:
+        with pytest.raises(HipError) as err:
+            call(**changes)
+        assert err.value.status == status, changes
+    with pytest.raises(HipError):
+        engine.attn_prompt_dev(engine.attn_prompt_desc(**good), kv, b, 0, b, 8, b, 0, b, 0, b, 0, b, 0)
