@@ -223,6 +223,19 @@ class AttnPromptDesc(C.Structure):
     ]
 
 
+class AttnDecodeDesc(C.Structure):
+    _fields_ = [
+        ("type", C.c_int),
+        ("scale", C.c_float),
+        ("seqs", C.c_size_t),
+        ("q_heads", C.c_size_t),
+        ("prefix", C.c_size_t),
+        ("table_stride", C.c_size_t),
+        ("q_stride", C.c_size_t),
+        ("out_stride", C.c_size_t),
+    ]
+
+
 SIGNATURES = {
     "hh_gguf_open": (ST, [C.c_char_p, PP]),
     "hh_gguf_close": (None, [P]),
@@ -295,6 +308,7 @@ SIGNATURES = {
     "hh_rope_factors": (ST, [I, SZ, C.c_double, C.c_double, C.c_double, P, P]),
     "hh_kv_copy_dev": (ST, [P, C.POINTER(KvDesc), SZ, SZ, P, SZ, P, SZ, SZ]),
     "hh_attn_prompt_dev": (ST, [P, C.POINTER(AttnPromptDesc), C.POINTER(KvDesc)] + [P, SZ] * 6),
+    "hh_attn_decode_dev": (ST, [P, C.POINTER(AttnDecodeDesc), C.POINTER(KvDesc)] + [P, SZ] * 6),
     "hh_streamer_create": (ST, [P, SZ, SZ, SZ, PP]),
     "hh_streamer_destroy": (None, [P]),
     "hh_streamer_slot_for": (ST, [P, SZ, C.POINTER(SZ)]),

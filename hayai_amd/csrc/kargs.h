@@ -166,20 +166,37 @@ struct hh_kv_copy_args {
     uint32_t n, chunks;  // moves, 16-byte chunks of a page
 };
 
-// Causal attention of packed prompts (attn_prompt.hip); strides in elements.  A tile is `tile_tokens` tokens'
-// `group` heads of one kv head; `slots` bounds the tiles of a kv head.
-struct hh_attn_prompt_args {
+// What attention of a prompt and of a decode batch have in common (attn_rows.h); strides in elements.  A tile is
+// `tile_tokens` tokens' `group` heads of one kv head.
+struct hh_attn_args {
     hh_kv_args kv;
     const void* q;
     void* out;
-    const int32_t* starts;  // seqs + 1
-    const int32_t* lens;    // seqs
-    const int32_t* tables;  // seqs rows of `entries`
-    float* part;            // keys in `splits` parts: 128 rows of sums a part of a tile
+    const int32_t* lens;    // of each sequence
+    const int32_t* tables;  // rows of `entries`
+    float* part;            // tiles whose keys are in `splits` parts: 128 rows of sums a part
     float* part_sum;        // their bases and sums of weights
     uint64_t q_stride, out_stride;
-    uint32_t tokens, seqs, entries, group, tile_tokens, slots, splits;
+    uint32_t seqs, entries, group, tile_tokens, splits;
     float c;  // scale * log2(e)
+};
+
+// Causal attention of packed prompts (attn_prompt.hip).  `slots` bounds the tiles of a kv head.
+struct hh_attn_prompt_args {
+    hh_attn_args a;
+    const int32_t* starts;  // seqs + 1
+    uint32_t tokens, slots;
+};
+
+// Attention of one token a sequence (attn_decode.hip): the first `prefix` tokens of all sequences from the
+// pages of `shared` (tiles of `a`), the others in pieces, each with row_tiles * heads * 16 rows of sums.
+struct hh_attn_decode_args {
+    hh_attn_args a;
+    const int32_t* shared;
+    float* piece;
+    float* piece_sum;
+    uint32_t* plan;  // each sequence's first piece and how many it has
+    uint32_t prefix, shared_entries, tiles, row_tiles, pieces, least;
 };
 
 // Synthetic GGUF bytes: splitmix64 stream, then f16 scale fields drawn U(lo, hi).

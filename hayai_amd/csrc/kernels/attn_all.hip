@@ -3,3 +3,4 @@
 #include "rope.hip"
 #include "kv_pages.hip"
 #include "attn_prompt.hip"
+#include "attn_decode.hip"

@@ -1,0 +1,339 @@
+// Attention of one token a sequence over its pages, for a batch whose sequences begin with the same `prefix`
+// tokens: out[s][h] = sum_j p_j v_j / sum_j p_j over all tokens j of sequence s.
+//
+// The shared tokens are taken once for all: tiles of 128 rows (32 sequences' 4 heads) against the prefix's
+// pages, as a prompt's are (attn_rows.h), their keys in parts.  A sequence's own tokens are read by workgroups
+// of one kv head's up to 16 heads, memory bound: keys and values go from the pages straight into operands of
+// the 16-column matrix products (attn_tiles.h), 16 KB in flight a wave, each of the four waves every fourth
+// step of 32 keys (16 of f32), joined through LDS at the end.  Lengths are known on the device alone, so every workgroup sums them up
+// and finds the piece of work that falls to it: as many pieces as the chip has room for, of equal length
+// whatever the sequences' are.  A second kernel joins the parts of a row.
+//
+// Weights are rounded to the cache's type for the second product; sums and the parts are f32.
+#include "attn_rows.h"
+
+#define HH_ATTN_UNIT 128  // keys a piece is a multiple of
+
+// Tokens of sequence s that no other shares, and the first of them.  A sequence shorter than the prefix takes no
+// part in it.
+HH_DEV uint32_t hh_attn_own(const hh_attn_decode_args& p, uint32_t s, uint32_t& from) {
+    const uint32_t len = (uint32_t)min((int64_t)max(0, p.a.lens[s]), (int64_t)p.a.entries << p.a.kv.shift);
+    from = len >= p.prefix ? p.prefix : 0;
+    return len - from;
+}
+
+struct hh_attn_piece {
+    uint32_t seq, at, count, units;  // the at-th of the sequence's `count` pieces of `units` units
+};
+// Piece number `piece`; the first workgroup leaves the plan for the join.
+HH_DEV bool hh_attn_plan(const hh_attn_decode_args& p, uint32_t piece, bool first, hh_attn_piece& mine) {
+    __shared__ uint32_t red[8];
+    __shared__ hh_attn_piece found;
+    const uint32_t tid = threadIdx.x, lane = tid % HH_WAVE, wave = tid / HH_WAVE;
+    auto units = [&](uint32_t s) {
+        uint32_t from;
+        return s < p.a.seqs ? (hh_attn_own(p, s, from) + HH_ATTN_UNIT - 1) / HH_ATTN_UNIT : 0;
+    };
+    uint64_t all = 0;
+    for (uint32_t s = tid; s < p.a.seqs; s += 256) all += units(s);
+    all = hh_wave64<hh_addu64>(all);
+    __shared__ uint64_t sums[4];
+    if (lane == 0) sums[wave] = all;
+    if (tid == 0) found.count = 0;
+    __syncthreads();
+    all = sums[0] + sums[1] + sums[2] + sums[3];
+    const uint32_t each = (uint32_t)max((uint64_t)p.least, (all + p.pieces - 1) / p.pieces);
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < p.a.seqs; s0 += 256) {
+        const uint32_t s = s0 + tid, n = s < p.a.seqs ? max(1u, (units(s) + each - 1) / each) : 0;
+        const uint32_t scan = (uint32_t)hh_scan64(n);
+        if (lane == HH_WAVE - 1) red[wave + (s0 / 256 & 1) * 4] = scan;
+        __syncthreads();
+        uint32_t base = before;
+        for (uint32_t w = 0; w < 4; w++) {
+            if (w < wave) base += red[w + (s0 / 256 & 1) * 4];
+            before += red[w + (s0 / 256 & 1) * 4];
+        }
+        const uint32_t at = base + scan - n;
+        if (piece - at < n) found = hh_attn_piece{s, piece - at, n, each};
+        if (first && s < p.a.seqs) {
+            p.plan[2 * s] = at;
+            p.plan[2 * s + 1] = n;
+        }
+    }
+    __syncthreads();
+    mine = found;
+    return mine.count != 0;
+}
+
+template <class A, class C, int DP, bool FULL>
+HH_DEV void hh_attn_single(const hh_attn_decode_args& p, uint32_t block) {
+    typedef typename A::E E;
+    typedef typename C::E CE;
+    typedef hh_mat<C> M;
+    typedef typename M::frag F;
+    constexpr int EF = C::VEC, SZ = sizeof(CE), STEP = 4 * EF, KT = STEP / 16, NC = DP / (4 * EF), DT = DP / 16;
+    const hh_attn_args& a = p.a;
+    const uint32_t lane = threadIdx.x % HH_WAVE, ln = lane % 16, g = lane / 16;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / HH_WAVE);
+    const uint32_t kvh = block % a.kv.heads, rt = block / a.kv.heads % p.row_tiles, number = block / a.kv.heads / p.row_tiles;
+    const uint32_t dim = FULL ? DP : a.kv.dim, shift = a.kv.shift, mask = (1u << shift) - 1;
+    hh_attn_piece piece;
+    if (!hh_attn_plan(p, number, block == 0, piece)) return;
+    uint32_t from;
+    const uint32_t own = hh_attn_own(p, piece.seq, from);
+    const uint32_t k0 = min(own, piece.at * piece.units * HH_ATTN_UNIT) + from;
+    const uint32_t k1 = min((uint64_t)own, (uint64_t)(piece.at + 1) * piece.units * HH_ATTN_UNIT) + from;
+    const bool alone = piece.count == 1 && (p.prefix == 0 || from == 0);
+    const int32_t* const table = a.tables + (size_t)piece.seq * a.entries;
+
+    const uint32_t head = kvh * a.group + min(rt * 16 + ln, a.group - 1);
+    F q[NC];
+    const E* qrow = (const E*)a.q + (size_t)piece.seq * a.q_stride + head * dim;
+#pragma unroll
+    for (int c = 0; c < NC; c++) q[c] = hh_query<A, C, FULL>(qrow, (4 * c + g) * EF, dim, true);
+
+    // row ln of K's t-th tile is key 8 (ln / 4) + 4 t + ln % 4 of 16-bit types, so that a lane's scores are of keys EF g ..
+    const uint32_t krow = SZ == 4 ? ln : 8 * (ln / 4) + ln % 4;
+    uint32_t id_k = 0, id_v = 0;
+    auto ask = [&](uint32_t k) {
+        id_k = hh_page(table, k + krow, shift, a.entries);
+        id_v = hh_page(table, k + EF * g, shift, a.entries);
+    };
+    F kf[KT][NC], vf[DT];
+    auto load_k = [&](uint32_t k, uint32_t id) {
+        const uint8_t* page = a.kv.base + (id < a.kv.pages ? id : 0) * a.kv.stride + g * 16;
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+            const uint8_t* row = page + hh_kv_key<C>(a.kv, kvh, (k + krow + 4 * t) & mask);
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const bool in = FULL || (4 * c + g) * EF < dim;
+                kf[t][c] = *(const F*)(in ? row + c * 64 : row - g * 16);
+            }
+        }
+    };
+    auto load_v = [&](uint32_t k, uint32_t id) {
+        const uint8_t* page = a.kv.base + (id < a.kv.pages ? id : 0) * a.kv.stride + ((k + EF * g) & mask) * SZ;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+            vf[i] = *(const F*)(page + hh_kv_value<C>(a.kv, kvh, FULL ? i * 16 + ln : min(i * 16 + ln, dim - 1)));
+    };
+
+    hh_f32x4 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++) o[i] = hh_f32x4{0, 0, 0, 0};
+    float base = HH_ATTN_LOWEST, sum = 0;
+    uint32_t k = k0 + wave * STEP;
+    bool zero_k = false, zero_v = false;
+    if (k < k1) {
+        ask(k);
+        load_k(k, id_k);
+        zero_k = id_k >= a.kv.pages;
+    }
+    for (; k < k1; k += 4 * STEP) {
+        load_v(k, id_v);
+        zero_v = id_v >= a.kv.pages;
+        const bool more = k + 4 * STEP < k1;
+        if (more) ask(k + 4 * STEP);
+        if (!FULL || __any(zero_k)) {
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+                    if (zero_k || (!FULL && (4 * c + g) * EF >= dim)) kf[t][c] = F{};
+        }
+        float s[EF];
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+            hh_f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < NC; c++) acc = M::mul16(kf[t][c], q[c], acc);
+#pragma unroll
+            for (int x = 0; x < 4; x++) s[4 * t + x] = acc[x];
+        }
+        if (more) {
+            load_k(k + 4 * STEP, id_k);
+            zero_k = id_k >= a.kv.pages;
+        }
+        const bool last = k + STEP > k1;
+        if (last) {
+#pragma unroll
+            for (int x = 0; x < EF; x++) s[x] = k + EF * g + x < k1 ? s[x] : -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int x = 1; x < EF; x++) top = fmaxf(top, s[x]);
+        top *= a.c;
+        if (__any(top > base + HH_ATTN_SLACK)) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float next = top > base + HH_ATTN_SLACK ? top : base, f = hh_exp2(base - next);
+            base = next;
+            sum *= f;
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[i][x] *= f;
+        }
+        F w;
+#pragma unroll
+        for (int x = 0; x < EF; x++) {
+            s[x] = hh_exp2(fmaf(s[x], a.c, -base));
+            w[x] = C::put(s[x]);
+        }
+#pragma unroll
+        for (int n = EF / 2; n > 0; n /= 2)
+#pragma unroll
+            for (int x = 0; x < n; x++) s[x] += s[x + n];
+        sum += s[0];
+        if (last || __any(zero_v)) {
+#pragma unroll
+            for (int i = 0; i < DT; i++) vf[i] = hh_first<C>(vf[i], zero_v ? 0 : (int)(k1 - k) - (int)(EF * g));
+        }
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[i] = M::mul16(vf[i], w, o[i]);
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+
+    // the waves' sums, joined: 4-element chunk c of row r lies at chunk c ^ r
+    __shared__ float bases[4][16], weights[4][16];
+    float* const red = (float*)hh_attn_lds<0, 256 * DP>();
+    if (lane < 16) {
+        bases[wave][lane] = base;
+        weights[wave][lane] = sum;
+    }
+    __syncthreads();
+    const float top = fmaxf(fmaxf(bases[0][ln], bases[1][ln]), fmaxf(bases[2][ln], bases[3][ln])), f = hh_exp2(base - top);
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+        *(hh_f32x4*)(red + ((wave * 16 + ln) * (DP / 4) + ((i * 4 + g) ^ ln)) * 4) = o[i] * f;
+    __syncthreads();
+    const size_t rows = ((size_t)number * p.row_tiles + rt) * a.kv.heads + kvh;
+#pragma unroll
+    for (uint32_t at = threadIdx.x; at < 4 * DP; at += 256) {
+        const uint32_t r = at / (DP / 4), d = at % (DP / 4) * 4;
+        if (rt * 16 + r >= a.group || d >= dim) continue;
+        const float t = fmaxf(fmaxf(bases[0][r], bases[1][r]), fmaxf(bases[2][r], bases[3][r]));
+        float total = 0;
+        hh_f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            total = fmaf(weights[w][r], hh_exp2(bases[w][r] - t), total);
+            v += *(const hh_f32x4*)(red + ((w * 16 + r) * (DP / 4) + (at % (DP / 4) ^ r)) * 4);
+        }
+        if (alone) {
+            const float by = total == 0 ? 0.f : 1.f / total;
+            E e[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) e[x] = A::put(v[x] * by);
+            hh_store_n((E*)a.out + (size_t)piece.seq * a.out_stride + (kvh * a.group + rt * 16 + r) * dim + d, e);
+        } else {
+            *(hh_f32x4*)(p.piece + (rows * 16 + r) * DP + d) = v;
+            if (d == 0) {
+                p.piece_sum[2 * (rows * 16 + r)] = t;
+                p.piece_sum[2 * (rows * 16 + r) + 1] = total;
+            }
+        }
+    }
+}
+
+// The shared tokens' tiles first, then the sequences' own pieces.
+template <class A, class C, int DP, bool FULL>
+HH_DEV void hh_attn_shared(const hh_attn_decode_args& p) {
+    const hh_attn_args& a = p.a;
+    const uint32_t ahead = p.tiles * a.kv.heads * a.splits;
+    if (blockIdx.x >= ahead) {
+        hh_attn_single<A, C, DP, FULL>(p, blockIdx.x - ahead);
+        return;
+    }
+    const uint32_t kvh = blockIdx.x % a.kv.heads, tile = blockIdx.x / a.kv.heads % p.tiles, split = blockIdx.x / a.kv.heads / p.tiles;
+    hh_attn_rows<A, C, DP, FULL, false>(a, hh_attn_tile{0, 0, tile * a.tile_tokens, a.seqs, p.prefix}, p.shared,
+                                        p.shared_entries, kvh, tile * a.kv.heads + kvh, split, a.splits);
+}
+
+// A row's parts joined: sum_i f_i o_i / sum_i f_i s_i, f_i = exp2(base_i - max base).  One head of a sequence a
+// workgroup, DP / 4 threads a part.
+template <class A, int DP>
+HH_DEV void hh_attn_join(const hh_attn_decode_args& p) {
+    typedef typename A::E E;
+    constexpr uint32_t L = DP / 4, N = 256 / L;
+    const hh_attn_args& a = p.a;
+    const uint32_t heads = a.kv.heads * a.group, s = blockIdx.x / heads, head = blockIdx.x % heads;
+    const uint32_t kvh = head / a.group, r = head % a.group, n = threadIdx.x / L, d = threadIdx.x % L * 4;
+    uint32_t from;
+    const uint32_t first = p.plan[2 * s], count = p.plan[2 * s + 1];
+    hh_attn_own(p, s, from);
+    const uint32_t parts = p.prefix && from ? a.splits : 0;
+    if (parts == 0 && count == 1) return;
+    float top = HH_ATTN_LOWEST, sum = 0;
+    hh_f32x4 o = {0, 0, 0, 0};
+    // rows of the shared tokens' parts and of the own pieces
+    const size_t row0 = ((size_t)(s / a.tile_tokens) * a.kv.heads + kvh) * a.splits * 128 + s % a.tile_tokens * a.group + r;
+    const size_t row1 = (((size_t)first * p.row_tiles + r / 16) * a.kv.heads + kvh) * 16 + r % 16, step1 = (size_t)p.row_tiles * a.kv.heads * 16;
+    const float *o0 = a.part + row0 * DP + d, *s0 = a.part_sum + row0 * 2, *o1 = p.piece + row1 * DP + d, *s1 = p.piece_sum + row1 * 2;
+#pragma unroll 4
+    for (uint32_t i = n; i < parts + count; i += N) {
+        const bool own = i >= parts;
+        const size_t at = own ? (i - parts) * step1 : (size_t)i * 128;
+        const float* sums = (own ? s1 : s0) + 2 * at;
+        const hh_f32x4 v = *(const hh_f32x4*)((own ? o1 : o0) + at * DP);
+        const float b = sums[0], w = sums[1];
+        if (w == 0) continue;  // it saw no key
+        const float next = fmaxf(top, b), f = hh_exp2(top - next), g = hh_exp2(b - next);
+        top = next;
+        sum = fmaf(w, g, sum * f);
+#pragma unroll
+        for (int x = 0; x < 4; x++) o[x] = fmaf(v[x], g, o[x] * f);
+    }
+    __shared__ float tops[N], weights[N];
+    __shared__ hh_f32x4 red[256];
+    red[threadIdx.x] = o;
+    if (d == 0) {
+        tops[n] = top;
+        weights[n] = sum;
+    }
+    __syncthreads();
+    if (n || d >= a.kv.dim) return;
+    for (uint32_t i = 1; i < N; i++) top = fmaxf(top, tops[i]);
+    o = hh_f32x4{0, 0, 0, 0};
+    sum = 0;
+    for (uint32_t i = 0; i < N; i++) {
+        const float f = hh_exp2(tops[i] - top);
+        sum = fmaf(weights[i], f, sum);
+#pragma unroll
+        for (int x = 0; x < 4; x++) o[x] = fmaf(red[i * L + threadIdx.x][x], f, o[x]);
+    }
+    const float by = sum == 0 ? 0.f : 1.f / sum;
+    E e[4];
+#pragma unroll
+    for (int x = 0; x < 4; x++) e[x] = A::put(o[x] * by);
+    hh_store_n((E*)a.out + (size_t)s * a.out_stride + head * a.kv.dim + d, e);
+}
+
+#define HH_ATTN_DECODE(N, A, C, D)                                                                                                  \
+    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_decode_##D##_##N(const hh_attn_decode_args p) { \
+        hh_attn_single<A, C, D, true>(p, blockIdx.x);                                                                               \
+    }                                                                                                                               \
+    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_decode_##D##_any_##N(const hh_attn_decode_args p) { \
+        hh_attn_single<A, C, D, false>(p, blockIdx.x);                                                                              \
+    }                                                                                                                               \
+    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_shared_##D##_##N(const hh_attn_decode_args p) { \
+        hh_attn_shared<A, C, D, true>(p);                                                                                           \
+    }                                                                                                                               \
+    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_shared_##D##_any_##N(const hh_attn_decode_args p) { \
+        hh_attn_shared<A, C, D, false>(p);                                                                                          \
+    }
+#define HH_ATTN_DECODES(N, A, C) HH_ATTN_DECODE(N, A, C, 64) HH_ATTN_DECODE(N, A, C, 128) HH_ATTN_DECODE(N, A, C, 256)
+HH_ATTN_DECODES(f32, hh_af32, hh_af32)
+HH_ATTN_DECODES(f16, hh_af16, hh_af16)
+HH_ATTN_DECODES(bf16, hh_abf16, hh_abf16)
+HH_ATTN_DECODES(f32_f16, hh_af32, hh_af16)
+HH_ATTN_DECODES(f32_bf16, hh_af32, hh_abf16)
+#define HH_ATTN_JOIN(N, A, D) \
+    extern "C" __global__ void __launch_bounds__(256) hh_attn_join_##D##_##N(const hh_attn_decode_args p) { hh_attn_join<A, D>(p); }
+#define HH_ATTN_JOINS(N, A) HH_ATTN_JOIN(N, A, 64) HH_ATTN_JOIN(N, A, 128) HH_ATTN_JOIN(N, A, 256)
+HH_ATTN_JOINS(f32, hh_af32)
+HH_ATTN_JOINS(f16, hh_af16)
+HH_ATTN_JOINS(bf16, hh_abf16)

@@ -1,0 +1,219 @@
+// A tile of 128 rows against the keys of a page table: the core of a prompt's attention (attn_prompt.hip) and of
+// a batch's with the tokens that it shares (attn_decode.hip).
+#ifndef HH_KERNELS_ATTN_ROWS_H
+#define HH_KERNELS_ATTN_ROWS_H
+
+#include "attn_tiles.h"
+
+// rows of an LDS tile: 16-byte chunk c of row r lies at chunk c ^ swizzle(r), so that the 16 rows that are read
+// at once lie in all banks
+template <int BYTES>
+HH_DEV constexpr uint32_t hh_attn_swizzle(uint32_t row) {
+    return BYTES == 128 ? row / 2 % 8 : row % 16;
+}
+
+// The tile's rows: heads kvh * group .. of tokens first .. of a run of `tokens`, whose rows of q and out begin at
+// `start`; the run's last token sees `len` keys.
+struct hh_attn_tile {
+    uint32_t seq, start, first, tokens, len;
+};
+
+// CAUSAL: each earlier token sees a key less; else all of them see len, and the sums always go to `part`.  at: the tile's
+// number in `part`; split: which of its `splits` parts of keys.
+template <class A, class C, int DP, bool FULL, bool CAUSAL>
+HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const int32_t* table, uint32_t entries, uint32_t kvh,
+                         uint32_t at, uint32_t split, uint32_t splits) {
+    typedef typename A::E E;
+    typedef typename C::E CE;
+    typedef hh_mat<C> M;
+    typedef typename M::frag F;
+    constexpr int EF = C::VEC, SZ = sizeof(CE), BN = 128 / SZ, NT = BN / 32, NC = DP / (2 * EF), DT = DP / 32;
+    constexpr int NG = BN / 16;  // a page's end may lie after any 16 keys
+    constexpr int KB = DP * SZ, VB = BN * SZ, KBYTES = BN * KB, BYTES = KBYTES + DP * VB;
+    constexpr int KP = KBYTES / 1024 / 4, VP = DP * VB / 1024 / 4;  // 1 KB pieces a wave copies
+    const uint32_t lane = threadIdx.x % HH_WAVE, ln = lane % 32, hf = lane / 32;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / HH_WAVE);
+    const uint32_t dim = FULL ? DP : a.kv.dim, group = a.group, shift = a.kv.shift;
+
+    const uint32_t rows = min(a.tile_tokens, tile.tokens - tile.first) * group;
+    const uint32_t r = wave * 32 + ln, tok = tile.first + min(r, rows - 1) / group, head = kvh * group + min(r, rows - 1) % group;
+    // keys that the lane's row sees, and the tile's first and last row
+    auto seen = [&](uint32_t t) {
+        if (!CAUSAL) return tile.len;
+        return (uint32_t)max(0, min((int)tile.len, (int)tile.len - (int)tile.tokens + (int)t + 1));
+    };
+    const uint32_t limit = seen(tok), least = seen(tile.first), most = seen(tile.first + (rows - 1) / group);
+    const uint32_t tiles = (most + BN - 1) / BN;
+    const uint32_t t0 = (uint32_t)((uint64_t)tiles * split / splits);
+    const uint32_t t1 = (uint32_t)((uint64_t)tiles * (split + 1) / splits);
+
+    F q[NC];
+    const E* qrow = (const E*)a.q + (size_t)(tile.start + tok) * a.q_stride + head * dim;
+#pragma unroll
+    for (int c = 0; c < NC; c++) q[c] = hh_query<A, C, FULL>(qrow, (2 * c + hf) * EF, dim, true);
+
+    // copies: a piece's rows and chunks by lane
+    constexpr int KR = KB / 16 < 64 ? 64 / (KB / 16) : 1;  // rows of K a piece (or one)
+    const uint32_t krow = lane / (KB / 16), vrow = lane / 8;
+    uint32_t id_k = 0, id_v[2] = {0, 0};  // page numbers: lane g's of granule g; the lane's values' granules
+    auto vchunk = [&](int odd) { return lane % 8 ^ hh_attn_swizzle<128>(vrow + 8 * odd); };
+    auto ask = [&](uint32_t t) {
+        id_k = hh_page(table, t * BN + lane % NG * 16, shift, entries);
+#pragma unroll
+        for (int o = 0; o < 2; o++) id_v[o] = hh_page(table, t * BN + vchunk(o) * EF, shift, entries);
+    };
+    const uint8_t* const zeros = (const uint8_t*)&hh_kv_zeros;
+    auto copy = [&](uint8_t* buf, uint32_t t) {
+#pragma unroll
+        for (int i = 0; i < KP; i++) {
+            const uint32_t p = wave * KP + i, row = p * KR + krow;
+            // row 8j + 4h + i of 32 holds key 16 (j / 2) + 8 h + 4 (j % 2) + i of 16-bit types: hf's EF keys are
+            // neighbours in its registers
+            const uint32_t key = SZ == 4 ? row : (row & ~31u) | (row & 16) | (row & 4) << 1 | (row & 8) >> 1 | (row & 3);
+            const uint32_t id = __builtin_amdgcn_readlane(id_k, __builtin_amdgcn_readfirstlane(p * KR / 16));
+            const uint32_t chunk = lane % (KB / 16) ^ hh_attn_swizzle<KB>(row);
+            const bool in = id < a.kv.pages && (FULL || chunk * EF < dim);
+            const uint8_t* src = a.kv.base + id * a.kv.stride +
+                                 hh_kv_key<C>(a.kv, kvh, (t * BN + key) & ((1u << shift) - 1)) + chunk * 16;
+            hh_copy16(in ? src : zeros, buf + p * 1024);
+        }
+#pragma unroll
+        for (int i = 0; i < VP; i++) {
+            const uint32_t p = wave * VP + i, d = p * 8 + vrow, id = id_v[p & 1];
+            const uint8_t* src = a.kv.base + id * a.kv.stride + hh_kv_value<C>(a.kv, kvh, FULL ? d : min(d, dim - 1)) +
+                                 ((t * BN + vchunk(p & 1) * EF) & ((1u << shift) - 1)) * SZ;
+            hh_copy16(id < a.kv.pages ? src : zeros, buf + KBYTES + p * 1024);
+        }
+    };
+
+    hh_f32x16 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++) o[i] = hh_f32x16{};
+    float base = HH_ATTN_LOWEST, sum = 0;
+    uint32_t odd = 0;  // not 0: a value of a crossed tile is no finite number
+    const uint32_t kswz = hh_attn_swizzle<KB>(ln) ^ hf, vswz = hh_attn_swizzle<128>(ln) ^ hf;
+
+    auto compute = [&](uint8_t* buf, uint32_t t) {
+        const uint32_t k0 = t * BN;
+        uint8_t* const vbuf = buf + KBYTES;
+        const bool crossed = k0 + BN > least;
+        if (crossed) {  // values past the sequence's end and those that are no finite numbers as zeros
+            for (uint32_t i = threadIdx.x; i < DP * 8; i += 256) {
+                F* const at = (F*)(vbuf + i / 8 * VB + (i % 8 ^ hh_attn_swizzle<128>(i / 8)) * 16);
+                *at = hh_finite<C>(hh_first<C>(*at, (int)tile.len - (int)(k0 + i % 8 * EF)), odd);
+            }
+            __syncthreads();
+        }
+        float s[NT * 16];
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            hh_f32x16 acc = {};
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                acc = M::mul32(*(const F*)(buf + (j * 32 + ln) * KB + ((2 * c) ^ kswz) * 16), q[c], acc);
+#pragma unroll
+            for (int x = 0; x < 16; x++) s[j * 16 + x] = acc[x];
+        }
+        if (crossed) {
+#pragma unroll
+            for (int x = 0; x < NT * 16; x++)
+                s[x] = k0 + (2 * (x / EF) + hf) * EF + x % EF < limit ? s[x] : -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int x = 1; x < NT * 16; x++) top = fmaxf(top, s[x]);
+        top *= a.c;
+        if (__any(top > base + HH_ATTN_SLACK)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float next = top > base + HH_ATTN_SLACK ? top : base, f = hh_exp2(base - next);
+            base = next;
+            sum *= f;
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) o[i][x] *= f;
+        }
+        F p[NT * 16 / EF];
+#pragma unroll
+        for (int x = 0; x < NT * 16; x++) {
+            s[x] = hh_exp2(fmaf(s[x], a.c, -base));
+            p[x / EF][x % EF] = C::put(s[x]);
+        }
+#pragma unroll
+        for (int w = NT * 8; w > 0; w /= 2)
+#pragma unroll
+            for (int x = 0; x < w; x++) s[x] += s[x + w];
+        sum += s[0];
+        auto value = [&](int i, int f) { return *(const F*)(vbuf + (i * 32 + ln) * VB + ((2 * f) ^ vswz) * 16); };
+#pragma unroll
+        for (int f = 0; f < NT * 16 / EF; f++)
+#pragma unroll
+            for (int i = 0; i < DT; i++) o[i] = M::mul32(value(i, f), p[f], o[i]);
+    };
+
+    uint8_t* const buf0 = hh_attn_lds<0, BYTES>();
+    uint8_t* const buf1 = hh_attn_lds<1, BYTES>();
+    if (t0 < t1) {
+        ask(t0);
+        copy(buf0, t0);
+        ask(t0 + 1);
+    }
+    for (uint32_t t = t0; t < t1; t += 2) {
+        hh_attn_meet();
+        if (t + 1 < t1) copy(buf1, t + 1);
+        ask(t + 2);
+        compute(buf0, t);
+        if (t + 1 >= t1) break;
+        hh_attn_meet();
+        if (t + 2 < t1) copy(buf0, t + 2);
+        ask(t + 3);
+        compute(buf1, t + 1);
+    }
+
+    sum += __shfl_xor(sum, 32);
+    odd = __syncthreads_or(odd != 0);
+    if (r >= rows) return;
+    // what the crossed tiles left out, added for the row's own keys: to element d of this half's
+    auto left_out = [&](auto add) {
+        for (uint32_t key = max(least / BN, t0) * BN; key < min(limit, t1 * BN); key++) {
+            const uint32_t id = hh_page(table, key, shift, entries);
+            if (id >= a.kv.pages) continue;
+            const uint8_t* page = a.kv.base + id * a.kv.stride;
+            for (uint32_t d = hf * 4; d < dim; d += 8)
+                for (uint32_t x = d; x < d + 4; x++) {
+                    const float v = C::get(((const CE*)(page + hh_kv_value<C>(a.kv, kvh, x)))[key & ((1u << shift) - 1)]);
+                    if (!__builtin_isfinite(v)) add(x, v);
+                }
+        }
+    };
+    if (!CAUSAL || splits > 1) {
+        const size_t part = (size_t)at * splits + split;
+        float* const po = a.part + (part * 128 + r) * DP;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                *(hh_f32x4*)(po + i * 32 + j * 8 + hf * 4) = hh_f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+        if (odd) left_out([&](uint32_t d, float v) { po[d] += v; });
+        if (hf == 0) {
+            a.part_sum[2 * (part * 128 + r)] = base;
+            a.part_sum[2 * (part * 128 + r) + 1] = sum;
+        }
+        return;
+    }
+    const float by = sum == 0 ? 0.f : 1.f / sum;
+    E* const out = (E*)a.out + (size_t)(tile.start + tok) * a.out_stride + head * dim;
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t d = i * 32 + j * 8 + hf * 4;
+            E v[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) v[x] = A::put(sum == 0 ? 0.f : o[i][4 * j + x] * by);
+            if (FULL || d < dim) hh_store_n(out + d, v);
+        }
+    if (odd) left_out([&](uint32_t d, float v) { out[d] = A::put(A::get(out[d]) + v); });
+}
+
+#endif

@@ -10,6 +10,7 @@
 #define HH_KERNELS_ATTN_TILES_H
 
 #include "kv_pages.h"
+#include "wave64.h"
 
 typedef float hh_f32x4 __attribute__((ext_vector_type(4)));
 typedef float hh_f32x16 __attribute__((ext_vector_type(16)));
@@ -99,6 +100,10 @@ HH_DEV float hh_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A 16-byte source for what a page number outside the cache stands for: zeros.
 __device__ const hh_u4 hh_kv_zeros = {0, 0, 0, 0};
+
+// Workgroups of four waves that registers are made for: two a CU where a tile fits half its LDS and half its
+// registers.
+#define HH_ATTN_PER_CU(C, D) ((D) == 256 || (sizeof(C::E) == 4 && (D) == 128) ? 1 : 2)
 
 constexpr int hh_attn_wait(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | 0x70 | (lgkm << 8); }
 // This wave's copies into LDS landed and its LDS reads done, then the workgroup meets.

@@ -1,5 +1,5 @@
 // Dispatch of the attention operators: rotary positions into the cache (rope.hip), copies of its
-// pages (kv_pages.hip), attention of prompts (attn_prompt.hip).
+// pages (kv_pages.hip), attention of prompts (attn_prompt.hip) and of decode batches (attn_decode.hip).
 #include <algorithm>
 
 #include "engine.h"
@@ -19,9 +19,11 @@ void attn_kernels(std::vector<std::string>& k) {
         const std::string ty = attn_types(t[0], t[1]);
         for (const char* v : {"halves_", "pairs_"}) k.push_back(std::string("hh_rope_") + v + ty);
         for (const char* v : {"64_", "64_any_", "128_", "128_any_", "256_", "256_any_"})
-            k.push_back(std::string("hh_attn_prompt_") + v + ty);
+            for (const char* kind : {"hh_attn_prompt_", "hh_attn_decode_", "hh_attn_shared_"})
+                k.push_back(std::string(kind) + v + ty);
         for (const char* v : {"64_", "128_", "256_"})
-            if (t[0] == t[1]) k.push_back(std::string("hh_attn_prompt_join_") + v + ty);
+            for (const char* kind : {"hh_attn_prompt_join_", "hh_attn_join_"})
+                if (t[0] == t[1]) k.push_back(std::string(kind) + v + ty);
     }
     k.push_back("hh_kv_copy");
 }
@@ -85,15 +87,16 @@ static std::string dim_name(size_t dim) {
     return std::to_string(padded_dim(dim)) + (dim == padded_dim(dim) ? "_" : "_any_");
 }
 
-hh_status hh_engine::enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_args a) {
+hh_status hh_engine::enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_args p) {
+    hh_attn_args& a = p.a;
     hipFunction_t f, join;
     const size_t dp = padded_dim(a.kv.dim), cus = (size_t)props.multiProcessorCount;
     HH_TRY(kernel("hh_attn_prompt_" + dim_name(a.kv.dim) + attn_types(type, kv_type), &f));
     HH_TRY(kernel("hh_attn_prompt_join_" + std::to_string(dp) + "_" + act_type(type)->name, &join));
     a.tile_tokens = 128 / a.group;
-    a.slots = a.tokens / a.tile_tokens + a.seqs;
-    const size_t tiles = (size_t)a.slots * a.kv.heads;
-    if (tiles >= 1u << 24) return fail(HH_ERR_INVALID, "attn_prompt: %u tokens of %u sequences are too many", a.tokens, a.seqs);
+    const size_t slots = (size_t)p.tokens / a.tile_tokens + a.seqs, tiles = slots * a.kv.heads;
+    if (tiles >= 1u << 24) return fail(HH_ERR_INVALID, "attn_prompt: %u tokens of %u sequences are too many", p.tokens, a.seqs);
+    p.slots = (uint32_t)slots;
     // Few tiles: their keys are split, into parts of 256 keys or more, for two workgroups a CU.
     const size_t keys = (size_t)a.entries << a.kv.shift;
     a.splits = (uint32_t)std::max<size_t>(1, std::min({2 * cus / tiles, keys / 256, (size_t)64}));
@@ -103,11 +106,51 @@ hh_status hh_engine::enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_a
         a.part = (float*)ws_attn;
         a.part_sum = a.part + rows * dp;
     }
-    void* params[] = {&a};
+    void* params[] = {&p};
     HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)tiles, a.splits, 1, 256, 1, 1, 0, stream, params, nullptr),
                "hipModuleLaunchKernel(attn_prompt)");
     if (a.splits > 1)
         HH_TRY_HIP(hipModuleLaunchKernel(join, (uint32_t)tiles, (uint32_t)(128 * dp / 1024), 1, 256, 1, 1, 0, stream, params, nullptr),
                    "hipModuleLaunchKernel(attn_prompt_join)");
+    return HH_OK;
+}
+
+hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_args p) {
+    hh_attn_args& a = p.a;
+    hipFunction_t f, join;
+    const size_t dp = padded_dim(a.kv.dim), cus = (size_t)props.multiProcessorCount, heads = a.kv.heads;
+    // Shared tokens are taken apart in whole tiles of keys, of two sequences on and from 256 of them.
+    p.prefix = a.seqs < 2 || p.prefix < 256 ? 0 : p.prefix / 64 * 64;
+    HH_TRY(kernel((p.prefix ? "hh_attn_shared_" : "hh_attn_decode_") + dim_name(a.kv.dim) + attn_types(type, kv_type), &f));
+    HH_TRY(kernel("hh_attn_join_" + std::to_string(dp) + "_" + act_type(type)->name, &join));
+    size_t ahead = 0, part_rows = 0;
+    if (p.prefix) {
+        a.tile_tokens = 128 / a.group;
+        p.tiles = (a.seqs + a.tile_tokens - 1) / a.tile_tokens;
+        const size_t tiles = p.tiles * heads;
+        a.splits = (uint32_t)std::max<size_t>(1, std::min<size_t>(2 * cus / tiles, p.prefix / 256));
+        ahead = tiles * a.splits;
+        part_rows = ahead * 128;
+    }
+    // The sequences' own tokens: pieces of at least one unit, four workgroups a CU.
+    p.row_tiles = (a.group + 15) / 16;
+    p.pieces = (uint32_t)std::max<size_t>(1, 4 * cus / (heads * p.row_tiles));
+    p.least = 1;
+    const size_t numbers = (size_t)p.pieces + a.seqs, blocks = numbers * p.row_tiles * heads, piece_rows = blocks * 16;
+    if (ahead + blocks >= 1u << 24 || a.seqs * heads * a.group >= 1u << 24)
+        return fail(HH_ERR_INVALID, "attn_decode: %u sequences are too many", a.seqs);
+    HH_TRY(grow(&ws_attn, &ws_attn_cap, (part_rows + piece_rows) * (dp + 2) * sizeof(float) + a.seqs * 8));
+    a.part = (float*)ws_attn;
+    p.piece = a.part + part_rows * dp;
+    a.part_sum = p.piece + piece_rows * dp;
+    p.piece_sum = a.part_sum + part_rows * 2;
+    p.plan = (uint32_t*)(p.piece_sum + piece_rows * 2);
+    void* params[] = {&p};
+    HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)(ahead + blocks), 1, 1, 256, 1, 1, 0, stream, params, nullptr),
+               "hipModuleLaunchKernel(attn_decode)");
+    // (no table has room for a second piece: every row is whole)
+    if (p.prefix || ((size_t)a.entries << a.kv.shift) > 128 * p.least)
+        HH_TRY_HIP(hipModuleLaunchKernel(join, (uint32_t)(a.seqs * heads * a.group), 1, 1, 256, 1, 1, 0, stream, params, nullptr),
+                   "hipModuleLaunchKernel(attn_join)");
     return HH_OK;
 }

@@ -1124,27 +1124,65 @@ hh_status hh_attn_prompt_dev(hh_engine* e, const hh_attn_prompt_desc* d, const h
     HH_TRY(check_kv_type(d->type, kv, "attn_prompt"));
     hh_attn_prompt_args a{};
     size_t layer = 0, qs = d->q_stride, os = d->out_stride;
-    HH_TRY(check_kv(e, kv, cache, cache_off, 1, &layer, &a.kv, "attn_prompt cache"));
+    HH_TRY(check_kv(e, kv, cache, cache_off, 1, &layer, &a.a.kv, "attn_prompt cache"));
     HH_TRY(check_attn(e, d->type, d->scale, d->tokens, d->seqs, d->q_heads, d->table_stride, kv, q, q_off, &qs, out, out_off,
                       &os, lens, lens_off, tables, tables_off, "attn_prompt"));
     HH_TRY(check_vector(e, starts, starts_off, d->seqs + 1, "attn_prompt starts"));
     if (d->tokens == 0 || d->seqs == 0) return HH_OK;
     HH_TRY(e->select());
-    a.q = at(q, q_off);
-    a.out = at(out, out_off);
+    a.a.q = at(q, q_off);
+    a.a.out = at(out, out_off);
+    a.a.lens = (const int32_t*)at(lens, lens_off);
+    a.a.tables = (const int32_t*)at(tables, tables_off);
+    a.a.q_stride = qs;
+    a.a.out_stride = os;
+    a.a.seqs = (uint32_t)d->seqs;
+    a.a.entries = (uint32_t)d->table_stride;
+    a.a.group = (uint32_t)(d->q_heads / kv->kv_heads);
+    a.a.c = (float)((double)d->scale * 1.4426950408889634074);
     a.starts = (const int32_t*)at(starts, starts_off);
-    a.lens = (const int32_t*)at(lens, lens_off);
-    a.tables = (const int32_t*)at(tables, tables_off);
-    a.q_stride = qs;
-    a.out_stride = os;
     a.tokens = (uint32_t)d->tokens;
-    a.seqs = (uint32_t)d->seqs;
-    a.entries = (uint32_t)d->table_stride;
-    a.group = (uint32_t)(d->q_heads / kv->kv_heads);
-    a.c = (float)((double)d->scale * 1.4426950408889634074);
     try {
         std::lock_guard<std::mutex> lk(e->ws_mutex);
         return e->enqueue_attn_prompt(d->type, kv->type, a);
+    } catch (const std::bad_alloc&) {
+        return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
+}
+
+hh_status hh_attn_decode_dev(hh_engine* e, const hh_attn_decode_desc* d, const hh_kv_desc* kv, const hh_buf* q,
+                             size_t q_off, const hh_buf* cache, size_t cache_off, const hh_buf* prefix_pages,
+                             size_t prefix_pages_off, const hh_buf* lens, size_t lens_off, const hh_buf* tables,
+                             size_t tables_off, hh_buf* out, size_t out_off) {
+    HH_NOT_NULL(e, "engine");
+    HH_NOT_NULL(d, "attn_decode desc");
+    HH_TRY(check_kv_type(d->type, kv, "attn_decode"));
+    hh_attn_decode_args a{};
+    size_t layer = 0, qs = d->q_stride, os = d->out_stride;
+    HH_TRY(check_kv(e, kv, cache, cache_off, 1, &layer, &a.a.kv, "attn_decode cache"));
+    HH_TRY(check_attn(e, d->type, d->scale, d->seqs, d->seqs, d->q_heads, d->table_stride, kv, q, q_off, &qs, out, out_off,
+                      &os, lens, lens_off, tables, tables_off, "attn_decode"));
+    if (d->prefix > INT32_MAX) return fail(HH_ERR_INVALID, "attn_decode: prefix=%zu exceeds 31 bits", d->prefix);
+    const size_t shared = (d->prefix + kv->page_size - 1) / kv->page_size;
+    if (shared) HH_TRY(check_vector(e, prefix_pages, prefix_pages_off, shared, "attn_decode prefix_pages"));
+    if (d->seqs == 0) return HH_OK;
+    HH_TRY(e->select());
+    a.a.q = at(q, q_off);
+    a.a.out = at(out, out_off);
+    a.a.lens = (const int32_t*)at(lens, lens_off);
+    a.a.tables = (const int32_t*)at(tables, tables_off);
+    a.a.q_stride = qs;
+    a.a.out_stride = os;
+    a.a.seqs = (uint32_t)d->seqs;
+    a.a.entries = (uint32_t)d->table_stride;
+    a.a.group = (uint32_t)(d->q_heads / kv->kv_heads);
+    a.a.c = (float)((double)d->scale * 1.4426950408889634074);
+    a.shared = (const int32_t*)at(prefix_pages, prefix_pages_off);
+    a.prefix = (uint32_t)d->prefix;
+    a.shared_entries = (uint32_t)shared;
+    try {
+        std::lock_guard<std::mutex> lk(e->ws_mutex);
+        return e->enqueue_attn_decode(d->type, kv->type, a);
     } catch (const std::bad_alloc&) {
         return fail(HH_ERR_OUT_OF_MEMORY, "host allocation failed");
     }

@@ -356,7 +356,8 @@ struct hh_engine {
     // Attention over pages (attn.cpp).
     hh_status enqueue_rope(int type, int kv_type, int layout, size_t tokens, const hh_rope_args& a);
     hh_status enqueue_kv_copy(size_t layers, const hh_kv_copy_args& a);
-    hh_status enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_args a);
+    hh_status enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_args p);
+    hh_status enqueue_attn_decode(int type, int kv_type, hh_attn_decode_args p);
     // Reports (and clears) a grid-barrier timeout recorded by a fused kernel.  Syncs.
     hh_status check_device_error();
 };

@@ -785,6 +785,20 @@ class HipEngine:
                                            cache_off, starts.handle, starts_off, lens.handle, lens_off, tables.handle,
                                            tables_off, out.handle, out_off))
 
+    @staticmethod
+    def attn_decode_desc(ggml_type: int, seqs: int, q_heads: int, scale: float, table_stride: int, prefix: int = 0,
+                         q_stride: int = 0, out_stride: int = 0) -> _abi.AttnDecodeDesc:
+        return _abi.AttnDecodeDesc(ggml_type, scale, seqs, q_heads, prefix, table_stride, q_stride, out_stride)
+
+    def attn_decode_dev(self, desc: _abi.AttnDecodeDesc, kv: _abi.KvDesc, q: DeviceBuffer, q_off: int, cache: DeviceBuffer,
+                        cache_off: int, prefix_pages, prefix_pages_off: int, lens: DeviceBuffer, lens_off: int,
+                        tables: DeviceBuffer, tables_off: int, out: DeviceBuffer, out_off: int) -> None:
+        """Attention of one token a sequence over its lens[s] cached tokens, of which the first `prefix` are the
+        same in all sequences and are read once, from prefix_pages.  Enqueue only."""
+        _check(self.lib.hh_attn_decode_dev(self.handle, C.byref(desc), C.byref(kv), q.handle, q_off, cache.handle,
+                                           cache_off, _handle(prefix_pages), prefix_pages_off, lens.handle, lens_off,
+                                           tables.handle, tables_off, out.handle, out_off))
+
     # ---------------------------------------------------------------- synthetic data
     def synth_weights_dev(self, ggml_type: int, dst: DeviceBuffer, off: int, n_blocks: int, seed: int,
                           lo: float, hi: float) -> None:

@@ -506,7 +506,8 @@ hh_status hh_sample_dev(hh_engine* e, const hh_sample_desc* d, const hh_buf* log
 /* No counterpart in the reference's device runtime (its attention runs on the CPU).  What a layer
  * does between the products of its queries, keys and values and that of its output, over a cache of
  * pages: hh_rope_kv_dev turns queries and keys by their positions and puts keys and values into the
- * cache, hh_kv_copy_dev copies pages (forked sequences, a cache made dense again).
+ * cache, hh_kv_copy_dev copies pages (forked sequences, a cache made dense again), hh_attn_prompt_dev and
+ * hh_attn_decode_dev are the attention of prompts and of a decode batch.
  *
  * Activations are of `type`, as in the 8-bit path (element-aligned byte offsets, rows `*_stride`
  * elements apart, 0: packed); a row holds its token's heads one after another, kv.head_dim elements
@@ -514,7 +515,8 @@ hh_status hh_sample_dev(hh_engine* e, const hh_sample_desc* d, const hh_buf* log
  * activations; other pairs are HH_ERR_KERNEL_MISSING.  Page numbers, slots, positions and lengths are
  * int32 on the device, read when the kernels run, so a captured graph follows what they hold at its
  * replay; none of them can lead a kernel outside the buffers that were named.  All calls are
- * enqueue-only and give the same bits every time.  Buffers of one call must not overlap except where
+ * enqueue-only, may be captured into a graph (the attention after one eager call of the same sizes, for its
+ * workspace) and give the same bits every time.  Buffers of one call must not overlap except where
  * said. */
 
 /* A cache of n_pages pages, page p `page_stride` elements after page p - 1 (0: packed).  A page has
@@ -599,6 +601,26 @@ hh_status hh_attn_prompt_dev(hh_engine* e, const hh_attn_prompt_desc* d, const h
                              size_t q_off, const hh_buf* cache, size_t cache_off, const hh_buf* starts, size_t starts_off,
                              const hh_buf* lens, size_t lens_off, const hh_buf* tables, size_t tables_off, hh_buf* out,
                              size_t out_off);
+
+/* The same for one new token a sequence: row s of q and out is sequence s's last token, which sees all of its lens[s]
+ * cached tokens (tables as above; none: zeros, as for the padding of a batch).
+ * prefix: the sequences' first `prefix` tokens are the same, and prefix_pages (int32[prefix / page_size, rounded up])
+ * names pages that hold them: row 0 of tables, say.  They are read once for all sequences.  A sequence of
+ * fewer tokens reads its own table alone.  prefix 0 (prefix_pages unused, may be NULL): none are shared.  What the
+ * tables' rows name for these tokens has to be the same keys and values, in the same pages or in copies. */
+typedef struct hh_attn_decode_desc {
+    int type;            /* of q and out */
+    float scale;         /* > 0, finite */
+    size_t seqs;
+    size_t q_heads;      /* 1..64 times kv_heads */
+    size_t prefix;
+    size_t table_stride; /* pages a sequence can have */
+    size_t q_stride, out_stride; /* elements */
+} hh_attn_decode_desc;
+hh_status hh_attn_decode_dev(hh_engine* e, const hh_attn_decode_desc* d, const hh_kv_desc* kv, const hh_buf* q,
+                             size_t q_off, const hh_buf* cache, size_t cache_off, const hh_buf* prefix_pages,
+                             size_t prefix_pages_off, const hh_buf* lens, size_t lens_off, const hh_buf* tables,
+                             size_t tables_off, hh_buf* out, size_t out_off);
 
 /* ------------------------------------------------------------------ streaming ------- */
 

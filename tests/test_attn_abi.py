@@ -68,3 +68,13 @@ def test_rope_factors_refused():
         assert lib.hh_rope_factors(*args, C.cast(out, C.c_void_p), None) == 2, args
     assert lib.hh_rope_factors(0, 64, 1e4, 2.0, 100.0, None, None) == 2
     assert lib.hh_rope_factors(0, 64, 1e4, 2.0, 100.0, C.cast(out, C.c_void_p), None) == 0
+
+
+def test_attention_null_arguments_and_layout():
+    lib, kv = _abi.load(), _abi.KvDesc()
+    assert lib.hh_attn_prompt_dev(None, C.byref(_abi.AttnPromptDesc()), C.byref(kv), *[None, 0] * 6) == 2
+    assert b"engine is NULL" in lib.hh_last_error()
+    assert lib.hh_attn_decode_dev(None, C.byref(_abi.AttnDecodeDesc()), C.byref(kv), *[None, 0] * 6) == 2
+    assert b"engine is NULL" in lib.hh_last_error()
+    assert C.sizeof(_abi.AttnPromptDesc) == 56 and _abi.AttnPromptDesc.table_stride.offset == 32
+    assert C.sizeof(_abi.AttnDecodeDesc) == 56 and _abi.AttnDecodeDesc.prefix.offset == 24
