@@ -253,63 +253,23 @@ HH_DEV void hh_attn_shared(const hh_attn_decode_args& p) {
                                         p.shared_entries, kvh, tile * a.kv.heads + kvh, split, a.splits);
 }
 
-// A row's parts joined: sum_i f_i o_i / sum_i f_i s_i, f_i = exp2(base_i - max base).  One head of a sequence a
-// workgroup, DP / 4 threads a part.
+// A row's parts, joined: one head of a sequence a workgroup.
 template <class A, int DP>
 HH_DEV void hh_attn_join(const hh_attn_decode_args& p) {
-    typedef typename A::E E;
-    constexpr uint32_t L = DP / 4, N = 256 / L;
     const hh_attn_args& a = p.a;
     const uint32_t heads = a.kv.heads * a.group, s = blockIdx.x / heads, head = blockIdx.x % heads;
-    const uint32_t kvh = head / a.group, r = head % a.group, n = threadIdx.x / L, d = threadIdx.x % L * 4;
-    uint32_t from;
+    const uint32_t kvh = head / a.group, r = head % a.group;
     const uint32_t first = p.plan[2 * s], count = p.plan[2 * s + 1];
+    uint32_t from;
     hh_attn_own(p, s, from);
-    const uint32_t parts = p.prefix && from ? a.splits : 0;
-    if (parts == 0 && count == 1) return;
-    float top = HH_ATTN_LOWEST, sum = 0;
-    hh_f32x4 o = {0, 0, 0, 0};
-    // rows of the shared tokens' parts and of the own pieces
+    const uint32_t splits = p.prefix && from ? a.splits : 0;
+    if (splits == 0 && count == 1) return;
     const size_t row0 = ((size_t)(s / a.tile_tokens) * a.kv.heads + kvh) * a.splits * 128 + s % a.tile_tokens * a.group + r;
-    const size_t row1 = (((size_t)first * p.row_tiles + r / 16) * a.kv.heads + kvh) * 16 + r % 16, step1 = (size_t)p.row_tiles * a.kv.heads * 16;
-    const float *o0 = a.part + row0 * DP + d, *s0 = a.part_sum + row0 * 2, *o1 = p.piece + row1 * DP + d, *s1 = p.piece_sum + row1 * 2;
-#pragma unroll 4
-    for (uint32_t i = n; i < parts + count; i += N) {
-        const bool own = i >= parts;
-        const size_t at = own ? (i - parts) * step1 : (size_t)i * 128;
-        const float* sums = (own ? s1 : s0) + 2 * at;
-        const hh_f32x4 v = *(const hh_f32x4*)((own ? o1 : o0) + at * DP);
-        const float b = sums[0], w = sums[1];
-        if (w == 0) continue;  // it saw no key
-        const float next = fmaxf(top, b), f = hh_exp2(top - next), g = hh_exp2(b - next);
-        top = next;
-        sum = fmaf(w, g, sum * f);
-#pragma unroll
-        for (int x = 0; x < 4; x++) o[x] = fmaf(v[x], g, o[x] * f);
-    }
-    __shared__ float tops[N], weights[N];
-    __shared__ hh_f32x4 red[256];
-    red[threadIdx.x] = o;
-    if (d == 0) {
-        tops[n] = top;
-        weights[n] = sum;
-    }
-    __syncthreads();
-    if (n || d >= a.kv.dim) return;
-    for (uint32_t i = 1; i < N; i++) top = fmaxf(top, tops[i]);
-    o = hh_f32x4{0, 0, 0, 0};
-    sum = 0;
-    for (uint32_t i = 0; i < N; i++) {
-        const float f = hh_exp2(tops[i] - top);
-        sum = fmaf(weights[i], f, sum);
-#pragma unroll
-        for (int x = 0; x < 4; x++) o[x] = fmaf(red[i * L + threadIdx.x][x], f, o[x]);
-    }
-    const float by = sum == 0 ? 0.f : 1.f / sum;
-    E e[4];
-#pragma unroll
-    for (int x = 0; x < 4; x++) e[x] = A::put(o[x] * by);
-    hh_store_n((E*)a.out + (size_t)s * a.out_stride + head * a.kv.dim + d, e);
+    const size_t row1 = (((size_t)first * p.row_tiles + r / 16) * a.kv.heads + kvh) * 16 + r % 16;
+    hh_attn_join_row<A, DP>(hh_attn_parts{a.part + row0 * DP, a.part_sum + row0 * 2, splits, 128},
+                            hh_attn_parts{p.piece + row1 * DP, p.piece_sum + row1 * 2, count, (size_t)p.row_tiles * a.kv.heads * 16},
+                            1024 / DP, threadIdx.x % (DP / 4) * 4 < a.kv.dim,
+                            (typename A::E*)a.out + (size_t)s * a.out_stride + head * a.kv.dim);
 }
 
 #define HH_ATTN_DECODE(N, A, C, D)                                                                                                  \

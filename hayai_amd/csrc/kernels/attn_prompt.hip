@@ -47,39 +47,24 @@ HH_DEV void hh_attn_prompt(const hh_attn_prompt_args& p) {
                                        slot * p.a.kv.heads + kvh, blockIdx.y, gridDim.y);
 }
 
-// The pieces of rows whose keys were split, joined: sum_i f_i o_i / sum_i f_i s_i, f_i = exp2(base_i - max base).
-// A piece that saw no key has sum 0 and is left out (its o may hold 0 * NaN).
+// The parts of rows whose keys were split, joined.
 template <class A, int DP>
 HH_DEV void hh_attn_prompt_join(const hh_attn_prompt_args& p) {
     const hh_attn_args& a = p.a;
-    typedef typename A::E E;
     const uint32_t kvh = blockIdx.x % a.kv.heads, slot = p.slots - 1 - blockIdx.x / a.kv.heads;
     hh_attn_tile tile;
     if (!hh_attn_find(p, slot, threadIdx.x % HH_WAVE, tile)) return;
     const uint32_t rows = min(a.tile_tokens, tile.tokens - tile.first) * a.group;
-    const uint32_t at = blockIdx.y * 256 + threadIdx.x, r = at / (DP / 4), d = at % (DP / 4) * 4;
-    if (r >= rows || d >= a.kv.dim) return;
-    const size_t part = ((size_t)slot * a.kv.heads + kvh) * a.splits * 128 + r;
-    float top = HH_ATTN_LOWEST;
-    for (uint32_t i = 0; i < a.splits; i++) top = fmaxf(top, a.part_sum[2 * (part + i * 128)]);
-    hh_f32x4 o = {0, 0, 0, 0};
-    float sum = 0;
-    for (uint32_t i = 0; i < a.splits; i++) {
-        const float s = a.part_sum[2 * (part + i * 128) + 1], b = a.part_sum[2 * (part + i * 128)];
-        if (s == 0) continue;
-        const float f = hh_exp2(b - top);
-        const hh_f32x4 v = *(const hh_f32x4*)(a.part + (part + i * 128) * DP + d);
-        sum = fmaf(s, f, sum);
-#pragma unroll
-        for (int x = 0; x < 4; x++) o[x] = fmaf(v[x], f, o[x]);
-    }
-    const uint32_t head = kvh * a.group + r % a.group;
-    E* const out = (E*)a.out + (size_t)(tile.start + tile.first + r / a.group) * a.out_stride + head * a.kv.dim + d;
-    const float by = sum == 0 ? 0.f : 1.f / sum;
-    E v[4];
-#pragma unroll
-    for (int x = 0; x < 4; x++) v[x] = A::put(o[x] * by);
-    hh_store_n(out, v);
+    constexpr uint32_t N = 1024 / DP;
+    uint32_t teams = 1;  // a row
+    while (teams < N && teams < a.splits) teams *= 2;
+    const uint32_t r = blockIdx.y * (N / teams) + threadIdx.x / (DP / 4) / teams, at = min(r, rows - 1);
+    if (blockIdx.y * (N / teams) >= rows) return;
+    const size_t row = ((size_t)slot * a.kv.heads + kvh) * a.splits * 128 + at;
+    const hh_attn_parts parts = {a.part + row * DP, a.part_sum + row * 2, a.splits, 128};
+    typename A::E* const out = (typename A::E*)a.out + (size_t)(tile.start + tile.first + at / a.group) * a.out_stride +
+                               (kvh * a.group + at % a.group) * a.kv.dim;
+    hh_attn_join_row<A, DP>(parts, hh_attn_parts{}, teams, r < rows && threadIdx.x % (DP / 4) * 4 < a.kv.dim, out);
 }
 
 #define HH_ATTN_PROMPT(N, A, C, D)                                                                                            \

@@ -93,6 +93,7 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
     uint32_t odd = 0;  // not 0: a value of a crossed tile is no finite number
     const uint32_t kswz = hh_attn_swizzle<KB>(ln) ^ hf, vswz = hh_attn_swizzle<128>(ln) ^ hf;
 
+    const bool idle = wave * 32 >= rows;
     auto compute = [&](uint8_t* buf, uint32_t t) {
         const uint32_t k0 = t * BN;
         uint8_t* const vbuf = buf + KBYTES;
@@ -104,6 +105,7 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
             }
             __syncthreads();
         }
+        if (idle) return;
         float s[NT * 16];
 #pragma unroll
         for (int j = 0; j < NT; j++) {
@@ -214,6 +216,61 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
             if (FULL || d < dim) hh_store_n(out + d, v);
         }
     if (odd) left_out([&](uint32_t d, float v) { out[d] = A::put(A::get(out[d]) + v); });
+}
+
+// Two runs of a row's parts, joined: sum_i f_i o_i / sum_i f_i s_i, f_i = exp2(base_i - max base), by `teams` (a power of
+// two) of the workgroup's teams of DP / 4 threads, which hold 4 elements each and take every teams-th part; all threads
+// call it, and the first team's store the row.  A part that saw no key has sum 0 and is left out (its o may hold
+// 0 * NaN).
+struct hh_attn_parts {
+    const float *o, *s;  // the first part's elements, base and sum
+    uint32_t n;
+    size_t step;  // rows from a part to the next
+};
+template <class A, int DP>
+HH_DEV void hh_attn_join_row(const hh_attn_parts& x, const hh_attn_parts& y, uint32_t teams, bool store, typename A::E* out) {
+    typedef typename A::E E;
+    constexpr uint32_t L = DP / 4, N = 256 / L;
+    const uint32_t team = threadIdx.x / L, d = threadIdx.x % L * 4;
+    float top = HH_ATTN_LOWEST, sum = 0;
+    hh_f32x4 o = {0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t i = team % teams; i < x.n + y.n; i += teams) {
+        const bool late = i >= x.n;
+        const size_t at = late ? (i - x.n) * y.step : i * x.step;
+        const float* sums = (late ? y.s : x.s) + 2 * at;
+        const hh_f32x4 v = *(const hh_f32x4*)((late ? y.o : x.o) + at * DP + d);
+        const float b = sums[0], w = sums[1];
+        const bool any = w != 0;
+        const float next = any ? fmaxf(top, b) : top, f = hh_exp2(top - next), g = hh_exp2(b - next);
+        top = next;
+        sum = any ? fmaf(w, g, sum * f) : sum;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = any ? fmaf(v[e], g, o[e] * f) : o[e];
+    }
+    __shared__ float tops[N], weights[N];
+    __shared__ hh_f32x4 red[256];
+    red[threadIdx.x] = o;
+    if (d == 0) {
+        tops[team] = top;
+        weights[team] = sum;
+    }
+    __syncthreads();
+    if (team % teams || !store) return;
+    for (uint32_t i = 1; i < teams; i++) top = fmaxf(top, tops[team + i]);
+    o = hh_f32x4{0, 0, 0, 0};
+    sum = 0;
+    for (uint32_t i = 0; i < teams; i++) {
+        const float f = hh_exp2(tops[team + i] - top);
+        sum = fmaf(weights[team + i], f, sum);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(red[i * L + threadIdx.x][e], f, o[e]);
+    }
+    const float by = sum == 0 ? 0.f : 1.f / sum;
+    E v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = A::put(o[e] * by);
+    hh_store_n(out + d, v);
 }
 
 #endif

@@ -109,8 +109,10 @@ hh_status hh_engine::enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_a
     void* params[] = {&p};
     HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)tiles, a.splits, 1, 256, 1, 1, 0, stream, params, nullptr),
                "hipModuleLaunchKernel(attn_prompt)");
+    size_t teams = 1;  // of dp / 4 threads a row
+    while (teams < 1024 / dp && teams < a.splits) teams *= 2;
     if (a.splits > 1)
-        HH_TRY_HIP(hipModuleLaunchKernel(join, (uint32_t)tiles, (uint32_t)(128 * dp / 1024), 1, 256, 1, 1, 0, stream, params, nullptr),
+        HH_TRY_HIP(hipModuleLaunchKernel(join, (uint32_t)tiles, (uint32_t)(128 * teams * dp / 1024), 1, 256, 1, 1, 0, stream, params, nullptr),
                    "hipModuleLaunchKernel(attn_prompt_join)");
     return HH_OK;
 }
@@ -119,6 +121,7 @@ hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_a
     hh_attn_args& a = p.a;
     hipFunction_t f, join;
     const size_t dp = padded_dim(a.kv.dim), cus = (size_t)props.multiProcessorCount, heads = a.kv.heads;
+    const size_t part_keys = act_type(kv_type)->bytes == 4 ? 64 : 256;  // (f32 products take eight times as long)
     // Shared tokens are taken apart in whole tiles of keys, of two sequences on and from 256 of them.
     p.prefix = a.seqs < 2 || p.prefix < 256 ? 0 : p.prefix / 64 * 64;
     HH_TRY(kernel((p.prefix ? "hh_attn_shared_" : "hh_attn_decode_") + dim_name(a.kv.dim) + attn_types(type, kv_type), &f));
@@ -128,7 +131,7 @@ hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_a
         a.tile_tokens = 128 / a.group;
         p.tiles = (a.seqs + a.tile_tokens - 1) / a.tile_tokens;
         const size_t tiles = p.tiles * heads;
-        a.splits = (uint32_t)std::max<size_t>(1, std::min<size_t>(2 * cus / tiles, p.prefix / 256));
+        a.splits = (uint32_t)std::max<size_t>(1, std::min<size_t>(2 * cus / tiles, p.prefix / part_keys));
         ahead = tiles * a.splits;
         part_rows = ahead * 128;
     }
