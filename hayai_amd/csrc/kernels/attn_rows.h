@@ -53,36 +53,59 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
     for (int c = 0; c < NC; c++) q[c] = hh_query<A, C, FULL>(qrow, (2 * c + hf) * EF, dim, true);
 
     // copies: a piece's rows and chunks by lane
-    constexpr int KR = KB / 16 < 64 ? 64 / (KB / 16) : 1;  // rows of K a piece (or one)
-    const uint32_t krow = lane / (KB / 16), vrow = lane / 8;
+    constexpr int KC = KB / 16, KR = 64 / KC;  // chunks of a row of K, rows a piece
+    const uint32_t krow = lane / KC, vrow = lane / 8, pmask = (1u << shift) - 1;
     uint32_t id_k = 0, id_v[2] = {0, 0};  // page numbers: lane g's of granule g; the lane's values' granules
     auto vchunk = [&](int odd) { return lane % 8 ^ hh_attn_swizzle<128>(vrow + 8 * odd); };
-    auto ask = [&](uint32_t t) {
-        id_k = hh_page(table, t * BN + lane % NG * 16, shift, entries);
+    auto ask_k = [&](uint32_t t) { id_k = hh_page(table, t * BN + lane % NG * 16, shift, entries); };
+    auto ask_v = [&](uint32_t t) {
 #pragma unroll
         for (int o = 0; o < 2; o++) id_v[o] = hh_page(table, t * BN + vchunk(o) * EF, shift, entries);
     };
+    // row 8j + 4h + i of 32 holds key 16 (j / 2) + 8 h + 4 (j % 2) + i of 16-bit types: hf's EF keys are neighbours in
+    // its registers
+    auto key_of = [&](uint32_t row) {
+        return SZ == 4 ? row : (row & ~31u) | (row & 16) | (row & 4) << 1 | (row & 8) >> 1 | (row & 3);
+    };
     const uint8_t* const zeros = (const uint8_t*)&hh_kv_zeros;
-    auto copy = [&](uint8_t* buf, uint32_t t) {
+    const uint32_t p0k = wave * KP, p0v = wave * VP;
+    uint32_t koff[KP];  // from the piece's 16 keys on
+#pragma unroll
+    for (int i = 0; i < KP; i++) {
+        const uint32_t row = (p0k + i) * KR + krow;
+        koff[i] = key_of(row) % 16 * dim * SZ + (lane % KC ^ hh_attn_swizzle<KB>(row)) * 16;
+    }
+    auto copy_k = [&](uint8_t* buf, uint32_t t) {
 #pragma unroll
         for (int i = 0; i < KP; i++) {
-            const uint32_t p = wave * KP + i, row = p * KR + krow;
-            // row 8j + 4h + i of 32 holds key 16 (j / 2) + 8 h + 4 (j % 2) + i of 16-bit types: hf's EF keys are
-            // neighbours in its registers
-            const uint32_t key = SZ == 4 ? row : (row & ~31u) | (row & 16) | (row & 4) << 1 | (row & 8) >> 1 | (row & 3);
-            const uint32_t id = __builtin_amdgcn_readlane(id_k, __builtin_amdgcn_readfirstlane(p * KR / 16));
-            const uint32_t chunk = lane % (KB / 16) ^ hh_attn_swizzle<KB>(row);
-            const bool in = id < a.kv.pages && (FULL || chunk * EF < dim);
-            const uint8_t* src = a.kv.base + id * a.kv.stride +
-                                 hh_kv_key<C>(a.kv, kvh, (t * BN + key) & ((1u << shift) - 1)) + chunk * 16;
-            hh_copy16(in ? src : zeros, buf + p * 1024);
+            const uint32_t g = __builtin_amdgcn_readfirstlane((p0k + i) * KR / 16);
+            const uint32_t id = __builtin_amdgcn_readlane(id_k, g);
+            const uint8_t* from = a.kv.base + id * a.kv.stride + hh_kv_key<C>(a.kv, kvh, (t * BN + g * 16) & pmask);
+            uint8_t* const to = buf + (p0k + i) * 1024;
+            if (FULL && __builtin_expect(id < a.kv.pages, 1))
+                hh_copy16(from + koff[i], to);
+            else
+                hh_copy16(id < a.kv.pages && (lane % KC ^ hh_attn_swizzle<KB>((p0k + i) * KR + krow)) * EF < dim ? from + koff[i] : zeros, to);
         }
+    };
+    auto copy_v = [&](uint8_t* buf, uint32_t t) {
+        const uint8_t* from[2];
+        const bool in[2] = {id_v[0] < a.kv.pages, id_v[1] < a.kv.pages};
 #pragma unroll
-        for (int i = 0; i < VP; i++) {
-            const uint32_t p = wave * VP + i, d = p * 8 + vrow, id = id_v[p & 1];
-            const uint8_t* src = a.kv.base + id * a.kv.stride + hh_kv_value<C>(a.kv, kvh, FULL ? d : min(d, dim - 1)) +
-                                 ((t * BN + vchunk(p & 1) * EF) & ((1u << shift) - 1)) * SZ;
-            hh_copy16(id < a.kv.pages ? src : zeros, buf + KBYTES + p * 1024);
+        for (int o = 0; o < 2; o++)
+            from[o] = a.kv.base + id_v[o] * a.kv.stride + ((t * BN + vchunk(o) * EF) & pmask) * SZ + (vrow << shift) * SZ;
+        const uint32_t first = hh_kv_value<C>(a.kv, kvh, 0);
+        if (FULL && __builtin_expect(__all(in[0] && in[1]), 1)) {
+#pragma unroll
+            for (int i = 0; i < VP; i++)
+                hh_copy16(from[(VP * 4 > 4 ? i : p0v + i) & 1] + (first + ((p0v + i) * 8 << shift) * SZ), buf + (p0v + i) * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VP; i++) {
+                const uint32_t o = (p0v + i) & 1, d = (p0v + i) * 8;  // (rows past dim: the last one's place)
+                const uint8_t* src = (o ? from[1] : from[0]) + (first + ((min(d + vrow, dim - 1) - vrow) << shift) * SZ);
+                hh_copy16((o ? in[1] : in[0]) ? src : zeros, buf + (p0v + i) * 1024);
+            }
         }
     };
 
@@ -107,15 +130,16 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
         }
         if (idle) return;
         float s[NT * 16];
+        hh_f32x16 acc[NT];
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            hh_f32x16 acc = {};
+        for (int j = 0; j < NT; j++) acc[j] = hh_f32x16{};
 #pragma unroll
-            for (int c = 0; c < NC; c++)
-                acc = M::mul32(*(const F*)(buf + (j * 32 + ln) * KB + ((2 * c) ^ kswz) * 16), q[c], acc);
+        for (int c = 0; c < NC; c++)
 #pragma unroll
-            for (int x = 0; x < 16; x++) s[j * 16 + x] = acc[x];
-        }
+            for (int j = 0; j < NT; j++)
+                acc[j] = M::mul32(*(const F*)(buf + (j * 32 + ln) * KB + ((2 * c) ^ kswz) * 16), q[c], acc[j]);
+#pragma unroll
+        for (int x = 0; x < NT * 16; x++) s[x] = acc[x / 16][x % 16];
         if (crossed) {
 #pragma unroll
             for (int x = 0; x < NT * 16; x++)
@@ -136,16 +160,14 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
                 for (int x = 0; x < 16; x++) o[i][x] *= f;
         }
         F p[NT * 16 / EF];
+        float sums[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int x = 0; x < NT * 16; x++) {
-            s[x] = hh_exp2(fmaf(s[x], a.c, -base));
-            p[x / EF][x % EF] = C::put(s[x]);
+            const float w = hh_exp2(fmaf(s[x], a.c, -base));
+            p[x / EF][x % EF] = C::put(w);
+            sums[x % 4] += w;
         }
-#pragma unroll
-        for (int w = NT * 8; w > 0; w /= 2)
-#pragma unroll
-            for (int x = 0; x < w; x++) s[x] += s[x + w];
-        sum += s[0];
+        sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         auto value = [&](int i, int f) { return *(const F*)(vbuf + (i * 32 + ln) * VB + ((2 * f) ^ vswz) * 16); };
 #pragma unroll
         for (int f = 0; f < NT * 16 / EF; f++)
@@ -156,19 +178,30 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
     uint8_t* const buf0 = hh_attn_lds<0, BYTES>();
     uint8_t* const buf1 = hh_attn_lds<1, BYTES>();
     if (t0 < t1) {
-        ask(t0);
-        copy(buf0, t0);
-        ask(t0 + 1);
+        ask_k(t0);
+        ask_v(t0);
+        copy_k(buf0, t0);
+        copy_v(buf0 + KBYTES, t0);
+        ask_k(t0 + 1);
+        ask_v(t0 + 1);
     }
     for (uint32_t t = t0; t < t1; t += 2) {
         hh_attn_meet();
-        if (t + 1 < t1) copy(buf1, t + 1);
-        ask(t + 2);
+        if (t + 1 < t1) {
+            copy_k(buf1, t + 1);
+            copy_v(buf1 + KBYTES, t + 1);
+        }
+        ask_k(t + 2);
+        ask_v(t + 2);
         compute(buf0, t);
         if (t + 1 >= t1) break;
         hh_attn_meet();
-        if (t + 2 < t1) copy(buf0, t + 2);
-        ask(t + 3);
+        if (t + 2 < t1) {
+            copy_k(buf0, t + 2);
+            copy_v(buf0 + KBYTES, t + 2);
+        }
+        ask_k(t + 3);
+        ask_v(t + 3);
         compute(buf1, t + 1);
     }
 
