@@ -196,7 +196,9 @@ struct hh_attn_decode_args {
     float* piece;
     float* piece_sum;
     uint32_t* plan;  // each sequence's first piece and how many it has
-    uint32_t prefix, shared_entries, tiles, row_tiles, pieces, least;
+    uint32_t prefix, shared_entries, tiles, row_tiles;
+    uint32_t room;           // units of own tokens that a table has room for
+    uint32_t pieces, least;  // at most (but for one a sequence more); for a workgroup a CU
 };
 
 // Synthetic GGUF bytes: splitmix64 stream, then f16 scale fields drawn U(lo, hi).

@@ -6,13 +6,13 @@
 // of one kv head's up to 16 heads, memory bound: keys and values go from the pages straight into operands of
 // the 16-column matrix products (attn_tiles.h), 16 KB in flight a wave, each of the four waves every fourth
 // step of 32 keys (16 of f32), joined through LDS at the end.  Lengths are known on the device alone, so every workgroup sums them up
-// and finds the piece of work that falls to it: as many pieces as the chip has room for, of equal length
-// whatever the sequences' are.  A second kernel joins the parts of a row.
+// and finds the piece of work that falls to it: pieces are of equal length whatever the sequences' are.  A second kernel joins the parts of a row.
 //
 // Weights are rounded to the cache's type for the second product; sums and the parts are f32.
 #include "attn_rows.h"
 
-#define HH_ATTN_UNIT 128  // keys a piece is a multiple of
+#define HH_ATTN_UNIT 128u  // keys a piece is a multiple of
+#define HH_ATTN_MOST 64u   // pieces of a sequence
 
 // Tokens of sequence s that no other shares, and the first of them.  A sequence shorter than the prefix takes no
 // part in it.
@@ -25,45 +25,49 @@ HH_DEV uint32_t hh_attn_own(const hh_attn_decode_args& p, uint32_t s, uint32_t& 
 struct hh_attn_piece {
     uint32_t seq, at, count, units;  // the at-th of the sequence's `count` pieces of `units` units
 };
-// Piece number `piece`; the first workgroup leaves the plan for the join.
-HH_DEV bool hh_attn_plan(const hh_attn_decode_args& p, uint32_t piece, bool first, hh_attn_piece& mine) {
-    __shared__ uint32_t red[8];
+// Piece number `piece`; the first workgroup leaves the plan for the join.  (32-bit sums: the host bounds what the tables
+// have room for.)
+HH_DEV bool hh_attn_plan(const hh_attn_decode_args& p, uint32_t piece, bool first, hh_attn_piece& out) {
+    __shared__ uint32_t red[8], sums[4];
     __shared__ hh_attn_piece found;
     const uint32_t tid = threadIdx.x, lane = tid % HH_WAVE, wave = tid / HH_WAVE;
+    // a sequence's units, and how many of them count: one that is shorter than the prefix has longer pieces
     auto units = [&](uint32_t s) {
         uint32_t from;
         return s < p.a.seqs ? (hh_attn_own(p, s, from) + HH_ATTN_UNIT - 1) / HH_ATTN_UNIT : 0;
     };
-    uint64_t all = 0;
-    for (uint32_t s = tid; s < p.a.seqs; s += 256) all += units(s);
-    all = hh_wave64<hh_addu64>(all);
-    __shared__ uint64_t sums[4];
+    uint32_t all = 0;
+    for (uint32_t s = tid; s < p.a.seqs; s += 256) all += min(units(s), p.room);
+    all = (uint32_t)hh_wave64<hh_addu64>(all);
     if (lane == 0) sums[wave] = all;
     if (tid == 0) found.count = 0;
     __syncthreads();
     all = sums[0] + sums[1] + sums[2] + sums[3];
-    const uint32_t each = (uint32_t)max((uint64_t)p.least, (all + p.pieces - 1) / p.pieces);
+    // Units a piece: four (one sequence of 4000: 7.7 us, with two 9.2), fewer where that would leave CUs without one, more
+    // where pieces would be too many in all or, for the join, in one sequence.
+    const uint32_t each = max((all + p.pieces - 1) / p.pieces, min(4u, max(1u, all / p.least)));
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < p.a.seqs; s0 += 256) {
-        const uint32_t s = s0 + tid, n = s < p.a.seqs ? max(1u, (units(s) + each - 1) / each) : 0;
-        const uint32_t scan = (uint32_t)hh_scan64(n);
-        if (lane == HH_WAVE - 1) red[wave + (s0 / 256 & 1) * 4] = scan;
+        const uint32_t s = s0 + tid, own = units(s), most = min(HH_ATTN_MOST, (p.room + each - 1) / each);
+        const uint32_t size = max(each, (own + max(1u, most) - 1) / max(1u, most));
+        const uint32_t n = s < p.a.seqs ? max(1u, (own + size - 1) / size) : 0, scan = (uint32_t)hh_scan64(n);
+        uint32_t* const part = red + (s0 / 256 & 1) * 4;
+        if (lane == HH_WAVE - 1) part[wave] = scan;
         __syncthreads();
-        uint32_t base = before;
+        uint32_t at = before + scan - n;
         for (uint32_t w = 0; w < 4; w++) {
-            if (w < wave) base += red[w + (s0 / 256 & 1) * 4];
-            before += red[w + (s0 / 256 & 1) * 4];
+            if (w < wave) at += part[w];
+            before += part[w];
         }
-        const uint32_t at = base + scan - n;
-        if (piece - at < n) found = hh_attn_piece{s, piece - at, n, each};
+        if (piece - at < n) found = hh_attn_piece{s, piece - at, n, size};
         if (first && s < p.a.seqs) {
             p.plan[2 * s] = at;
             p.plan[2 * s + 1] = n;
         }
     }
     __syncthreads();
-    mine = found;
-    return mine.count != 0;
+    out = found;
+    return out.count != 0;
 }
 
 template <class A, class C, int DP, bool FULL>

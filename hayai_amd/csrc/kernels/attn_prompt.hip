@@ -19,21 +19,29 @@ HH_DEV bool hh_attn_find(const hh_attn_prompt_args& p, uint32_t slot, uint32_t l
     const hh_attn_args& a = p.a;
     auto start = [&](uint32_t s) { return (uint32_t)max(0, min((int)p.tokens, p.starts[s])); };
     uint32_t lo = 0, hi = a.seqs;  // 64 sequences at a time, one a lane
-    while (hi - lo > 1) {
-        const uint32_t step = (hi - lo + 63) / 64, s = lo + lane * step;
-        const bool before = s < hi && start(min(s, a.seqs)) / a.tile_tokens + s <= slot;
-        const uint32_t n = max(1, __popcll(__ballot(before)));
-        lo += (n - 1) * step;
+    uint32_t from, to;
+    int len;
+    for (;;) {
+        const uint32_t step = (hi - lo + 63) / 64, s = lo + lane * step, here = min(s, a.seqs - 1);
+        const uint32_t f = start(here), e = start(here + 1);  // (asked for at once: one latency)
+        const int n = a.lens[here];
+        const bool before = s < hi && f / a.tile_tokens + s <= slot;
+        const uint32_t at = max(1, __popcll(__ballot(before))) - 1;
+        from = __builtin_amdgcn_readlane(f, at);
+        to = __builtin_amdgcn_readlane(e, at);
+        len = __builtin_amdgcn_readlane(n, at);
+        lo += at * step;
+        if (step == 1) break;
         hi = min(lo + step, hi);
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
-    const uint32_t from = start(lo), to = start(lo + 1), at = from / a.tile_tokens + lo;
+    const uint32_t at = from / a.tile_tokens + lo;
     t.seq = lo;
     t.start = from;
     t.tokens = to > from ? to - from : 0;
     if (slot < at || (uint64_t)(slot - at) * a.tile_tokens >= t.tokens) return false;
     t.first = (slot - at) * a.tile_tokens;
-    t.len = (uint32_t)min((int64_t)max(0, a.lens[lo]), (int64_t)a.entries << a.kv.shift);
+    t.len = (uint32_t)min((int64_t)max(0, len), (int64_t)a.entries << a.kv.shift);
     return true;
 }
 

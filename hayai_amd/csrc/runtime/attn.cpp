@@ -124,24 +124,33 @@ hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_a
     const size_t part_keys = act_type(kv_type)->bytes == 4 ? 64 : 256;  // (f32 products take eight times as long)
     // Shared tokens are taken apart in whole tiles of keys, of two sequences on and from 256 of them.
     p.prefix = a.seqs < 2 || p.prefix < 256 ? 0 : p.prefix / 64 * 64;
-    HH_TRY(kernel((p.prefix ? "hh_attn_shared_" : "hh_attn_decode_") + dim_name(a.kv.dim) + attn_types(type, kv_type), &f));
+    const std::string name = (p.prefix ? "hh_attn_shared_" : "hh_attn_decode_") + dim_name(a.kv.dim) + attn_types(type, kv_type);
+    HH_TRY(kernel(name, &f));
     HH_TRY(kernel("hh_attn_join_" + std::to_string(dp) + "_" + act_type(type)->name, &join));
     size_t ahead = 0, part_rows = 0;
     if (p.prefix) {
         a.tile_tokens = 128 / a.group;
         p.tiles = (a.seqs + a.tile_tokens - 1) / a.tile_tokens;
         const size_t tiles = p.tiles * heads;
-        a.splits = (uint32_t)std::max<size_t>(1, std::min<size_t>(2 * cus / tiles, p.prefix / part_keys));
+        a.splits = (uint32_t)std::max<size_t>(1, std::min<size_t>(cus / 2 / tiles, p.prefix / part_keys));
         ahead = tiles * a.splits;
         part_rows = ahead * 128;
     }
-    // The sequences' own tokens: pieces of at least one unit, four workgroups a CU.
+    // The sequences' own tokens: the kernel makes pieces by the lengths (hh_attn_plan).  Each workgroup that is not
+    // needed costs its look at the lengths, so that their number follows what the tables have room for: eight a CU for
+    // long ones (64 sequences of 2000: 106 us, four 114), else four (64 of 8192 + 500: 46, eight 49).
     p.row_tiles = (a.group + 15) / 16;
-    p.pieces = (uint32_t)std::max<size_t>(1, 4 * cus / (heads * p.row_tiles));
-    p.least = 1;
-    const size_t numbers = (size_t)p.pieces + a.seqs, blocks = numbers * p.row_tiles * heads, piece_rows = blocks * 16;
-    if (ahead + blocks >= 1u << 24 || a.seqs * heads * a.group >= 1u << 24)
+    const size_t keys = (size_t)a.entries << a.kv.shift, room = ((keys > p.prefix ? keys - p.prefix : 0) + 127) / 128;
+    const size_t least = std::max<size_t>(1, cus / (heads * p.row_tiles));
+    if (a.seqs * heads * a.group >= 1u << 24 || std::max<size_t>(room, 1) * a.seqs >= 1u << 31)
         return fail(HH_ERR_INVALID, "attn_decode: %u sequences are too many", a.seqs);
+    p.room = (uint32_t)room;
+    p.least = (uint32_t)least;
+    p.pieces = (uint32_t)std::min(std::max(room * a.seqs / 8, 4 * least), 8 * least);
+    // (with fewer than four units a piece there are fewer than twice `least` of them)
+    const size_t numbers = std::min(room * a.seqs, std::max(2 * least, std::min<size_t>(p.pieces, room * a.seqs / 4))) + a.seqs;
+    const size_t blocks = numbers * p.row_tiles * heads, piece_rows = blocks * 16;
+    if (ahead + blocks >= 1u << 24) return fail(HH_ERR_INVALID, "attn_decode: %u sequences are too many", a.seqs);
     HH_TRY(grow(&ws_attn, &ws_attn_cap, (part_rows + piece_rows) * (dp + 2) * sizeof(float) + a.seqs * 8));
     a.part = (float*)ws_attn;
     p.piece = a.part + part_rows * dp;
@@ -152,7 +161,7 @@ hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_a
     HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)(ahead + blocks), 1, 1, 256, 1, 1, 0, stream, params, nullptr),
                "hipModuleLaunchKernel(attn_decode)");
     // (no table has room for a second piece: every row is whole)
-    if (p.prefix || ((size_t)a.entries << a.kv.shift) > 128 * p.least)
+    if (p.prefix || room > 1)
         HH_TRY_HIP(hipModuleLaunchKernel(join, (uint32_t)(a.seqs * heads * a.group), 1, 1, 256, 1, 1, 0, stream, params, nullptr),
                    "hipModuleLaunchKernel(attn_join)");
     return HH_OK;
