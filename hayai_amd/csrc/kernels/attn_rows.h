@@ -241,12 +241,30 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
 #pragma unroll
     for (int i = 0; i < DT; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t d = i * 32 + j * 8 + hf * 4;
-            E v[4];
+        for (int j = 0; j < 4; j += 2) {
+            E v[2][4];
 #pragma unroll
-            for (int x = 0; x < 4; x++) v[x] = A::put(sum == 0 ? 0.f : o[i][4 * j + x] * by);
-            if (FULL || d < dim) hh_store_n(out + d, v);
+            for (int x = 0; x < 8; x++) v[x / 4][x % 4] = A::put(sum == 0 ? 0.f : o[i][4 * j + x] * by);
+            if (sizeof(E) == 4) {
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t d = i * 32 + (j + k) * 8 + hf * 4;
+                    if (FULL || d < dim) hh_store_n(out + d, v[k]);
+                }
+            } else {  // 8 bytes of j and j + 1 here and in the row's other half: 16 of one of them in each
+                uint32_t u[2][2];
+                __builtin_memcpy(u, v, 16);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const auto both = __builtin_amdgcn_permlane32_swap(u[0][k], u[1][k], false, false);
+                    u[0][k] = both[0];
+                    u[1][k] = both[1];
+                }
+                E w[8];
+                __builtin_memcpy(w, u, 16);
+                const uint32_t d = i * 32 + (j + hf) * 8;
+                if (FULL || d < dim) hh_store_n(out + d, w);
+            }
         }
     if (odd) left_out([&](uint32_t d, float v) { out[d] = A::put(A::get(out[d]) + v); });
 }

@@ -105,6 +105,25 @@ __device__ const hh_u4 hh_kv_zeros = {0, 0, 0, 0};
 // registers.
 #define HH_ATTN_PER_CU(C, D) ((D) == 256 || (sizeof(C::E) == 4 && (D) == 128) ? 1 : 2)
 
+template <class Op>
+HH_DEV uint32_t hh_wave32(uint32_t v) {
+    v = Op::of(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
+    v = Op::of(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
+    v = Op::of(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));
+    v = Op::of(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true));
+    v = Op::of(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, true));
+    v = Op::of(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, true));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+struct hh_add32 {
+    HH_DEV static uint32_t of(uint32_t a, uint32_t b) { return a + b; }
+};
+struct hh_max32 {
+    HH_DEV static uint32_t of(uint32_t a, uint32_t b) { return a > b ? a : b; }
+};
+HH_DEV uint32_t hh_wave_sum32(uint32_t v) { return hh_wave32<hh_add32>(v); }
+HH_DEV uint32_t hh_wave_max32(uint32_t v) { return hh_wave32<hh_max32>(v); }
+
 constexpr int hh_attn_wait(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | 0x70 | (lgkm << 8); }
 // This wave's copies into LDS landed and its LDS reads done, then the workgroup meets.
 HH_DEV void hh_attn_meet() {
