@@ -155,7 +155,7 @@ struct hh_rope_args {
     uint64_t q_stride, k_stride, v_stride, out_stride;
     double log2_base;
     float mscale;
-    uint32_t heads, rot;
+    uint32_t tokens, heads, rot;
 };
 
 // Pages moves[i][0] -> moves[i][1] in each layer (kv_pages.hip); strides and sizes in bytes.

@@ -17,7 +17,7 @@ static const int kAttnTypes[][2] = {{HH_TYPE_F32, HH_TYPE_F32}, {HH_TYPE_F16, HH
 void attn_kernels(std::vector<std::string>& k) {
     for (auto& t : kAttnTypes) {
         const std::string ty = attn_types(t[0], t[1]);
-        for (const char* v : {"halves_", "pairs_"}) k.push_back(std::string("hh_rope_") + v + ty);
+        for (const char* v : {"halves_", "pairs_", "halves8_", "pairs8_"}) k.push_back(std::string("hh_rope_") + v + ty);
         for (const char* v : {"64_", "64_any_", "128_", "128_any_", "256_", "256_any_"})
             for (const char* kind : {"hh_attn_prompt_", "hh_attn_decode_", "hh_attn_shared_"})
                 k.push_back(std::string(kind) + v + ty);
@@ -40,15 +40,19 @@ using namespace hh;
 
 hh_status hh_engine::enqueue_rope(int type, int kv_type, int layout, size_t tokens, const hh_rope_args& a) {
     hipFunction_t f;
-    HH_TRY(kernel(std::string("hh_rope_") + (layout == HH_ROPE_PAIRS ? "pairs_" : "halves_") + attn_types(type, kv_type), &f));
-    // a workgroup's 256 threads take a token's 16-byte pieces; of few tokens each is given to several
     const size_t el = act_type(type)->bytes, cus = (size_t)props.multiProcessorCount;
+    // Eight tokens a workgroup of 1024 threads from four workgroups every CU on, else one a workgroup of 256, and of few
+    // tokens each is given to several.
+    const size_t each = tokens >= 8 * cus ? 8 : 1;
+    HH_TRY(kernel(std::string("hh_rope_") + (layout == HH_ROPE_PAIRS ? "pairs" : "halves") + (each == 8 ? "8_" : "_") +
+                      attn_types(type, kv_type), &f));
     const size_t pieces = (a.heads + 2 * (size_t)a.kv.heads) * ((a.kv.dim * el + 15) / 16);
-    const size_t parts = std::max<size_t>(1, std::min((pieces + 255) / 256, 2 * cus / tokens));
+    const size_t parts = each == 8 ? 1 : std::max<size_t>(1, std::min((pieces + 255) / 256, 2 * cus / tokens));
     // a grid has fewer than 2^32 threads: 2^20 tokens at a time (parts are 1 there)
     for (size_t t = 0; t < tokens; t += (size_t)1 << 20) {
         const size_t n = std::min(tokens - t, (size_t)1 << 20);
         hh_rope_args p = a;
+        p.tokens = (uint32_t)n;
         p.q = (const char*)a.q + t * a.q_stride * el;
         p.k = (const char*)a.k + t * a.k_stride * el;
         p.v = (const char*)a.v + t * a.v_stride * el;
@@ -56,7 +60,8 @@ hh_status hh_engine::enqueue_rope(int type, int kv_type, int layout, size_t toke
         p.positions = a.positions + t;
         p.slots = a.slots + t;
         void* params[] = {&p};
-        HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)n, (uint32_t)parts, 1, 256, 1, 1, 0, stream, params, nullptr),
+        HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)((n + each - 1) / each), (uint32_t)parts, 1, each == 8 ? 1024 : 256, 1, 1, 0,
+                                         stream, params, nullptr),
                    "hipModuleLaunchKernel(rope)");
     }
     return HH_OK;

@@ -127,21 +127,60 @@ def test_rope(engine, ty, cty, layout):
         assert torch.equal(new[untouched], cache[untouched])
 
 
+@pytest.mark.parametrize("layout", [ROPE_HALVES, ROPE_PAIRS])
+@pytest.mark.parametrize("ty,cty", TYPES)
+def test_rope_prompt(engine, ty, cty, layout):
+    """Enough tokens for several of them a workgroup: runs of slots, runs that a page ends, slots of nobody's, a
+    rest of less than eight."""
+    t, heads, kvh, dim, rot, page = 8 * engine.device_info.compute_units + 13, 3, 2, 72, 44, 16
+    rng = np.random.default_rng(21)
+    x = normal(22, t, (heads + 2 * kvh) * dim).to(DT[ty])
+    n_pages = t // page + 40
+    slots = np.arange(t, dtype=np.int32) + page * 3
+    slots[200:900] = rng.permutation(np.arange(page * 3 + 200, page * 3 + 900))
+    slots[1000:1200] += 3  # runs that do not begin at a multiple of eight
+    slots[1200:1203] = -1
+    slots[1400:] += 64
+    positions = rng.integers(0, 100000, t).astype(np.int32)
+    el, wide = torch.empty(0, dtype=DT[ty]).element_size(), x.shape[1]
+    per = 2 * kvh * page * dim
+    cache = normal(23, n_pages, per).to(DT[cty])
+    xb, cb, out = put(engine, x), put(engine, cache), engine.alloc(t * heads * dim * el)
+    d = engine.rope_desc(ty, t, heads, rot, 10000.0, q_stride=wide, k_stride=wide, v_stride=wide, layout=layout)
+    engine.rope_kv_dev(d, engine.kv_desc(cty, kvh, dim, page, n_pages), xb, 0, xb, heads * dim * el, xb,
+                       (heads + kvh) * dim * el, ints(engine, positions.tolist()), 0, ints(engine, slots.tolist()), 0, None, 0,
+                       out, 0, cb, 0)
+    x64 = x.double().reshape(t, heads + 2 * kvh, dim)
+    want = turned(x64[:, :heads + kvh], positions, rot, 10000.0, layout, None, 1.0)
+    size = (x64[:, :heads + kvh] ** 2).sum(-1, keepdim=True).sqrt().expand_as(want) * 1.5 * 4 * 2.0**-24
+    size[..., rot:] = 0
+    near(get(out, DT[ty], (t, heads, dim)), want[:, :heads], DT[ty], size[:, :heads])
+    expect, slack = cache.double().clone(), torch.zeros(n_pages, per, dtype=torch.float64)
+    keep = np.nonzero(slots >= 0)[0]
+    p, at = torch.from_numpy(slots[keep] // page).long(), torch.from_numpy(slots[keep] % page).long()
+    expect[:, :per // 2].view(-1, kvh, page, dim)[p, :, at] = want[keep, heads:]
+    slack[:, :per // 2].view(-1, kvh, page, dim)[p, :, at] = size[keep, heads:]
+    expect[:, per // 2:].view(-1, kvh, dim, page)[p, :, :, at] = x64[keep, heads + kvh:]
+    new = get(cb, DT[cty], (n_pages, per))
+    near(new, expect, DT[cty], slack)
+    assert torch.equal(new[:3], cache[:3])
+
+
 def test_rope_in_place(engine):
-    t, heads, kvh, dim, page = 130, 12, 2, 128, 16
-    for layout in (ROPE_HALVES, ROPE_PAIRS):
+    heads, kvh, dim, page = 12, 2, 128, 16
+    for layout, t in ((ROPE_HALVES, 130), (ROPE_PAIRS, 130), (ROPE_HALVES, 2500), (ROPE_PAIRS, 2500)):
         x = normal(7, t, (heads + 2 * kvh) * dim).to(torch.bfloat16)
         outs = []
         for in_place in (False, True):
-            xb, cb = put(engine, x), engine.alloc(20 * 2 * kvh * page * dim * 2)
+            xb, cb = put(engine, x), engine.alloc(160 * 2 * kvh * page * dim * 2)
             cb.fill(0)
             out = xb if in_place else engine.alloc(x.numel() * 2)
             wide = x.shape[1]
             d = engine.rope_desc(BF16, t, heads, dim, q_stride=wide, k_stride=wide, v_stride=wide, out_stride=wide, layout=layout)
-            kv = engine.kv_desc(BF16, kvh, dim, page, 20)
+            kv = engine.kv_desc(BF16, kvh, dim, page, 160)
             engine.rope_kv_dev(d, kv, xb, 0, xb, heads * dim * 2, xb, (heads + kvh) * dim * 2, ints(engine, list(range(t))), 0,
                                ints(engine, list(range(t))), 0, None, 0, out, 0, cb, 0)
-            outs.append((get(out, torch.bfloat16, (t, wide))[:, :heads * dim], get(cb, torch.bfloat16, (20, 2 * kvh * page * dim))))
+            outs.append((get(out, torch.bfloat16, (t, wide))[:, :heads * dim], get(cb, torch.bfloat16, (160, 2 * kvh * page * dim))))
         assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
 
 
