@@ -168,11 +168,45 @@ def test_starts_that_do_not_ascend(engine):
     check(got[:20].reshape(20, 4, 64), want[:20], bound[:20], F16)
 
 
-def test_many_sequences(engine):
-    """More than the search takes at once, many of them empty."""
-    rng = np.random.default_rng(4)
-    seqs = [(int(n), int(n) + int(m)) for n, m in zip(rng.integers(0, 3, 300), rng.integers(0, 20, 300))]
+@pytest.mark.parametrize("count", [2, 63, 64, 65, 300])
+def test_many_sequences(engine, count):
+    """As many as are put in order, and more than the search takes at once; many of them empty, some long."""
+    rng = np.random.default_rng(count)
+    new = rng.integers(0, 3, count) * rng.choice([1, 1, 1, 40], count)
+    seqs = [(int(n), int(n) + int(m)) for n, m in zip(new, rng.integers(-5, 20, count))]
     Problem(F32, F32, seqs, 2, 1, 64, 16, seed=6).check(engine)
+    Problem(BF16, BF16, seqs, 64, 1, 64, 16, seed=7).check(engine)  # two tokens a tile
+
+
+def test_captured(engine):
+    """A captured prompt follows what its lists and queries hold at each replay; split keys and whole ones."""
+    for seqs, page in [([(9, 900), (30, 64), (1, 70)], 16), ([(60, 60), (70, 80)], 64)]:
+        p = Problem(BF16, BF16, seqs, 8, 2, 128, page, seed=15)
+        wide, kv = 1024, engine.kv_desc(BF16, 2, 128, page, p.n_pages)
+        b = {k: put(engine, v) for k, v in (("q", p.q), ("cache", p.cache), ("out", torch.zeros(p.tokens, wide).bfloat16()))}
+        starts, lens, tables = ints(engine, p.starts.tolist()), ints(engine, p.lens.tolist()), ints(engine, p.tables.reshape(-1).tolist())
+        d = engine.attn_prompt_desc(BF16, p.tokens, len(seqs), 8, p.scale, p.width)
+
+        def call():
+            engine.attn_prompt_dev(d, kv, b["q"], 0, b["cache"], 0, starts, 0, lens, 0, tables, 0, b["out"], 0)
+
+        call()
+        graph = engine.capture(call)
+        for step in range(3):
+            cut = [p.tokens // 3 + step, 0, 0][:len(seqs)]
+            new = [cut[0], p.tokens - cut[0]] + [0] * (len(seqs) - 2)
+            p.seqs = [(n, length) for n, (_, length) in zip(new, seqs)]
+            p.starts = np.cumsum([0] + new).astype(np.int32)
+            p.q = normal(step + 30, p.tokens, wide).bfloat16()
+            starts.write(p.starts)
+            b["q"].write(p.q.view(torch.uint8).numpy())
+            graph.launch()
+            want, bound = p.want()
+            check(get(b["out"], torch.bfloat16, want.shape), want, bound, BF16)
+            eager = get(b["out"], torch.bfloat16, (p.tokens, wide))
+            call()
+            assert torch.equal(eager, get(b["out"], torch.bfloat16, (p.tokens, wide)))
+        graph.free()
 
 
 def test_large_scores(engine):
