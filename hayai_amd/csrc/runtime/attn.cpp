@@ -102,9 +102,14 @@ hh_status hh_engine::enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_a
     const size_t slots = (size_t)p.tokens / a.tile_tokens + a.seqs, tiles = slots * a.kv.heads;
     if (tiles >= 1u << 24) return fail(HH_ERR_INVALID, "attn_prompt: %u tokens of %u sequences are too many", p.tokens, a.seqs);
     p.slots = (uint32_t)slots;
-    // Few tiles: their keys are split, into parts of 256 keys or more, for two workgroups a CU.
+    // Few tiles: their keys are split, for two workgroups a CU.  A part's sums cost 4 KB a head and token (its rows of them,
+    // written and read), so that it is the longer the more waves have rows: 128 keys each (3956 tokens of 8 sequences, 2 heads
+    // of 80 f16: parts of 512 34 us, of 220 40; 12 tokens behind 4704, 4/2 heads of 256: parts of 256 25 us, of 512 35), 16 of
+    // f32, whose products take eight times as long (512 tokens, 8/2 heads of 128: parts of 64 31 us, of 128 34, of 256 48).
     const size_t keys = (size_t)a.entries << a.kv.shift;
-    a.splits = (uint32_t)std::max<size_t>(1, std::min({2 * cus / tiles, keys / 256, (size_t)64}));
+    const size_t waves = std::min<size_t>(4, ((size_t)p.tokens * a.group / a.seqs + 31) / 32);
+    const size_t least = std::max<size_t>(waves, 1) * (act_type(kv_type)->bytes == 4 ? 16 : 128);
+    a.splits = (uint32_t)std::max<size_t>(1, std::min({2 * cus / tiles, keys / least, (size_t)64}));
     if (a.splits > 1) {
         const size_t rows = tiles * a.splits * 128;
         HH_TRY(grow(&ws_attn, &ws_attn_cap, rows * (dp + 2) * sizeof(float)));
@@ -127,8 +132,13 @@ hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_a
     hipFunction_t f, join;
     const size_t dp = padded_dim(a.kv.dim), cus = (size_t)props.multiProcessorCount, heads = a.kv.heads;
     const size_t part_keys = act_type(kv_type)->bytes == 4 ? 64 : 256;  // (f32 products take eight times as long)
-    // Shared tokens are taken apart in whole tiles of keys, of two sequences on and from 256 of them.
-    p.prefix = a.seqs < 2 || p.prefix < 256 ? 0 : p.prefix / 64 * 64;
+    // Shared tokens are taken apart, in whole tiles of keys, where that saves attn_share_min bytes of reading: more kernels' time
+    // than it costs (us, apart and not; 8/2 heads of 128 bf16 unless said: 8 x 1024, 7 MB: 12.2, 9.6; 4 x 4096, 13 MB: 12.9,
+    // 13.5; 30 x 1024, 30 MB: 14.4, 14.7; 60 x 600 of 9/3 heads of 64 f32, 54 MB: 14.3, 20.1; 2 x 8192 of 32/8, 34 MB: 15.9,
+    // 23.1; 16 x 2048 of 32/8, 126 MB: 15.0, 29.1).
+    const size_t token = 2 * heads * a.kv.dim * act_type(kv_type)->bytes;
+    const bool apart = a.seqs > 1 && (double)(a.seqs - 1) * p.prefix * (double)token >= (double)attn_share_min;
+    p.prefix = apart ? p.prefix / 64 * 64 : 0;
     const std::string name = (p.prefix ? "hh_attn_shared_" : "hh_attn_decode_") + dim_name(a.kv.dim) + attn_types(type, kv_type);
     HH_TRY(kernel(name, &f));
     HH_TRY(kernel("hh_attn_join_" + std::to_string(dp) + "_" + act_type(type)->name, &join));
@@ -136,8 +146,10 @@ hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_a
     if (p.prefix) {
         a.tile_tokens = 128 / a.group;
         p.tiles = (a.seqs + a.tile_tokens - 1) / a.tile_tokens;
-        const size_t tiles = p.tiles * heads;
-        a.splits = (uint32_t)std::max<size_t>(1, std::min<size_t>(cus / 2 / tiles, p.prefix / part_keys));
+        // parts for half the CUs, more where not all four waves have rows (2 sequences of 8192, 32/8 heads of 128 bf16: 32 parts
+        // 15.8 us, 16 parts 18.9; 64: 8 parts 49, 16 parts 54)
+        const size_t tiles = p.tiles * heads, waves = std::min<size_t>(4, ((size_t)a.seqs * a.group + 31) / 32);
+        a.splits = (uint32_t)std::max<size_t>(1, std::min<size_t>(2 * cus / waves / tiles, p.prefix / part_keys));
         ahead = tiles * a.splits;
         part_rows = ahead * 128;
     }

@@ -2172,6 +2172,7 @@ hh_status engine_create(int device, hh_engine** out) {
     if (const char* f = getenv("HAYAI_HIP_BLOCK_STREAM")) e->block_stream = atoi(f) != 0;
     if (const char* f = getenv("HAYAI_HIP_BLOCK_STREAM_MIN")) e->block_stream_min = (size_t)atoll(f);
     if (const char* f = getenv("HAYAI_HIP_MMF_MIN")) e->mmf_min = (size_t)std::max(65, atoi(f));
+    if (const char* f = getenv("HAYAI_HIP_ATTN_SHARE_MIN")) e->attn_share_min = strtoull(f, nullptr, 10);
     if (const char* f = getenv("HAYAI_HIP_MMI_MIN")) e->mmi_min = (size_t)std::max(2, atoi(f));
     if (const char* f = getenv("HAYAI_HIP_MMI_D")) e->mmi_d = atoi(f);
     err = hipMalloc(&e->grid_sync, kBarBytes);

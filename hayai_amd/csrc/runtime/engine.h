@@ -203,6 +203,8 @@ struct hh_engine {
     double moe_mmg_min = 0;
     size_t mmf_min = 0;         // HAYAI_HIP_MMF_MIN: all-Q4_K batches from which tokens are f16 (0: by the weights)
     size_t mmi_min = 17;        // HAYAI_HIP_MMI_MIN: fewest tokens per pass on the int8 kernels (>= 2)
+    // HAYAI_HIP_ATTN_SHARE_MIN: bytes of reading that a decode batch's shared tokens have to save to be taken apart
+    size_t attn_share_min = (size_t)24 << 20;
     int mmi_d = 0;              // HAYAI_HIP_MMI_D: ring depth of the int8 f16-MFMA kernels (0: chosen)
     int blocks_per_cu_override = 0;  // HAYAI_HIP_BLOCKS_PER_CU
     bool q4k_generic = false;        // HAYAI_HIP_Q4K_GENERIC=1: skip the int8-digit Q4_K kernels

@@ -1,11 +1,13 @@
 """GPU tests of a decode batch's attention over pages (attn_decode), with and without shared tokens, against
 its definition in 64 bits; the bounds' derivation stands in attn_reference.py."""
+import os
+
 import numpy as np
 import pytest
 import torch
 
 from attn_reference import DT, attend, check, gather, page_elements
-from hayai_amd import BF16, F16, F32, HipError
+from hayai_amd import BF16, F16, F32, HipEngine, HipError
 from test_gpu_attn_pages import get, ints, normal, put
 
 pytestmark = pytest.mark.gpu
@@ -108,17 +110,40 @@ SHARED = [([300, 290, 257], 256, 8, 2, 128, 64), ([1000, 700, 699], 699, 4, 4, 6
           ([1300, 1290, 1290], 1281, 64, 1, 64, 64)]
 
 
+@pytest.fixture(scope="module")
+def sharing():
+    """An engine that takes shared tokens apart however few they are."""
+    os.environ["HAYAI_HIP_ATTN_SHARE_MIN"] = "0"
+    try:
+        e = HipEngine(0)
+    finally:
+        del os.environ["HAYAI_HIP_ATTN_SHARE_MIN"]
+    yield e
+    e.close()
+
+
 @pytest.mark.parametrize("ty,cty", TYPES)
-def test_shared(engine, ty, cty):
+def test_shared(engine, sharing, ty, cty):
     for i, (lens, prefix, heads, kvh, dim, page) in enumerate(SHARED):
         print(f"[case] decode {ty} {cty} {SHARED[i]}", flush=True)
         b = Batch(ty, cty, lens, prefix, heads, kvh, dim, page, seed=i, pad=i % 2)
+        b.check(b.run(sharing))
         b.check(b.run(engine))
+
+
+@pytest.mark.parametrize("ty,cty", TYPES)
+def test_shared_by_many(engine, ty, cty):
+    """As many bytes as are taken apart by default."""
+    lens = [700 + 3 * i for i in range(70)]
+    lens[5], lens[20], lens[69] = 0, 100, 690
+    b = Batch(ty, cty, lens, 690, 8, 4, 128, 64, seed=40)
+    assert 69 * 690 * 8 * 128 * torch.empty(0, dtype=DT[cty]).element_size() >= 24 << 20
+    b.check(b.run(engine))
 
 
 @pytest.mark.parametrize("ty", [F32, F16, BF16])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_slots_past_the_length(engine, ty, bad):
+def test_slots_past_the_length(sharing, ty, bad):
     for lens, prefix, page in [([50, 130, 1], 0, 16), ([400, 300, 20, 265], 265, 64)]:
         b = Batch(ty, ty, lens, prefix, 4, 2, 128, page, seed=3)
         want, bound = b.want()
@@ -132,37 +157,37 @@ def test_slots_past_the_length(engine, ty, bad):
             if n % page and b.tables[s, n // page] not in b.shared and lens[s] >= prefix:
                 b.cache[b.tables[s, n // page], :per // 2].view(2, page, 128)[:, n % page:] = bad
                 b.cache[b.tables[s, n // page], per // 2:].view(2, 128, page)[:, :, n % page:] = bad
-        got = b.run(engine).reshape(want.shape)
+        got = b.run(sharing).reshape(want.shape)
         keep = [s for s, n in enumerate(lens) if n >= prefix]  # (the others lie in any page)
         check(got[keep], want[keep], bound[keep], ty)
 
 
-def test_entries_outside_the_cache_are_zeros(engine):
+def test_entries_outside_the_cache_are_zeros(sharing):
     b = Batch(BF16, BF16, [400, 300, 380], 256, 8, 2, 128, 32, seed=4)
     b.shared[3] = -1
     b.tables[:, 3] = -9
     b.tables[0, 10], b.tables[2, 9] = b.n_pages, -2**31
-    b.check(b.run(engine))
+    b.check(b.run(sharing))
     b = Batch(F32, F32, [40, 300], 0, 4, 2, 72, 16, seed=5)
     b.tables[0, 1], b.tables[1, 0] = -1, b.n_pages
-    b.check(b.run(engine))
+    b.check(b.run(sharing))
 
 
-def test_lengths_past_the_table(engine):
+def test_lengths_past_the_table(sharing):
     for prefix in (0, 256):
         b = Batch(F16, F16, [320, 320], prefix, 4, 2, 64, 16, seed=6)
         b.lens[0] = 2**31 - 1  # as 320
-        b.check(b.run(engine))
+        b.check(b.run(sharing))
         b.width, b.tables = 0, np.zeros((2, 0), np.int32)
-        assert torch.all(b.run(engine) == 0)
+        assert torch.all(b.run(sharing) == 0)
 
 
-def test_more_sequences_than_threads(engine):
+def test_more_sequences_than_threads(sharing):
     rng = np.random.default_rng(7)
     for prefix in (0, 320):
         lens = [int(n) if i % 5 else int(n) // 60 for i, n in enumerate(prefix + rng.integers(0, 90, 600))]
         b = Batch(F32, F32, lens, prefix, 2, 1, 64, 16, seed=7)
-        b.check(b.run(engine))
+        b.check(b.run(sharing))
 
 
 def test_one_long_among_short(engine):
@@ -170,7 +195,7 @@ def test_one_long_among_short(engine):
     b.check(b.run(engine))
 
 
-def test_large_scores(engine):
+def test_large_scores(sharing):
     for ty in (F32, F16, BF16):
         b = Batch(ty, ty, [900, 650], 600, 2, 1, 64, 16, seed=9, scale=1.0)
         keys = b.cache[:, :16 * 64].view(-1, 16, 64)
@@ -179,16 +204,16 @@ def test_large_scores(engine):
         for s in range(2):  # the copies of the page that the prefix ends in, if any, hold the same
             assert 600 % 16 == 8
             keys[b.tables[s, 37], :8] = keys[b.shared[37], :8]
-        b.check(b.run(engine))
+        b.check(b.run(sharing))
 
 
-def test_prefix_is_as_good_as_none(engine):
+def test_prefix_is_as_good_as_none(sharing):
     """The same batch with and without the hint: equal up to the order of sums and one rounding."""
     b = Batch(F16, F16, [2100, 2055, 2060, 2200], 2050, 8, 2, 128, 64, seed=10)
-    with_prefix = b.run(engine)
+    with_prefix = b.run(sharing)
     b.check(with_prefix)
     b.prefix = 0
-    b.check(b.run(engine))
+    b.check(b.run(sharing))
 
 
 def test_far_pages(engine):
@@ -210,9 +235,11 @@ def test_far_pages(engine):
     cache.free()
 
 
-def test_captured(engine):
+@pytest.mark.parametrize("apart", [True, False])
+def test_captured(engine, sharing, apart):
     """A captured step follows the lengths, pages and queries of each replay; another graph and eager calls use the same
     workspace between the replays."""
+    engine = sharing if apart else engine
     b = Batch(BF16, BF16, [700, 330, 400], 320, 8, 2, 128, 32, seed=13, width=40)
     c = Batch(F32, F32, [1000, 90], 0, 4, 2, 64, 16, seed=14)
     graphs = []
@@ -240,11 +267,11 @@ def test_captured(engine):
         g.free()
 
 
-def test_same_bits_every_time(engine):
+def test_same_bits_every_time(sharing):
     b = Batch(F16, F16, [900, 800, 770], 700, 8, 2, 128, 64, seed=16)
-    first = b.run(engine)
+    first = b.run(sharing)
     for _ in range(3):
-        assert torch.equal(first, b.run(engine))
+        assert torch.equal(first, b.run(sharing))
 
 
 def test_no_sequences(engine):

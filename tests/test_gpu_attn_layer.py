@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from attn_reference import attend, check, gather, half_step, page_elements
-from hayai_amd import BF16, F32
+from hayai_amd import BF16, F32, HipEngine
 from test_gpu_attn_pages import get, ints, near, normal, put, turned
 from test_gpu_i8 import codes_of
 
@@ -108,8 +108,12 @@ class Layer:
         near(get(b["y"], self.dt, (rows, D_MODEL)), want, self.dt, slack)
 
 
-@pytest.mark.parametrize("ty,cty", [(BF16, BF16), (F32, F32), (F32, BF16)])
-def test_layer(engine, ty, cty):
+@pytest.mark.parametrize("ty,cty,apart", [(BF16, BF16, True), (BF16, BF16, False), (F32, F32, True), (F32, BF16, False)])
+def test_layer(engine, ty, cty, apart, monkeypatch):
+    """apart: the decode steps' shared tokens, few as they are, by the kernel for many."""
+    if apart:
+        monkeypatch.setenv("HAYAI_HIP_ATTN_SHARE_MIN", "0")
+        engine = HipEngine(0)
     lengths = [301, 40, 7]
     layer = Layer(engine, ty, cty, 40, sum(lengths))
     pages = list(np.random.default_rng(1).permutation(40))
@@ -159,3 +163,5 @@ def test_layer(engine, ty, cty):
             graph.launch()
         layer.check(x, [at] * 5, slots, [(1, c, at + 1) for c in children])
     graph.free()
+    if apart:
+        engine.close()
