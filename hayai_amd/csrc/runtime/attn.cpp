@@ -41,9 +41,10 @@ using namespace hh;
 hh_status hh_engine::enqueue_rope(int type, int kv_type, int layout, size_t tokens, const hh_rope_args& a) {
     hipFunction_t f;
     const size_t el = act_type(type)->bytes, cus = (size_t)props.multiProcessorCount;
-    // Eight tokens a workgroup of 1024 threads from four workgroups every CU on, else one a workgroup of 256, and of few
-    // tokens each is given to several.
-    const size_t each = tokens >= 8 * cus ? 8 : 1;
+    // Eight tokens a workgroup of 1024 threads from three tokens a CU on (32/8 heads of 128 bf16, us, eight and one: 512 tokens
+    // 9.1, 8.4; 1024 tokens 10.1, 12.6; 4096 tokens 30, 51), else one a workgroup of 256, and of few tokens each is given to
+    // several.
+    const size_t each = tokens >= 3 * cus ? 8 : 1;
     HH_TRY(kernel(std::string("hh_rope_") + (layout == HH_ROPE_PAIRS ? "pairs" : "halves") + (each == 8 ? "8_" : "_") +
                       attn_types(type, kv_type), &f));
     const size_t pieces = (a.heads + 2 * (size_t)a.kv.heads) * ((a.kv.dim * el + 15) / 16);
