@@ -76,6 +76,7 @@ HH_DEV void hh_attn_single(const hh_attn_decode_args& p, uint32_t block) {
     typedef typename C::E CE;
     typedef hh_mat<C> M;
     typedef typename M::frag F;
+    constexpr float LIFT = hh_attn_lift<C>();
     constexpr int EF = C::VEC, SZ = sizeof(CE), STEP = 4 * EF, KT = STEP / 16, NC = DP / (4 * EF), DT = DP / 16;
     const hh_attn_args& a = p.a;
     const uint32_t lane = threadIdx.x % HH_WAVE, ln = lane % 16, g = lane / 16;
@@ -169,10 +170,10 @@ HH_DEV void hh_attn_single(const hh_attn_decode_args& p, uint32_t block) {
 #pragma unroll
         for (int x = 1; x < EF; x++) top = fmaxf(top, s[x]);
         top *= a.c;
-        if (__any(top > base + HH_ATTN_SLACK)) {
+        if (__any(top > base + (HH_ATTN_SLACK + LIFT))) {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float next = top > base + HH_ATTN_SLACK ? top : base, f = hh_exp2(base - next);
+            const float next = top > base + (HH_ATTN_SLACK + LIFT) ? top - LIFT : base, f = hh_exp2(base - next);
             base = next;
             sum *= f;
 #pragma unroll

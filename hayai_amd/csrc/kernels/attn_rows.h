@@ -28,9 +28,11 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
     typedef hh_mat<C> M;
     typedef typename M::frag F;
     constexpr int EF = C::VEC, SZ = sizeof(CE), BN = 128 / SZ, NT = BN / 32, NC = DP / (2 * EF), DT = DP / 32;
+    constexpr float LIFT = hh_attn_lift<C>();
     constexpr int NG = BN / 16;  // a page's end may lie after any 16 keys
     constexpr int KB = DP * SZ, VB = BN * SZ, KBYTES = BN * KB, BYTES = KBYTES + DP * VB;
     constexpr int KP = KBYTES / 1024 / 4, VP = DP * VB / 1024 / 4;  // 1 KB pieces a wave copies
+    static_assert(VP % 2 == 0, "a wave's pieces of V begin at an even one");
     const uint32_t lane = threadIdx.x % HH_WAVE, ln = lane % 32, hf = lane / 32;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / HH_WAVE);
     const uint32_t dim = FULL ? DP : a.kv.dim, group = a.group, shift = a.kv.shift;
@@ -98,11 +100,11 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
         if (FULL && __builtin_expect(__all(in[0] && in[1]), 1)) {
 #pragma unroll
             for (int i = 0; i < VP; i++)
-                hh_copy16(from[(VP * 4 > 4 ? i : p0v + i) & 1] + (first + ((p0v + i) * 8 << shift) * SZ), buf + (p0v + i) * 1024);
+                hh_copy16(from[i & 1] + (first + ((p0v + i) * 8 << shift) * SZ), buf + (p0v + i) * 1024);
         } else {
 #pragma unroll
             for (int i = 0; i < VP; i++) {
-                const uint32_t o = (p0v + i) & 1, d = (p0v + i) * 8;  // (rows past dim: the last one's place)
+                const uint32_t o = i & 1, d = (p0v + i) * 8;  // (rows past dim: the last one's place)
                 const uint8_t* src = (o ? from[1] : from[0]) + (first + ((min(d + vrow, dim - 1) - vrow) << shift) * SZ);
                 hh_copy16((o ? in[1] : in[0]) ? src : zeros, buf + (p0v + i) * 1024);
             }
@@ -149,9 +151,9 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
 #pragma unroll
         for (int x = 1; x < NT * 16; x++) top = fmaxf(top, s[x]);
         top *= a.c;
-        if (__any(top > base + HH_ATTN_SLACK)) {
+        if (__any(top > base + (HH_ATTN_SLACK + LIFT))) {
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float next = top > base + HH_ATTN_SLACK ? top : base, f = hh_exp2(base - next);
+            const float next = top > base + (HH_ATTN_SLACK + LIFT) ? top - LIFT : base, f = hh_exp2(base - next);
             base = next;
             sum *= f;
 #pragma unroll
@@ -266,7 +268,10 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
                 if (FULL || d < dim) hh_store_n(out + d, w);
             }
         }
-    if (odd) left_out([&](uint32_t d, float v) { out[d] = A::put(A::get(out[d]) + v); });
+    if (odd) {
+        __threadfence();  // (some of these elements were stored by the row's other half)
+        left_out([&](uint32_t d, float v) { out[d] = A::put(A::get(out[d]) + v); });
+    }
 }
 
 // Two runs of a row's parts, joined: sum_i f_i o_i / sum_i f_i s_i, f_i = exp2(base_i - max base), by `teams` (a power of

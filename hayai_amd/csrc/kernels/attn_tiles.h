@@ -92,10 +92,15 @@ HH_DEV typename hh_mat<C>::frag hh_finite(typename hh_mat<C>::frag f, uint32_t& 
 
 // Scores are in units of log2: weight = exp2(score * c - base), c = scale * log2(e).  base follows the
 // largest score, but only once it falls more than HH_ATTN_SLACK behind: weights of up to 2^8 are as good as
-// those of up to 1 in f32, f16 and bf16, and sums need no rescaling meanwhile.  It starts at the lowest f32,
-// where exp2(-inf - base) is 0 as well.
+// those of up to 1, and sums need no rescaling meanwhile.  In f16 it stays 2^7 below, so that weights are up to 2^15 and
+// what is lost under f16's smallest number is 2^-32 of the largest: at 2^-25 of it the many small weights of a long context
+// would be lost together.  It starts at the lowest f32, where exp2(-inf - base) is 0 as well.
 #define HH_ATTN_SLACK 8.f
 #define HH_ATTN_LOWEST (-3.402823466e38f)
+template <class C>
+HH_DEV constexpr float hh_attn_lift() {
+    return __is_same(C, hh_af16) ? 7.f : 0.f;
+}
 HH_DEV float hh_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A 16-byte source for what a page number outside the cache stands for: zeros.

@@ -207,6 +207,27 @@ def test_large_scores(sharing):
         b.check(b.run(sharing))
 
 
+def far_smaller(b, likely, rest):
+    """One token with a weight of 1 and a value of 0, the others with a weight of exp(-rest) and values of 1."""
+    b.q[:] = 0
+    b.q[:, ::b.dim] = 8.0
+    per = b.cache.shape[1] // 2
+    b.cache[:, :per], b.cache[:, per:] = 0, 1.0
+    page, at = divmod(likely, b.page)
+    for table in b.tables:
+        b.cache[table[page], :per].view(b.kvh, b.page, b.dim)[:, at, 0] = rest / b.scale / 8
+        b.cache[table[page], per:].view(b.kvh, b.dim, b.page)[:, :, at] = 0
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("prefix,likely", [(0, 3), (0, 30000), (29952, 7), (29952, 29990)])
+def test_many_small_weights(sharing, ty, prefix, likely):
+    """30000 tokens of e^-17.5: 8e-4 together, each below f16's smallest number."""
+    b = Batch(ty, ty, [30001, 30005], prefix, 2, 1, 64, 64, seed=17)
+    far_smaller(b, likely, 17.5)
+    b.check(b.run(sharing))
+
+
 def test_prefix_is_as_good_as_none(sharing):
     """The same batch with and without the hint: equal up to the order of sums and one rounding."""
     b = Batch(F16, F16, [2100, 2055, 2060, 2200], 2050, 8, 2, 128, 64, seed=10)

@@ -166,6 +166,26 @@ def test_rope_prompt(engine, ty, cty, layout):
     assert torch.equal(new[:3], cache[:3])
 
 
+def test_rope_more_tokens_than_a_launch(engine):
+    t, dim, page = (1 << 20) + 11, 8, 256
+    n_pages = t // page + 1
+    x = torch.from_numpy(np.random.default_rng(30).standard_normal((t, 3 * dim), dtype=np.float32)).half()
+    xb, cb, out = put(engine, x), engine.alloc(n_pages * 2 * page * dim * 2), engine.alloc(t * dim * 2)
+    cb.fill(0)
+    order = np.arange(t, dtype=np.int32)
+    d = engine.rope_desc(F16, t, 1, dim, q_stride=3 * dim, k_stride=3 * dim, v_stride=3 * dim)
+    engine.rope_kv_dev(d, engine.kv_desc(F16, 1, dim, page, n_pages), xb, 0, xb, 2 * dim, xb, 4 * dim, engine.upload(order % 1000), 0,
+                       engine.upload(order), 0, None, 0, out, 0, cb, 0)
+    at = np.r_[0:50, (1 << 20) - 20:t]
+    x64 = x[at].double().reshape(len(at), 3, dim)
+    want = turned(x64[:, :2], at % 1000, dim, 10000.0, ROPE_HALVES, None, 1.0)
+    size = (x64[:, :2] ** 2).sum(-1, keepdim=True).sqrt().expand_as(want) * 6 * 2.0**-24
+    near(get(out, torch.float16, (t, 1, dim))[at], want[:, :1], torch.float16, size[:, :1])
+    cache = get(cb, torch.float16, (n_pages, 2, page * dim))
+    near(cache[:, 0].reshape(-1, dim)[at], want[:, 1], torch.float16, size[:, 1])
+    assert torch.equal(cache[:, 1].reshape(n_pages, dim, page).permute(0, 2, 1).reshape(-1, dim)[:t], x[:, 2 * dim:])
+
+
 def test_rope_in_place(engine):
     heads, kvh, dim, page = 12, 2, 128, 16
     for layout, t in ((ROPE_HALVES, 130), (ROPE_PAIRS, 130), (ROPE_HALVES, 2500), (ROPE_PAIRS, 2500)):

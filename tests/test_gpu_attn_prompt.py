@@ -6,6 +6,7 @@ import torch
 
 from attn_reference import DT, attend, check, gather, page_elements
 from hayai_amd import BF16, F16, F32, HipError
+from test_gpu_attn_decode import far_smaller
 from test_gpu_attn_pages import get, ints, normal, put
 
 pytestmark = pytest.mark.gpu
@@ -217,6 +218,15 @@ def test_large_scores(engine):
         for t in range(900):
             keys[p.tables[0, t // 16], t % 16] *= 0.2 + t / 150
         p.check(engine)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("likely", [3, 29990])
+def test_many_small_weights(engine, ty, likely):
+    """30000 tokens of e^-17.5: 8e-4 together, each below f16's smallest number."""
+    p = Problem(ty, ty, [(5, 30001)], 2, 1, 64, 64, seed=17)
+    far_smaller(p, likely, 17.5)
+    p.check(engine)
 
 
 def test_far_pages(engine):
