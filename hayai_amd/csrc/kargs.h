@@ -186,6 +186,7 @@ struct hh_attn_prompt_args {
     hh_attn_args a;
     const int32_t* starts;  // seqs + 1
     uint32_t tokens, slots;
+    uint32_t turn;  // tiles' parts from which on the shortest come first
 };
 
 // Attention of one token a sequence (attn_decode.hip): the first `prefix` tokens of all sequences from the

@@ -70,14 +70,15 @@ HH_DEV bool hh_attn_plan(const hh_attn_decode_args& p, uint32_t piece, bool firs
     return out.count != 0;
 }
 
-template <class A, class C, int DP, bool FULL>
+template <class A, class C, int DP, int DU>
 HH_DEV void hh_attn_single(const hh_attn_decode_args& p, uint32_t block) {
     typedef typename A::E E;
     typedef typename C::E CE;
     typedef hh_mat<C> M;
     typedef typename M::frag F;
     constexpr float LIFT = hh_attn_lift<C>();
-    constexpr int EF = C::VEC, SZ = sizeof(CE), STEP = 4 * EF, KT = STEP / 16, NC = DP / (4 * EF), DT = DP / 16;
+    constexpr int EF = C::VEC, SZ = sizeof(CE), STEP = 4 * EF, KT = STEP / 16, D = DU ? DU : DP, NC = D / (4 * EF), DT = D / 16;
+    constexpr bool FULL = DU == 0;
     const hh_attn_args& a = p.a;
     const uint32_t lane = threadIdx.x % HH_WAVE, ln = lane % 16, g = lane / 16;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / HH_WAVE);
@@ -202,9 +203,10 @@ HH_DEV void hh_attn_single(const hh_attn_decode_args& p, uint32_t block) {
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
 
-    // the waves' sums, joined: 4-element chunk c of row r lies at chunk c ^ r
+    // the waves' sums, joined: 4-element chunk c of row r lies at chunk c ^ r % 8
     __shared__ float bases[4][16], weights[4][16];
-    float* const red = (float*)hh_attn_lds<0, 256 * DP>();
+    hh_f32x4* const red = (hh_f32x4*)hh_attn_lds<0, hh_attn_bytes<C, DP, DU>()>();
+    static_assert(64 * D * 4 <= hh_attn_bytes<C, DP, DU>(), "the sums fit the tile's buffer");
     if (lane < 16) {
         bases[wave][lane] = base;
         weights[wave][lane] = sum;
@@ -213,12 +215,12 @@ HH_DEV void hh_attn_single(const hh_attn_decode_args& p, uint32_t block) {
     const float top = fmaxf(fmaxf(bases[0][ln], bases[1][ln]), fmaxf(bases[2][ln], bases[3][ln])), f = hh_exp2(base - top);
 #pragma unroll
     for (int i = 0; i < DT; i++)
-        *(hh_f32x4*)(red + ((wave * 16 + ln) * (DP / 4) + ((i * 4 + g) ^ ln)) * 4) = o[i] * f;
+        red[(wave * 16 + ln) * (D / 4) + ((i * 4 + g) ^ ln % 8)] = o[i] * f;
     __syncthreads();
     const size_t rows = ((size_t)number * p.row_tiles + rt) * a.kv.heads + kvh;
 #pragma unroll
-    for (uint32_t at = threadIdx.x; at < 4 * DP; at += 256) {
-        const uint32_t r = at / (DP / 4), d = at % (DP / 4) * 4;
+    for (uint32_t at = threadIdx.x; at < 4 * D; at += 256) {
+        const uint32_t r = at / (D / 4), c = at % (D / 4), d = c * 4;
         if (rt * 16 + r >= a.group || d >= dim) continue;
         const float t = fmaxf(fmaxf(bases[0][r], bases[1][r]), fmaxf(bases[2][r], bases[3][r]));
         float total = 0;
@@ -226,7 +228,7 @@ HH_DEV void hh_attn_single(const hh_attn_decode_args& p, uint32_t block) {
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             total = fmaf(weights[w][r], hh_exp2(bases[w][r] - t), total);
-            v += *(const hh_f32x4*)(red + ((w * 16 + r) * (DP / 4) + (at % (DP / 4) ^ r)) * 4);
+            v += red[(w * 16 + r) * (D / 4) + (c ^ r % 8)];
         }
         if (alone) {
             const float by = total == 0 ? 0.f : 1.f / total;
@@ -245,16 +247,16 @@ HH_DEV void hh_attn_single(const hh_attn_decode_args& p, uint32_t block) {
 }
 
 // The shared tokens' tiles first, then the sequences' own pieces.
-template <class A, class C, int DP, bool FULL>
+template <class A, class C, int DP, int DU>
 HH_DEV void hh_attn_shared(const hh_attn_decode_args& p) {
     const hh_attn_args& a = p.a;
     const uint32_t ahead = p.tiles * a.kv.heads * a.splits;
     if (blockIdx.x >= ahead) {
-        hh_attn_single<A, C, DP, FULL>(p, blockIdx.x - ahead);
+        hh_attn_single<A, C, DP, DU>(p, blockIdx.x - ahead);
         return;
     }
     const uint32_t kvh = blockIdx.x % a.kv.heads, tile = blockIdx.x / a.kv.heads % p.tiles, split = blockIdx.x / a.kv.heads / p.tiles;
-    hh_attn_rows<A, C, DP, FULL, false>(a, hh_attn_tile{0, 0, tile * a.tile_tokens, a.seqs, p.prefix}, p.shared,
+    hh_attn_rows<A, C, DP, DU, false>(a, hh_attn_tile{0, 0, tile * a.tile_tokens, a.seqs, p.prefix}, p.shared,
                                         p.shared_entries, kvh, tile * a.kv.heads + kvh, split, a.splits);
 }
 
@@ -277,20 +279,14 @@ HH_DEV void hh_attn_join(const hh_attn_decode_args& p) {
                             (typename A::E*)a.out + (size_t)s * a.out_stride + head * a.kv.dim);
 }
 
-#define HH_ATTN_DECODE(N, A, C, D)                                                                                                  \
-    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_decode_##D##_##N(const hh_attn_decode_args p) { \
-        hh_attn_single<A, C, D, true>(p, blockIdx.x);                                                                               \
-    }                                                                                                                               \
-    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_decode_##D##_any_##N(const hh_attn_decode_args p) { \
-        hh_attn_single<A, C, D, false>(p, blockIdx.x);                                                                              \
-    }                                                                                                                               \
-    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_shared_##D##_##N(const hh_attn_decode_args p) { \
-        hh_attn_shared<A, C, D, true>(p);                                                                                           \
-    }                                                                                                                               \
-    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_shared_##D##_any_##N(const hh_attn_decode_args p) { \
-        hh_attn_shared<A, C, D, false>(p);                                                                                          \
+#define HH_ATTN_DECODE(N, A, C, D, DU, NAME)                                                                                    \
+    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, (DU) ? (DU) : (D))) hh_attn_decode_##NAME##_##N(const hh_attn_decode_args p) { \
+        hh_attn_single<A, C, D, DU>(p, blockIdx.x);                                                                             \
+    }                                                                                                                           \
+    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, (DU) ? (DU) : (D))) hh_attn_shared_##NAME##_##N(const hh_attn_decode_args p) { \
+        hh_attn_shared<A, C, D, DU>(p);                                                                                         \
     }
-#define HH_ATTN_DECODES(N, A, C) HH_ATTN_DECODE(N, A, C, 64) HH_ATTN_DECODE(N, A, C, 128) HH_ATTN_DECODE(N, A, C, 256)
+#define HH_ATTN_DECODES(N, A, C) HH_ATTN_DIMS(HH_ATTN_DECODE, N, A, C)
 HH_ATTN_DECODES(f32, hh_af32, hh_af32)
 HH_ATTN_DECODES(f16, hh_af16, hh_af16)
 HH_ATTN_DECODES(bf16, hh_abf16, hh_abf16)

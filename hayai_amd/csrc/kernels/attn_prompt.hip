@@ -76,26 +76,34 @@ HH_DEV bool hh_attn_find(const hh_attn_prompt_args& p, uint32_t slot, uint32_t l
     return true;
 }
 
-HH_DEV uint32_t hh_attn_slot(const hh_attn_prompt_args& p) {
-    const uint32_t i = blockIdx.x / p.a.kv.heads;
-    return p.a.seqs > 1 && p.a.seqs <= HH_WAVE ? i : p.slots - 1 - i;
+// The workgroup's tile and part: a tile's parts and kv heads next to each other (kv heads go round the XCDs), the tiles with the
+// most keys first.  From p.turn on the least come first, where the chip holds all: the second workgroup of a CU that has one of
+// the longest is one of the shortest (us, so and all in descending order: 1000 tokens, 32/8 heads of 80 f32: 79.0, 96.7; 1500
+// tokens, 32/8 heads of 128 bf16: 43.4, 45.4).
+struct hh_attn_place {
+    uint32_t kvh, slot, split;
+};
+HH_DEV hh_attn_place hh_attn_place_of(const hh_attn_prompt_args& p, uint32_t block, uint32_t blocks) {
+    uint32_t i = block / p.a.kv.heads;
+    if (i >= p.turn) i = blocks / p.a.kv.heads - 1 - (i - p.turn);
+    const uint32_t tile = i / p.a.splits;
+    return {block % p.a.kv.heads, p.a.seqs > 1 && p.a.seqs <= HH_WAVE ? tile : p.slots - 1 - tile, i % p.a.splits};
 }
 
-template <class A, class C, int DP, bool FULL>
+template <class A, class C, int DP, int DU>
 HH_DEV void hh_attn_prompt(const hh_attn_prompt_args& p) {
-    // kv heads go round the XCDs
-    const uint32_t kvh = blockIdx.x % p.a.kv.heads, slot = hh_attn_slot(p);
+    const hh_attn_place at = hh_attn_place_of(p, blockIdx.x, gridDim.x);
     hh_attn_tile tile;
-    if (!hh_attn_find(p, slot, threadIdx.x % HH_WAVE, tile)) return;
-    hh_attn_rows<A, C, DP, FULL, true>(p.a, tile, p.a.tables + (size_t)tile.seq * p.a.entries, p.a.entries, kvh,
-                                       slot * p.a.kv.heads + kvh, blockIdx.y, gridDim.y);
+    if (!hh_attn_find(p, at.slot, threadIdx.x % HH_WAVE, tile)) return;
+    hh_attn_rows<A, C, DP, DU, true>(p.a, tile, p.a.tables + (size_t)tile.seq * p.a.entries, p.a.entries, at.kvh,
+                                     at.slot * p.a.kv.heads + at.kvh, at.split, p.a.splits);
 }
 
 // The parts of rows whose keys were split, joined.
 template <class A, int DP>
 HH_DEV void hh_attn_prompt_join(const hh_attn_prompt_args& p) {
     const hh_attn_args& a = p.a;
-    const uint32_t kvh = blockIdx.x % a.kv.heads, slot = hh_attn_slot(p);
+    const uint32_t kvh = blockIdx.x % a.kv.heads, slot = blockIdx.x / a.kv.heads;
     hh_attn_tile tile;
     if (!hh_attn_find(p, slot, threadIdx.x % HH_WAVE, tile)) return;
     const uint32_t rows = min(a.tile_tokens, tile.tokens - tile.first) * a.group;
@@ -111,14 +119,11 @@ HH_DEV void hh_attn_prompt_join(const hh_attn_prompt_args& p) {
     hh_attn_join_row<A, DP>(parts, hh_attn_parts{}, teams, r < rows && threadIdx.x % (DP / 4) * 4 < a.kv.dim, out);
 }
 
-#define HH_ATTN_PROMPT(N, A, C, D)                                                                                            \
-    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_prompt_##D##_##N(const hh_attn_prompt_args a) { \
-        hh_attn_prompt<A, C, D, true>(a);                                                                                     \
-    }                                                                                                                         \
-    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, D)) hh_attn_prompt_##D##_any_##N(const hh_attn_prompt_args a) { \
-        hh_attn_prompt<A, C, D, false>(a);                                                                                    \
+#define HH_ATTN_PROMPT(N, A, C, D, DU, NAME)                                                                                    \
+    extern "C" __global__ void __launch_bounds__(256, HH_ATTN_PER_CU(C, (DU) ? (DU) : (D))) hh_attn_prompt_##NAME##_##N(const hh_attn_prompt_args a) { \
+        hh_attn_prompt<A, C, D, DU>(a);                                                                                         \
     }
-#define HH_ATTN_PROMPTS(N, A, C) HH_ATTN_PROMPT(N, A, C, 64) HH_ATTN_PROMPT(N, A, C, 128) HH_ATTN_PROMPT(N, A, C, 256)
+#define HH_ATTN_PROMPTS(N, A, C) HH_ATTN_DIMS(HH_ATTN_PROMPT, N, A, C)
 HH_ATTN_PROMPTS(f32, hh_af32, hh_af32)
 HH_ATTN_PROMPTS(f16, hh_af16, hh_af16)
 HH_ATTN_PROMPTS(bf16, hh_abf16, hh_abf16)

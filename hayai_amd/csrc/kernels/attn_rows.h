@@ -18,21 +18,29 @@ struct hh_attn_tile {
     uint32_t seq, start, first, tokens, len;
 };
 
-// CAUSAL: each earlier token sees a key less; else all of them see len, and the sums always go to `part`.  at: the tile's
+// Bytes of a tile of keys and values in LDS.
+template <class C, int DP, int DU>
+constexpr int hh_attn_bytes() {
+    return 128 * DP + 128 * (DU ? DU : DP);
+}
+
+// DP: a head's elements, or those that they lie within; DU: 0 where the head has all of them, else how many are computed
+// (a head of 72 to 96 takes three quarters of 128's products).  CAUSAL: each earlier token sees a key less; else all of them see len, and the sums always go to `part`.  at: the tile's
 // number in `part`; split: which of its `splits` parts of keys.
-template <class A, class C, int DP, bool FULL, bool CAUSAL>
+template <class A, class C, int DP, int DU, bool CAUSAL>
 HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const int32_t* table, uint32_t entries, uint32_t kvh,
                          uint32_t at, uint32_t split, uint32_t splits) {
     typedef typename A::E E;
     typedef typename C::E CE;
     typedef hh_mat<C> M;
     typedef typename M::frag F;
-    constexpr int EF = C::VEC, SZ = sizeof(CE), BN = 128 / SZ, NT = BN / 32, NC = DP / (2 * EF), DT = DP / 32;
+    constexpr int EF = C::VEC, SZ = sizeof(CE), BN = 128 / SZ, NT = BN / 32, D = DU ? DU : DP, NC = D / (2 * EF), DT = D / 32;
+    constexpr bool FULL = DU == 0;
     constexpr float LIFT = hh_attn_lift<C>();
     constexpr int NG = BN / 16;  // a page's end may lie after any 16 keys
-    constexpr int KB = DP * SZ, VB = BN * SZ, KBYTES = BN * KB, BYTES = KBYTES + DP * VB;
-    constexpr int KP = KBYTES / 1024 / 4, VP = DP * VB / 1024 / 4;  // 1 KB pieces a wave copies
-    static_assert(VP % 2 == 0, "a wave's pieces of V begin at an even one");
+    constexpr int KB = DP * SZ, VB = BN * SZ, KBYTES = BN * KB, BYTES = hh_attn_bytes<C, DP, DU>();
+    constexpr int KP = KBYTES / 1024 / 4, VP = D * VB / 1024 / 4;  // 1 KB pieces a wave copies
+    static_assert(BYTES == KBYTES + D * VB && (!FULL || VP % 2 == 0), "a whole head's waves begin at even pieces of V");
     const uint32_t lane = threadIdx.x % HH_WAVE, ln = lane % 32, hf = lane / 32;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / HH_WAVE);
     const uint32_t dim = FULL ? DP : a.kv.dim, group = a.group, shift = a.kv.shift;
@@ -104,7 +112,7 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
         } else {
 #pragma unroll
             for (int i = 0; i < VP; i++) {
-                const uint32_t o = i & 1, d = (p0v + i) * 8;  // (rows past dim: the last one's place)
+                const uint32_t o = (p0v + i) & 1, d = (p0v + i) * 8;  // (rows past dim: the last one's place)
                 const uint8_t* src = (o ? from[1] : from[0]) + (first + ((min(d + vrow, dim - 1) - vrow) << shift) * SZ);
                 hh_copy16((o ? in[1] : in[0]) ? src : zeros, buf + (p0v + i) * 1024);
             }
@@ -124,7 +132,7 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
         uint8_t* const vbuf = buf + KBYTES;
         const bool crossed = k0 + BN > least;
         if (crossed) {  // values past the sequence's end and those that are no finite numbers as zeros
-            for (uint32_t i = threadIdx.x; i < DP * 8; i += 256) {
+            for (uint32_t i = threadIdx.x; i < D * 8; i += 256) {
                 F* const at = (F*)(vbuf + i / 8 * VB + (i % 8 ^ hh_attn_swizzle<128>(i / 8)) * 16);
                 *at = hh_finite<C>(hh_first<C>(*at, (int)tile.len - (int)(k0 + i % 8 * EF)), odd);
             }

@@ -129,6 +129,11 @@ struct hh_max32 {
 HH_DEV uint32_t hh_wave_sum32(uint32_t v) { return hh_wave32<hh_add32>(v); }
 HH_DEV uint32_t hh_wave_max32(uint32_t v) { return hh_wave32<hh_max32>(v); }
 
+// A kernel for each width of heads: whole 64, 128 and 256 elements, and those within 64, 96, 128 and 256.
+#define HH_ATTN_DIMS(KERNEL, N, A, C)                                                                          \
+    KERNEL(N, A, C, 64, 0, 64) KERNEL(N, A, C, 64, 64, 64_any) KERNEL(N, A, C, 128, 96, 96_any) KERNEL(N, A, C, 128, 0, 128) \
+    KERNEL(N, A, C, 128, 128, 128_any) KERNEL(N, A, C, 256, 0, 256) KERNEL(N, A, C, 256, 256, 256_any)
+
 constexpr int hh_attn_wait(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | 0x70 | (lgkm << 8); }
 // This wave's copies into LDS landed and its LDS reads done, then the workgroup meets.
 HH_DEV void hh_attn_meet() {

@@ -18,7 +18,7 @@ void attn_kernels(std::vector<std::string>& k) {
     for (auto& t : kAttnTypes) {
         const std::string ty = attn_types(t[0], t[1]);
         for (const char* v : {"halves_", "pairs_", "halves8_", "pairs8_"}) k.push_back(std::string("hh_rope_") + v + ty);
-        for (const char* v : {"64_", "64_any_", "128_", "128_any_", "256_", "256_any_"})
+        for (const char* v : {"64_", "64_any_", "96_any_", "128_", "128_any_", "256_", "256_any_"})
             for (const char* kind : {"hh_attn_prompt_", "hh_attn_decode_", "hh_attn_shared_"})
                 k.push_back(std::string(kind) + v + ty);
         for (const char* v : {"64_", "128_", "256_"})
@@ -87,38 +87,66 @@ hh_status hh_engine::enqueue_kv_copy(size_t layers, const hh_kv_copy_args& a) {
     return HH_OK;
 }
 
-// Kernels are made for heads of 64, 128 and 256 elements, whole or with the rest as zeros.
+// Kernels are made for heads of 64, 128 and 256 elements, whole or with the rest as zeros, and for those of up to 96 laid
+// out as 128 (us, computed as 96 and as 128: 3000 tokens, 32/8 heads of 80 bf16: 86.7, 96.5; 64 sequences of 2000: 74.3, 77.9).
 static size_t padded_dim(size_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 static std::string dim_name(size_t dim) {
+    if (dim > 64 && dim <= 96) return "96_any_";
     return std::to_string(padded_dim(dim)) + (dim == padded_dim(dim) ? "_" : "_any_");
+}
+
+// In how many parts the keys of a prompt's tiles are best taken, by an estimate in the time that a workgroup alone on its CU
+// takes for one key (of 128 elements in 16 bits: 22 ns).  A part has keys / splits.  Two on a CU take 1.5 times as long (f32,
+// bound by its products: twice) for the mean of the keys that tiles see, and no less than 1.25 times the longest.  Joining
+// costs a launch (160) and writing and reading the parts' sums (2.3 a row and CU); a key of f32 takes about six times as long.
+// Measured (us; 32/8 heads of 128 bf16, by splits, the one taken in brackets): 256 tokens behind 1000: 1: 34.9, 2: 28.3,
+// 3: 27.9, [4: 26.3], 6: 31.4; behind 16000: 2: 186, 4: 110, [8: 97]; 512 behind 1000: 1: 40.7, [2: 34.9], 3: 39.5, 4: 37.0;
+// 1024: [1: 30.0], 2: 36.2; behind 4000: 1: 115, [2: 104]; 1024 of 8/2 heads of 256: 1: 55.5, 2: 44.0, [4: 39.4], 6: 45.8;
+// 100 f32 behind 1000: 4: 54.4, [8: 41.2], 12: 51.1, 16: 54.0.
+static uint32_t prompt_splits(size_t tiles, size_t keys, size_t mean, size_t rows, size_t cus, size_t dp, bool f32) {
+    const float unit = f32 ? 1 / 6.0f : 1.0f, both = f32 ? 2.0f : 1.5f;
+    float least = 0;
+    uint32_t best = 1;
+    for (uint32_t s = 1; s == 1 || (s <= 64 && s * tiles <= 2 * cus && s * 16 <= keys); s++) {
+        const float per_cu = (float)(s * tiles) / (float)cus;
+        float cost = (float)keys / (float)s;
+        if (per_cu > 1) cost = std::max(1.25f * cost, both * (float)mean / (float)s);
+        if (s > 1) cost += unit * (160.0f * 128 / (float)dp + 2.3f * (float)(s * rows) / (float)cus);
+        if (s == 1 || cost < least) least = cost, best = s;
+    }
+    return best;
 }
 
 hh_status hh_engine::enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_args p) {
     hh_attn_args& a = p.a;
     hipFunction_t f, join;
     const size_t dp = padded_dim(a.kv.dim), cus = (size_t)props.multiProcessorCount;
-    HH_TRY(kernel("hh_attn_prompt_" + dim_name(a.kv.dim) + attn_types(type, kv_type), &f));
+    const std::string name = "hh_attn_prompt_" + dim_name(a.kv.dim) + attn_types(type, kv_type);
+    HH_TRY(kernel(name, &f));
     HH_TRY(kernel("hh_attn_prompt_join_" + std::to_string(dp) + "_" + act_type(type)->name, &join));
     a.tile_tokens = 128 / a.group;
-    const size_t slots = (size_t)p.tokens / a.tile_tokens + a.seqs, tiles = slots * a.kv.heads;
+    // as many tiles as the sequences can have: ranked by keys or, of more than a wave's lanes, each from its own slot on
+    const size_t slots = a.seqs <= 64 ? (p.tokens + (size_t)a.seqs * (a.tile_tokens - 1)) / a.tile_tokens
+                                      : (size_t)p.tokens / a.tile_tokens + a.seqs;
+    const size_t tiles = slots * a.kv.heads;
     if (tiles >= 1u << 24) return fail(HH_ERR_INVALID, "attn_prompt: %u tokens of %u sequences are too many", p.tokens, a.seqs);
     p.slots = (uint32_t)slots;
-    // Few tiles: their keys are split, for two workgroups a CU.  A part's sums cost 4 KB a head and token (its rows of them,
-    // written and read), so that it is the longer the more waves have rows: 128 keys each (3956 tokens of 8 sequences, 2 heads
-    // of 80 f16: parts of 512 34 us, of 220 40; 12 tokens behind 4704, 4/2 heads of 256: parts of 256 25 us, of 512 35), 16 of
-    // f32, whose products take eight times as long (512 tokens, 8/2 heads of 128: parts of 64 31 us, of 128 34, of 256 48).
+    // Few tiles: their keys are split, for at most two workgroups a CU.
     const size_t keys = (size_t)a.entries << a.kv.shift;
-    const size_t waves = std::min<size_t>(4, ((size_t)p.tokens * a.group / a.seqs + 31) / 32);
-    const size_t least = std::max<size_t>(waves, 1) * (act_type(kv_type)->bytes == 4 ? 16 : 128);
-    a.splits = (uint32_t)std::max<size_t>(1, std::min({2 * cus / tiles, keys / least, (size_t)64}));
+    a.splits = prompt_splits(tiles, keys, keys - std::min<size_t>(keys, p.tokens / a.seqs / 2),
+                             (size_t)p.tokens * a.group * a.kv.heads, cus, dp, act_type(kv_type)->bytes == 4);
     if (a.splits > 1) {
         const size_t rows = tiles * a.splits * 128;
         HH_TRY(grow(&ws_attn, &ws_attn_cap, rows * (dp + 2) * sizeof(float)));
         a.part = (float*)ws_attn;
         a.part_sum = a.part + rows * dp;
     }
+    // Between one and two workgroups a CU, all there at once: the second ones in ascending order.
+    const size_t blocks = tiles * a.splits;  // (2 cus at most where splits > 1)
+    const bool pairs = blocks > cus && blocks <= 2 * cus && resident_blocks(name, 256) == 2;
+    p.turn = pairs ? (uint32_t)(cus / a.kv.heads) : UINT32_MAX;
     void* params[] = {&p};
-    HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)tiles, a.splits, 1, 256, 1, 1, 0, stream, params, nullptr),
+    HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)blocks, 1, 1, 256, 1, 1, 0, stream, params, nullptr),
                "hipModuleLaunchKernel(attn_prompt)");
     size_t teams = 1;  // of dp / 4 threads a row
     while (teams < 1024 / dp && teams < a.splits) teams *= 2;

@@ -179,6 +179,17 @@ def test_many_sequences(engine, count):
     Problem(BF16, BF16, seqs, 64, 1, 64, 16, seed=7).check(engine)  # two tokens a tile
 
 
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+def test_as_many_tiles_as_can_be(engine, ty):
+    """Every sequence ends one row into a tile: of 64 the last slot is taken.  More workgroups than CUs and at most twice as
+    many, of one sequence and of many, some with parts; whole tiles only."""
+    for seqs, heads, kvh, dim in [([(17, 17)] * 64, 8, 1, 64), ([(33, 40), (1, 300)] * 32, 4, 1, 64), ([(17, 19)] * 65, 8, 1, 64),
+                                  ([(1100, 1100)], 32, 32, 80), ([(256, 256)], 16, 4, 128), ([(129, 200)] * 10, 16, 16, 96),
+                                  ([(300, 2000), (20, 4000)], 28, 14, 64), ([(512, 512)], 8, 2, 128)]:
+        print(f"[case] prompt {ty} {len(seqs)} of {seqs[0]} {heads} {kvh} {dim}", flush=True)
+        Problem(ty, ty, seqs, heads, kvh, dim, 32, seed=23).check(engine)
+
+
 def test_captured(engine):
     """A captured prompt follows what its lists and queries hold at each replay; split keys and whole ones."""
     for seqs, page in [([(9, 900), (30, 64), (1, 70)], 16), ([(60, 60), (70, 80)], 64)]:
