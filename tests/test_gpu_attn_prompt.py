@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from attn_reference import DT, attend, check, gather, page_elements
-from hayai_amd import BF16, F16, F32, HipError
+from hayai_amd import BF16, F16, F32, HipEngine, HipError
 from test_gpu_attn_decode import far_smaller
 from test_gpu_attn_pages import get, ints, normal, put
 
@@ -219,6 +219,24 @@ def test_captured(engine):
             call()
             assert torch.equal(eager, get(b["out"], torch.bfloat16, (p.tokens, wide)))
         graph.free()
+
+
+def test_captured_first_of_all():
+    """An engine's first call is captured, with more workgroups than CUs and at most twice as many."""
+    p = Problem(F16, F16, [(1100, 1100)], 32, 32, 64, 64, seed=31)
+    want, bound = p.want()
+    engine = HipEngine(0)
+    wide, kv = 32 * 64, engine.kv_desc(F16, 32, 64, 64, p.n_pages)
+    q, cache, out = put(engine, p.q), put(engine, p.cache), put(engine, torch.zeros(p.tokens, wide).half())
+    starts, lens, tables = ints(engine, p.starts.tolist()), ints(engine, p.lens.tolist()), ints(engine, p.tables.reshape(-1).tolist())
+    d = engine.attn_prompt_desc(F16, p.tokens, 1, 32, p.scale, p.width)
+    graph = engine.capture(lambda: engine.attn_prompt_dev(d, kv, q, 0, cache, 0, starts, 0, lens, 0, tables, 0, out, 0))
+    for _ in range(3):
+        out.write(torch.zeros(p.tokens, wide).half().view(torch.uint8).numpy())
+        graph.launch()
+        check(get(out, torch.float16, want.shape), want, bound, F16)
+    graph.free()
+    engine.close()
 
 
 def test_large_scores(engine):
