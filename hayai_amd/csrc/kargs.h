@@ -187,6 +187,7 @@ struct hh_attn_prompt_args {
     const int32_t* starts;  // seqs + 1
     uint32_t tokens, slots;
     uint32_t turn;  // tiles' parts from which on the shortest come first
+    uint32_t step, whole;  // log2 of the keys in a tile; as many as are taken in one part
 };
 
 // Attention of one token a sequence (attn_decode.hip): the first `prefix` tokens of all sequences from the

@@ -90,13 +90,25 @@ HH_DEV hh_attn_place hh_attn_place_of(const hh_attn_prompt_args& p, uint32_t blo
     return {block % p.a.kv.heads, p.a.seqs > 1 && p.a.seqs <= HH_WAVE ? tile : p.slots - 1 - tile, i % p.a.splits};
 }
 
+// In how many parts a tile takes its keys: what the host found best for a full table, but none without a tile of
+// keys, and one for few: it needs no join (us, with empty parts in brackets: 100 tokens in a table for 32000, 32/8 heads of
+// 128 bf16: 13.4 [22.0]; 300: 24.0 [28.5]; 30 behind 1000: 13.8 [14.8]; 1000 behind 1000 in their own: 56.4 [54.7]).
+HH_DEV uint32_t hh_attn_splits(const hh_attn_prompt_args& p, const hh_attn_tile& t) {
+    const int to = (int)min(t.first + p.a.tile_tokens, t.tokens);
+    const uint32_t keys = (uint32_t)max(0, min((int)t.len, (int)t.len - (int)t.tokens + to));
+    const uint32_t tiles = (keys + (1u << p.step) - 1) >> p.step;
+    return keys > p.whole ? min(p.a.splits, tiles) : 1;
+}
+
 template <class A, class C, int DP, int DU>
 HH_DEV void hh_attn_prompt(const hh_attn_prompt_args& p) {
     const hh_attn_place at = hh_attn_place_of(p, blockIdx.x, gridDim.x);
     hh_attn_tile tile;
     if (!hh_attn_find(p, at.slot, threadIdx.x % HH_WAVE, tile)) return;
+    const uint32_t splits = hh_attn_splits(p, tile);
+    if (at.split >= splits) return;
     hh_attn_rows<A, C, DP, DU, true>(p.a, tile, p.a.tables + (size_t)tile.seq * p.a.entries, p.a.entries, at.kvh,
-                                     at.slot * p.a.kv.heads + at.kvh, at.split, p.a.splits);
+                                     at.slot * p.a.kv.heads + at.kvh, at.split, splits);
 }
 
 // The parts of rows whose keys were split, joined.
@@ -106,14 +118,15 @@ HH_DEV void hh_attn_prompt_join(const hh_attn_prompt_args& p) {
     const uint32_t kvh = blockIdx.x % a.kv.heads, slot = blockIdx.x / a.kv.heads;
     hh_attn_tile tile;
     if (!hh_attn_find(p, slot, threadIdx.x % HH_WAVE, tile)) return;
-    const uint32_t rows = min(a.tile_tokens, tile.tokens - tile.first) * a.group;
+    const uint32_t rows = min(a.tile_tokens, tile.tokens - tile.first) * a.group, splits = hh_attn_splits(p, tile);
+    if (splits == 1) return;
     constexpr uint32_t N = 1024 / DP;
     uint32_t teams = 1;  // a row
     while (teams < N && teams < a.splits) teams *= 2;
     const uint32_t r = blockIdx.y * (N / teams) + threadIdx.x / (DP / 4) / teams, at = min(r, rows - 1);
     if (blockIdx.y * (N / teams) >= rows) return;
     const size_t row = ((size_t)slot * a.kv.heads + kvh) * a.splits * 128 + at;
-    const hh_attn_parts parts = {a.part + row * DP, a.part_sum + row * 2, a.splits, 128};
+    const hh_attn_parts parts = {a.part + row * DP, a.part_sum + row * 2, splits, 128};
     typename A::E* const out = (typename A::E*)a.out + (size_t)(tile.start + tile.first + at / a.group) * a.out_stride +
                                (kvh * a.group + at % a.group) * a.kv.dim;
     hh_attn_join_row<A, DP>(parts, hh_attn_parts{}, teams, r < rows && threadIdx.x % (DP / 4) * 4 < a.kv.dim, out);

@@ -25,8 +25,9 @@ constexpr int hh_attn_bytes() {
 }
 
 // DP: a head's elements, or those that they lie within; DU: 0 where the head has all of them, else how many are computed
-// (a head of 72 to 96 takes three quarters of 128's products).  CAUSAL: each earlier token sees a key less; else all of them see len, and the sums always go to `part`.  at: the tile's
-// number in `part`; split: which of its `splits` parts of keys.
+// (a head of 72 to 96 takes three quarters of 128's products).  CAUSAL: each earlier token sees a key less; else all of
+// them see len, and the sums always go to `part`.  at: the tile's number in `part`, where each has a.splits parts; split:
+// which of the `splits` parts that it takes.
 template <class A, class C, int DP, int DU, bool CAUSAL>
 HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const int32_t* table, uint32_t entries, uint32_t kvh,
                          uint32_t at, uint32_t split, uint32_t splits) {
@@ -232,7 +233,7 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
         }
     };
     if (!CAUSAL || splits > 1) {
-        const size_t part = (size_t)at * splits + split;
+        const size_t part = (size_t)at * a.splits + split;
         float* const po = a.part + (part * 128 + r) * DP;
 #pragma unroll
         for (int i = 0; i < DT; i++)

@@ -133,8 +133,11 @@ hh_status hh_engine::enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_a
     p.slots = (uint32_t)slots;
     // Few tiles: their keys are split, for at most two workgroups a CU.
     const size_t keys = (size_t)a.entries << a.kv.shift;
-    a.splits = prompt_splits(tiles, keys, keys - std::min<size_t>(keys, p.tokens / a.seqs / 2),
-                             (size_t)p.tokens * a.group * a.kv.heads, cus, dp, act_type(kv_type)->bytes == 4);
+    const size_t all_rows = (size_t)p.tokens * a.group * a.kv.heads;
+    const bool f32 = act_type(kv_type)->bytes == 4;
+    a.splits = prompt_splits(tiles, keys, keys - std::min<size_t>(keys, p.tokens / a.seqs / 2), all_rows, cus, dp, f32);
+    p.step = f32 ? 5 : 6;
+    p.whole = f32 ? 32 : 128;
     if (a.splits > 1) {
         const size_t rows = tiles * a.splits * 128;
         HH_TRY(grow(&ws_attn, &ws_attn_cap, rows * (dp + 2) * sizeof(float)));

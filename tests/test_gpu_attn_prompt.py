@@ -190,6 +190,21 @@ def test_as_many_tiles_as_can_be(engine, ty):
         Problem(ty, ty, seqs, heads, kvh, dim, 32, seed=23).check(engine)
 
 
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+def test_tables_with_room(engine, ty):
+    """Tables for many more tokens than there are: parts without keys, tiles of one part beside tiles of many, both sides
+    of where one is enough."""
+    for seqs, dim in [([(100, 100)], 128), ([(3, 120), (40, 300), (0, 0), (1, 1), (5, 3)], 64), ([(1, 128), (1, 129), (1, 32), (1, 33)], 64),
+                      ([(200, 200)], 80), ([(33, 1025), (64, 64)], 256)]:
+        print(f"[case] prompt {ty} {seqs} {dim}", flush=True)
+        p = Problem(ty, ty, seqs, 8, 2, dim, 64, seed=29, width=500)
+        first = p.check(engine)
+        p.seqs, p.lens[:] = [(n, min(length, n)) for n, length in p.seqs], np.minimum(p.lens, [n for n, _ in seqs])
+        p.check(engine)
+        p.seqs, p.lens[:] = seqs, [length for _, length in seqs]
+        assert torch.equal(first, p.run(engine))
+
+
 def test_captured(engine):
     """A captured prompt follows what its lists and queries hold at each replay; split keys and whole ones."""
     for seqs, page in [([(9, 900), (30, 64), (1, 70)], 16), ([(60, 60), (70, 80)], 64)]:
