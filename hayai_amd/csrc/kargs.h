@@ -190,7 +190,7 @@ struct hh_attn_prompt_args {
     uint32_t step, whole;  // log2 of the keys in a tile; as many as are taken in one part
 };
 
-// Attention of one token a sequence (attn_decode.hip): the first `prefix` tokens of all sequences from the
+// Attention of one token a sequence (attn_decode.hip): the first `prefix` tokens of the sequences of `sharing` or more from the
 // pages of `shared` (tiles of `a`), the others in pieces, each with row_tiles * heads * 16 rows of sums.
 struct hh_attn_decode_args {
     hh_attn_args a;
@@ -198,7 +198,7 @@ struct hh_attn_decode_args {
     float* piece;
     float* piece_sum;
     uint32_t* plan;  // each sequence's first piece and how many it has
-    uint32_t prefix, shared_entries, tiles, row_tiles;
+    uint32_t prefix, sharing, shared_entries, tiles, row_tiles;
     uint32_t room;           // units of own tokens that a table has room for
     uint32_t pieces, least;  // at most (but for one a sequence more); for a workgroup a CU
 };

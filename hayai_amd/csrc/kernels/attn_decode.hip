@@ -14,11 +14,11 @@
 #define HH_ATTN_UNIT 128u  // keys a piece is a multiple of
 #define HH_ATTN_MOST 64u   // pieces of a sequence
 
-// Tokens of sequence s that no other shares, and the first of them.  A sequence shorter than the prefix takes no
-// part in it.
+// Tokens of sequence s that are not taken with the shared ones, and the first of them.  A sequence shorter than the caller's
+// prefix has none of its tokens in those pages, also where it reaches the whole tiles of it that are taken apart.
 HH_DEV uint32_t hh_attn_own(const hh_attn_decode_args& p, uint32_t s, uint32_t& from) {
     const uint32_t len = (uint32_t)min((int64_t)max(0, p.a.lens[s]), (int64_t)p.a.entries << p.a.kv.shift);
-    from = len >= p.prefix ? p.prefix : 0;
+    from = len >= p.sharing ? p.prefix : 0;
     return len - from;
 }
 

@@ -170,6 +170,7 @@ hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_a
     // 23.1; 16 x 2048 of 32/8, 126 MB: 15.0, 29.1).
     const size_t token = 2 * heads * a.kv.dim * act_type(kv_type)->bytes;
     const bool apart = a.seqs > 1 && (double)(a.seqs - 1) * p.prefix * (double)token >= (double)attn_share_min;
+    p.sharing = p.prefix;
     p.prefix = apart ? p.prefix / 64 * 64 : 0;
     const std::string name = (p.prefix ? "hh_attn_shared_" : "hh_attn_decode_") + dim_name(a.kv.dim) + attn_types(type, kv_type);
     HH_TRY(kernel(name, &f));

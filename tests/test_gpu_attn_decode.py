@@ -320,3 +320,50 @@ def test_refusals(engine):
         with pytest.raises(HipError) as err:
             call(**changes)
         assert err.value.status == status, changes
+
+
+# prefix, heads, kv heads, dim, page: no multiples of 64, so that what is taken apart is less than what is shared; one under 64
+NEARLY = [(699, 4, 4, 64, 16), (690, 8, 2, 128, 64), (590, 8, 1, 128, 128), (265, 6, 2, 96, 256), (1281, 64, 1, 64, 64), (65, 9, 3, 72, 16),
+          (63, 4, 2, 64, 32)]
+
+
+def around(prefix):
+    """Lengths on both sides of the prefix and of the whole 64 tokens in it."""
+    whole = prefix // 64 * 64
+    return [prefix + 90, whole - 1, whole, whole + 1, (whole + prefix) // 2, prefix - 1, prefix, prefix + 1]
+
+
+@pytest.mark.parametrize("ty,cty", TYPES)
+def test_nearly_the_prefix(sharing, ty, cty):
+    """Sequences of a few tokens less than the prefix have tokens of their own, in their own tables alone."""
+    for i, (prefix, heads, kvh, dim, page) in enumerate(NEARLY):
+        print(f"[case] decode {ty} {cty} {NEARLY[i]}", flush=True)
+        b = Batch(ty, cty, around(prefix), prefix, heads, kvh, dim, page, seed=50 + i)
+        b.check(b.run(sharing))
+
+
+@pytest.mark.parametrize("ty,cty", TYPES)
+def test_nearly_the_prefix_by_many(engine, ty, cty):
+    """The same with as many bytes as are taken apart by default."""
+    lens = [700 + 3 * i for i in range(70)]
+    lens[1], lens[7], lens[30], lens[31], lens[69] = 640, 689, 641, 639, 665
+    b = Batch(ty, cty, lens, 690, 8, 4, 128, 64, seed=60)
+    b.check(b.run(engine))
+
+
+def test_nearly_the_prefix_captured(sharing):
+    """Lengths that pass the prefix in both directions from replay to replay."""
+    b = Batch(BF16, BF16, [900, 689, 689, 760, 689], 690, 8, 2, 128, 32, seed=61)
+    b.check(b.run(sharing))
+    graph = sharing.capture(lambda: b.call(sharing))
+    for step, lens in enumerate([[700, 640, 641, 690, 689], [640, 639, 689, 689, 300], [900, 0, 645, 650, 688], [690, 689, 640, 760, 1]]):
+        b.lens[:] = lens
+        b.q = normal(step + 62, *b.q.shape).to(torch.bfloat16)
+        b.buffers["lens"].write(b.lens.astype(np.int32))
+        b.buffers["q"].write(b.q.view(torch.uint8).numpy())
+        graph.launch()
+        got = b.read()
+        b.check(got)
+        b.call(sharing)
+        assert torch.equal(got, b.read())
+    graph.free()
