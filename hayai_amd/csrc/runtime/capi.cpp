@@ -945,6 +945,16 @@ hh_status hh_sample_dev(hh_engine* e, const hh_sample_desc* d, const hh_buf* log
 
 // ---------------------------------------------------------------- attention ----------
 
+// Whether pages of two of `layers` caches have an element in common: page p of layer l begins at p * stride + l * layer_stride.
+static bool layers_meet(size_t stride, size_t page, size_t n_pages, size_t layer_stride, size_t layers) {
+    for (size_t l = 1; l < layers; l++) {  // layer l and the first one: every other pair lies like one of these
+        const size_t p = l * layer_stride / stride, past = l * layer_stride % stride;
+        if (p >= n_pages) return false;
+        if (past < page || (p + 1 < n_pages && stride - past < page)) return true;
+    }
+    return false;
+}
+
 // The cache's pages in a device-visible buffer of the engine, `layers` caches *layer_stride elements apart.
 static hh_status check_kv(hh_engine* e, const hh_kv_desc* kv, const hh_buf* cache, size_t off, size_t layers,
                           size_t* layer_stride, hh_kv_args* out, const char* what) {
@@ -968,6 +978,9 @@ static hh_status check_kv(hh_engine* e, const hh_kv_desc* kv, const hh_buf* cach
     const size_t last = ((kv->n_pages - 1) * stride + page) * el;
     if (layers > 1 && *layer_stride > (SIZE_MAX - last) / el / (layers - 1))
         return fail(HH_ERR_INVALID, "%s: size overflow", what);
+    if (layers_meet(stride, page, kv->n_pages, *layer_stride, layers))
+        return fail(HH_ERR_INVALID, "%s: pages of %zu layers %zu elements apart overlap (page_stride %zu)", what, layers, *layer_stride,
+                    stride);
     HH_TRY(check_range(cache, off, (layers - 1) * *layer_stride * el + last, what));
     if ((((uintptr_t)cache->ptr + off) | stride * el | (layers > 1 ? *layer_stride * el : 0)) % 16)
         return fail(HH_ERR_INVALID, "%s: pages must start on 16-byte boundaries (strides %zu, %zu)", what, stride,

@@ -573,8 +573,9 @@ hh_status hh_rope_factors(int scaling, size_t rot_dim, double base, double scale
                           float* mscale);
 
 /* Pages copied in `layers` caches, `layer_stride` elements apart (a multiple of 16 bytes; 0: n_pages *
- * page_stride): moves is int32[n][2], (from, to), taken as if one after another.  A move with a page outside [0, n_pages) does
- * nothing, so lists may be padded with -1. */
+ * page_stride; one layer's pages may lie between another's, but layers that overlap are HH_ERR_INVALID): moves is
+ * int32[n][2], (from, to), taken as if one after another.  A move with a page outside [0, n_pages) does nothing, so
+ * lists may be padded with -1. */
 hh_status hh_kv_copy_dev(hh_engine* e, const hh_kv_desc* kv, size_t layers, size_t layer_stride, hh_buf* cache,
                          size_t cache_off, const hh_buf* moves, size_t moves_off, size_t n);
 

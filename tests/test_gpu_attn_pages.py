@@ -294,3 +294,38 @@ def test_refusals(engine):
         with pytest.raises(hayai_amd.HipError) as err:
             engine.kv_copy_dev(*args, **kw)
         assert err.value.status == 2, (args[2:], kw)
+
+
+def test_kv_copy_layers_that_overlap(engine):
+    """Layers whose pages have bytes in common are refused: their copies have no order.  Layers apart, one page's next to each other,
+    and others in the gaps between pages go through."""
+    kvh, dim, page = 1, 8, 16
+    per = 2 * kvh * dim * page
+    size = 1 << 20
+    b, moves = engine.alloc(size), engine.upload(np.array([(0, 1)], np.int32))
+
+    def elements(n, stride, layer_stride, layers):
+        return [set(range(p * stride + l * layer_stride, p * stride + l * layer_stride + per)) for l in range(layers) for p in range(n)]
+
+    refused = 0
+    for n, stride, layer_stride, layers in [
+            (2, per, 8, 2), (2, per, per, 2), (2, 3 * per, 2 * per + 8, 2), (2, 3 * per, per - 8, 3), (3, 2 * per, 2 * per, 2),
+            (2, 2 * per, per, 3), (4, 2 * per, 3 * per - 8, 3), (1, per, per - 8, 5), (3, 5 * per, 4 * per, 4), (3, 2 * per, 6 * per - 8, 2),
+            (2, per, 2 * per, 3), (2, 3 * per, per, 3), (3, 10 * per, 11 * per, 4), (1, per, per, 9), (3, 2 * per, 5 * per, 2),
+            (3, 2 * per + 8, per + 8, 2), (4, 2 * per, 9 * per, 3), (3, 4 * per, 14 * per, 4)]:
+        kv = engine.kv_desc(F16, kvh, dim, page, n, stride)
+        parts = elements(n, stride, layer_stride, layers)
+        if len(set().union(*parts)) < sum(len(p) for p in parts):
+            with pytest.raises(hayai_amd.HipError) as err:
+                engine.kv_copy_dev(kv, b, 0, moves, 0, 1, layers=layers, layer_stride=layer_stride)
+            assert err.value.status == 2, (n, stride, layer_stride, layers)
+            refused += 1
+            continue
+        cache = np.random.default_rng(0).integers(0, 1 << 16, size // 2, dtype=np.uint16)
+        b.write(cache)
+        engine.kv_copy_dev(kv, b, 0, moves, 0, 1 if n > 1 else 0, layers=layers, layer_stride=layer_stride)
+        if n > 1:
+            for l in range(layers):
+                cache[l * layer_stride + stride:][:per] = cache[l * layer_stride:][:per]
+        assert np.array_equal(b.read(np.uint16, size // 2), cache), (n, stride, layer_stride, layers)
+    assert refused == 8
