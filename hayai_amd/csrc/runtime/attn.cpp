@@ -176,8 +176,8 @@ hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_a
     HH_TRY(kernel(name, &f));
     HH_TRY(kernel("hh_attn_join_" + std::to_string(dp) + "_" + act_type(type)->name, &join));
     size_t ahead = 0, part_rows = 0;
+    a.tile_tokens = 128 / a.group;  // (the join divides by it also where no tokens are taken apart)
     if (p.prefix) {
-        a.tile_tokens = 128 / a.group;
         p.tiles = (a.seqs + a.tile_tokens - 1) / a.tile_tokens;
         // parts for half the CUs, more where not all four waves have rows (2 sequences of 8192, 32/8 heads of 128 bf16: 32 parts
         // 15.8 us, 16 parts 18.9; 64: 8 parts 49, 16 parts 54)
