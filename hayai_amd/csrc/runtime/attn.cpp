@@ -146,7 +146,7 @@ hh_status hh_engine::enqueue_attn_prompt(int type, int kv_type, hh_attn_prompt_a
     }
     // Between one and two workgroups a CU, all there at once: the second ones in ascending order.
     const size_t blocks = tiles * a.splits;  // (2 cus at most where splits > 1)
-    const bool pairs = blocks > cus && blocks <= 2 * cus && resident_blocks(name, 256) >= 2;
+    const bool pairs = blocks > cus && blocks <= 2 * cus && occupancy(name, 256) >= 2;
     p.turn = pairs ? (uint32_t)(cus / a.kv.heads) : UINT32_MAX;
     void* params[] = {&p};
     HH_TRY_HIP(hipModuleLaunchKernel(f, (uint32_t)blocks, 1, 1, 256, 1, 1, 0, stream, params, nullptr),

@@ -123,7 +123,10 @@ hh_status hh_engine::kernel(const std::string& name, hipFunction_t* out) {
 }
 
 int hh_engine::resident_blocks(const std::string& name, int block) {
-    if (blocks_per_cu_override > 0) return blocks_per_cu_override;
+    return blocks_per_cu_override > 0 ? blocks_per_cu_override : occupancy(name, block);
+}
+
+int hh_engine::occupancy(const std::string& name, int block) {
     auto it = blocks_per_cu.find(name);
     if (it != blocks_per_cu.end()) return it->second;
     hipFunction_t f;

@@ -226,7 +226,8 @@ struct hh_engine {
     std::string noalloc_error;
     hh_status enqueue_ffn_noalloc(const hh_ffn_desc* d, const uint8_t* pack, const float* x, float* y);
     hh_status kernel(const std::string& name, hipFunction_t* out);
-    int resident_blocks(const std::string& name, int block);
+    int resident_blocks(const std::string& name, int block);  // HAYAI_HIP_BLOCKS_PER_CU, else occupancy()
+    int occupancy(const std::string& name, int block);         // workgroups of a kernel that a CU holds
     template <class A>
     hh_status launch(hipFunction_t f, uint32_t grid, uint32_t block, const A& args) {
         void* params[] = {const_cast<A*>(&args)};
