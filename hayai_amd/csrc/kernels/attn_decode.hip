@@ -231,7 +231,7 @@ HH_DEV void hh_attn_single(const hh_attn_decode_args& p, uint32_t block) {
             v += red[(w * 16 + r) * (D / 4) + (c ^ r % 8)];
         }
         if (alone) {
-            const float by = total == 0 ? 0.f : 1.f / total;
+            const float by = own ? 1.f / total : 0.f;  // (weights of 0 alone: 0 * inf, NaN)
             E e[4];
 #pragma unroll
             for (int x = 0; x < 4; x++) e[x] = A::put(v[x] * by);
@@ -268,14 +268,14 @@ HH_DEV void hh_attn_join(const hh_attn_decode_args& p) {
     const uint32_t kvh = head / a.group, r = head % a.group;
     const uint32_t first = p.plan[2 * s], count = p.plan[2 * s + 1];
     uint32_t from;
-    hh_attn_own(p, s, from);
+    const uint32_t own = hh_attn_own(p, s, from);
     const uint32_t splits = p.prefix && from ? a.splits : 0;
     if (splits == 0 && count == 1) return;
     const size_t row0 = ((size_t)(s / a.tile_tokens) * a.kv.heads + kvh) * a.splits * 128 + s % a.tile_tokens * a.group + r;
     const size_t row1 = (((size_t)first * p.row_tiles + r / 16) * a.kv.heads + kvh) * 16 + r % 16;
     hh_attn_join_row<A, DP>(hh_attn_parts{a.part + row0 * DP, a.part_sum + row0 * 2, splits, 128},
                             hh_attn_parts{p.piece + row1 * DP, p.piece_sum + row1 * 2, count, (size_t)p.row_tiles * a.kv.heads * 16},
-                            1024 / DP, threadIdx.x % (DP / 4) * 4 < a.kv.dim,
+                            1024 / DP, from + own != 0, threadIdx.x % (DP / 4) * 4 < a.kv.dim,
                             (typename A::E*)a.out + (size_t)s * a.out_stride + head * a.kv.dim);
 }
 

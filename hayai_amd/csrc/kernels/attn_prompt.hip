@@ -94,8 +94,8 @@ HH_DEV hh_attn_place hh_attn_place_of(const hh_attn_prompt_args& p, uint32_t blo
 // keys, and one for few: it needs no join (us, with empty parts in brackets: 100 tokens in a table for 32000, 32/8 heads of
 // 128 bf16: 13.4 [22.0]; 300: 24.0 [28.5]; 30 behind 1000: 13.8 [14.8]; 1000 behind 1000 in their own: 56.4 [54.7]).
 HH_DEV uint32_t hh_attn_splits(const hh_attn_prompt_args& p, const hh_attn_tile& t) {
-    const int to = (int)min(t.first + p.a.tile_tokens, t.tokens);
-    const uint32_t keys = (uint32_t)max(0, min((int)t.len, (int)t.len - (int)t.tokens + to));
+    const uint32_t to = min(t.first + p.a.tile_tokens, t.tokens);
+    const uint32_t keys = hh_attn_seen(t, to - 1);
     const uint32_t tiles = (keys + (1u << p.step) - 1) >> p.step;
     return keys > p.whole ? min(p.a.splits, tiles) : 1;
 }
@@ -129,7 +129,8 @@ HH_DEV void hh_attn_prompt_join(const hh_attn_prompt_args& p) {
     const hh_attn_parts parts = {a.part + row * DP, a.part_sum + row * 2, splits, 128};
     typename A::E* const out = (typename A::E*)a.out + (size_t)(tile.start + tile.first + at / a.group) * a.out_stride +
                                (kvh * a.group + at % a.group) * a.kv.dim;
-    hh_attn_join_row<A, DP>(parts, hh_attn_parts{}, teams, r < rows && threadIdx.x % (DP / 4) * 4 < a.kv.dim, out);
+    hh_attn_join_row<A, DP>(parts, hh_attn_parts{}, teams, hh_attn_seen(tile, tile.first + at / a.group) != 0,
+                            r < rows && threadIdx.x % (DP / 4) * 4 < a.kv.dim, out);
 }
 
 #define HH_ATTN_PROMPT(N, A, C, D, DU, NAME)                                                                                    \

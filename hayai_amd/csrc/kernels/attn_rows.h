@@ -18,6 +18,11 @@ struct hh_attn_tile {
     uint32_t seq, start, first, tokens, len;
 };
 
+// Keys that the run's token t sees where each earlier token sees a key less.
+HH_DEV uint32_t hh_attn_seen(const hh_attn_tile& tile, uint32_t t) {
+    return (uint32_t)max(0, min((int)tile.len, (int)tile.len - (int)tile.tokens + (int)t + 1));
+}
+
 // Bytes of a tile of keys and values in LDS.
 template <class C, int DP, int DU>
 constexpr int hh_attn_bytes() {
@@ -49,10 +54,7 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
     const uint32_t rows = min(a.tile_tokens, tile.tokens - tile.first) * group;
     const uint32_t r = wave * 32 + ln, tok = tile.first + min(r, rows - 1) / group, head = kvh * group + min(r, rows - 1) % group;
     // keys that the lane's row sees, and the tile's first and last row
-    auto seen = [&](uint32_t t) {
-        if (!CAUSAL) return tile.len;
-        return (uint32_t)max(0, min((int)tile.len, (int)tile.len - (int)tile.tokens + (int)t + 1));
-    };
+    auto seen = [&](uint32_t t) { return CAUSAL ? hh_attn_seen(tile, t) : tile.len; };
     const uint32_t limit = seen(tok), least = seen(tile.first), most = seen(tile.first + (rows - 1) / group);
     const uint32_t tiles = (most + BN - 1) / BN;
     const uint32_t t0 = (uint32_t)((uint64_t)tiles * split / splits);
@@ -247,7 +249,7 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
         }
         return;
     }
-    const float by = sum == 0 ? 0.f : 1.f / sum;
+    const float by = 1.f / sum;  // (weights of 0 alone: 0 * inf, NaN)
     E* const out = (E*)a.out + (size_t)(tile.start + tok) * a.out_stride + head * dim;
 #pragma unroll
     for (int i = 0; i < DT; i++)
@@ -255,7 +257,7 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
         for (int j = 0; j < 4; j += 2) {
             E v[2][4];
 #pragma unroll
-            for (int x = 0; x < 8; x++) v[x / 4][x % 4] = A::put(sum == 0 ? 0.f : o[i][4 * j + x] * by);
+            for (int x = 0; x < 8; x++) v[x / 4][x % 4] = A::put(limit == 0 ? 0.f : o[i][4 * j + x] * by);
             if (sizeof(E) == 4) {
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
@@ -285,15 +287,15 @@ HH_DEV void hh_attn_rows(const hh_attn_args& a, const hh_attn_tile& tile, const 
 
 // Two runs of a row's parts, joined: sum_i f_i o_i / sum_i f_i s_i, f_i = exp2(base_i - max base), by `teams` (a power of
 // two) of the workgroup's teams of DP / 4 threads, which hold 4 elements each and take every teams-th part; all threads
-// call it, and the first team's store the row.  A part that saw no key has sum 0 and is left out (its o may hold
-// 0 * NaN).
+// call it, and the first team's store the row.  A part that saw no key, or none with a weight, has sum 0 and is left out (its o
+// may hold 0 * NaN).  any_key: the row saw one; if none had a weight it is 0 / 0, NaN, as it would be in one part.
 struct hh_attn_parts {
     const float *o, *s;  // the first part's elements, base and sum
     uint32_t n;
     size_t step;  // rows from a part to the next
 };
 template <class A, int DP>
-HH_DEV void hh_attn_join_row(const hh_attn_parts& x, const hh_attn_parts& y, uint32_t teams, bool store, typename A::E* out) {
+HH_DEV void hh_attn_join_row(const hh_attn_parts& x, const hh_attn_parts& y, uint32_t teams, bool any_key, bool store, typename A::E* out) {
     typedef typename A::E E;
     constexpr uint32_t L = DP / 4, N = 256 / L;
     const uint32_t team = threadIdx.x / L, d = threadIdx.x % L * 4;
@@ -331,7 +333,7 @@ HH_DEV void hh_attn_join_row(const hh_attn_parts& x, const hh_attn_parts& y, uin
 #pragma unroll
         for (int e = 0; e < 4; e++) o[e] = fmaf(red[i * L + threadIdx.x][e], f, o[e]);
     }
-    const float by = sum == 0 ? 0.f : 1.f / sum;
+    const float by = any_key ? 1.f / sum : 0.f;
     E v[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] = A::put(o[e] * by);

@@ -585,7 +585,7 @@ hh_status hh_kv_copy_dev(hh_engine* e, const hh_kv_desc* kv, size_t layers, size
  * tables (int32[seqs][table_stride]).  The i-th of its n rows sees the first lens[s] - n + i + 1 tokens: a whole
  * prompt has lens[s] = n, the next part of a longer one has more.  For each query head h (kv head h / (q_heads /
  * kv_heads)):  out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j).
- * A row that sees no token gets zeros.  Rows of no sequence stay as they were.  Lengths are taken to what the
+ * A row that sees no token gets zeros, one whose keys all score minus infinity 0 / 0, NaN.  Rows of no sequence stay as they were.  Lengths are taken to what the
  * table has room for; an entry that is read and outside [0, n_pages) stands for a page of zeros.  What lies
  * past a sequence's length, or past what a row sees, has no influence, NaN and infinities included.
  * Scores, weights' sums and outputs are summed in f32; over a 16-bit cache the products' operands are of the

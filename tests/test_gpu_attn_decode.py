@@ -367,3 +367,29 @@ def test_nearly_the_prefix_captured(sharing):
         b.call(sharing)
         assert torch.equal(got, b.read())
     graph.free()
+
+
+@pytest.mark.parametrize("ty,cty", TYPES)
+def test_scores_of_minus_infinity(sharing, ty, cty):
+    """The first `low` keys of each sequence score minus infinity: weights of 0 where another key is seen, else NaN (0 / 0)."""
+    for i, (lens, low, prefix, heads, kvh, dim, page) in enumerate([
+            ([50, 50, 1, 0], [20, 50, 1, 0], 0, 4, 2, 64, 16), ([3000, 3000, 200], [2500, 3000, 190], 0, 8, 2, 128, 64),
+            ([700, 750, 640], [660, 750, 640], 640, 8, 2, 128, 32), ([40, 300], [40, 131], 0, 3, 1, 72, 32)]):
+        b = Batch(ty, cty, lens, prefix, heads, kvh, dim, page, seed=70 + i)
+        b.q[:, ::dim] = b.q[:, ::dim].abs() + 0.5
+        keys = b.cache[:, :kvh * page * dim].view(-1, kvh, page, dim)
+        finite = keys.clone()
+        for s, n in enumerate(low):
+            for t in range(n):
+                keys[b.tables[s, t // page], :, t % page, 0] = -float("inf")
+        for t in range(min(low) if prefix else 0, prefix):  # (shared pages: what one sequence changes holds for all)
+            assert keys[b.shared[t // page], 0, t % page, 0] == -float("inf")
+        got = b.run(sharing)[:, :heads * dim].reshape(-1, heads, dim)
+        q = b.q.double().numpy().reshape(-1, heads, dim)
+        for s, n in enumerate(lens):
+            if n and low[s] == n:
+                assert torch.all(torch.isnan(got[s])), (i, s)
+                continue
+            k, v = gather(torch.cat([finite.flatten(1), b.cache[:, kvh * page * dim:]], 1), b.tables[s], n, kvh, dim, page)
+            want, bound = attend(q[s:s + 1], k[low[s]:], v[low[s]:], [n - low[s]], b.scale, ty, cty)
+            check(got[s:s + 1], want, bound, ty)

@@ -321,3 +321,30 @@ def test_refusals(engine):
         assert err.value.status == status, changes
     with pytest.raises(HipError):
         engine.attn_prompt_dev(engine.attn_prompt_desc(**good), kv, b, 0, b, 8, b, 0, b, 0, b, 0, b, 0)
+
+
+@pytest.mark.parametrize("ty,cty", TYPES)
+def test_scores_of_minus_infinity(engine, ty, cty):
+    """The first `low` keys score minus infinity: weights of 0 in rows that see another key, NaN (0 / 0) in rows that see these
+    alone, zeros in rows that see none."""
+    for i, (seqs, low, heads, kvh, dim, page) in enumerate([([(40, 40)], [20], 4, 2, 64, 16), ([(3, 2500), (5, 3)], [2498, 3], 8, 2, 128, 64),
+                                                            ([(200, 1200)], [1000 + 64], 8, 1, 128, 32), ([(30, 30), (3, 90)], [30, 0], 3, 1, 72, 32),
+                                                            ([(60, 40)], [33], 1, 1, 64, 64)]):
+        p = Problem(ty, cty, seqs, heads, kvh, dim, page, seed=40 + i)
+        p.q[:, ::dim] = p.q[:, ::dim].abs() + 0.5
+        finite = p.cache.clone()
+        keys = p.cache[:, :kvh * page * dim].view(-1, kvh, page, dim)
+        for s, n in enumerate(low):
+            for t in range(n):
+                keys[p.tables[s, t // page], :, t % page, 0] = -float("inf")
+        got = p.run(engine)[:p.tokens].reshape(-1, heads, dim)
+        q = p.q.double().numpy().reshape(-1, heads, dim)
+        for s, (n, length) in enumerate(seqs):
+            rows, seen = slice(p.starts[s], p.starts[s] + n), length - n + 1 + np.arange(n)
+            k, v = gather(finite, p.tables[s], length, kvh, dim, page)
+            want, bound = attend(q[rows], k[low[s]:], v[low[s]:], seen - low[s], p.scale, ty, cty)
+            blind, lost = seen <= 0, (seen > 0) & (seen <= low[s])
+            assert torch.all(got[rows][blind] == 0), (i, s)
+            assert torch.all(torch.isnan(got[rows][lost])), (i, s)
+            rest = ~blind & ~lost
+            check(got[rows][rest], want[rest], bound[rest], ty)
