@@ -1,5 +1,5 @@
-// Activation element types of the 8-bit operators (i8_rows.hip, i8_gemm.hip, sample.hip): f32, f16
-// or bf16 in memory, f32 in registers.  Vectors are 16 bytes and need only their elements'
+// Activation element types of the 8-bit operators (i8_rows.hip, i8_gemm.hip, sample.hip) and of attention, its cache's
+// too: f32, f16 or bf16 in memory, f32 in registers.  Vectors are 16 bytes and need only their elements'
 // alignment (gfx950 loads and stores unaligned dwords whole), so rows of any stride take them.
 #ifndef HH_KERNELS_ACT_TYPES_H
 #define HH_KERNELS_ACT_TYPES_H

@@ -8,7 +8,8 @@
 // step of 32 keys (16 of f32), joined through LDS at the end.  Lengths are known on the device alone, so every workgroup sums them up
 // and finds the piece of work that falls to it: pieces are of equal length whatever the sequences' are.  A second kernel joins the parts of a row.
 //
-// Weights are rounded to the cache's type for the second product; sums and the parts are f32.
+// Weights are rounded to the cache's type for the second product (by up to 2^-8 of each for bf16, 2^-11 for f16); sums and
+// the parts are f32.
 #include "attn_rows.h"
 
 #define HH_ATTN_UNIT 128u  // keys a piece is a multiple of

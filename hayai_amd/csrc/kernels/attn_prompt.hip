@@ -5,8 +5,8 @@
 // through the keys in tiles that all of them read from LDS; the next tile is copied there meanwhile.  Weights go
 // from the first product's result to the second's operand inside a lane (attn_tiles.h).
 //
-// Weights are rounded to the cache's type for the second product (2^-9 of each for bf16, 2^-12 for f16;
-// f32 keeps them); sums of weights and outputs are f32.
+// Weights are rounded to the cache's type for the second product (by up to 2^-8 of each for bf16, 2^-11 for f16;
+// f32 keeps them): the matrix cores take both operands in one type.  Sums of weights and outputs are f32.
 //
 // Tiles in which some row sees fewer keys than another are masked by comparison.  There values that are no
 // finite numbers are left out of the product (0 * inf would be NaN in rows that do not see the key) and

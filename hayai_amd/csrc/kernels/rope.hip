@@ -7,9 +7,9 @@
 // is kept: in 32 bits a position of 100000 would leave 2^-7 of a radian.  cos and sin are rounded to
 // f32 once, products and sums are f32, each output is rounded once.
 //
-// Bound by launch latency for few tokens (9 + 6 heads of 64 f32, one token: 3.1 us), by memory for a prompt (2048
-// tokens, 32/4 heads of 128 f16: 12.7 us, 3.3 TB/s; a token a workgroup 15.9).  A workgroup takes a token, or eight neighbouring ones of a prompt; its threads
-// ask for their first 16 bytes of either half of a head, make the tokens' cosines and sines (64-bit functions,
+// Bound by launch latency for few tokens (9 + 6 heads of 64 f32, one token: the kernel 3.5 us), by memory for a prompt (2048
+// tokens, 32/4 heads of 128 f16: 11.8 us a call among others, 3.5 TB/s; a token a workgroup 15.2).  A workgroup takes a token, or
+// eight neighbouring ones of a prompt; its threads ask for their first 16 bytes of either half of a head, make the tokens' cosines and sines (64-bit functions,
 // once for all heads), then turn.  Both of a pair are read and written by one thread, so q may be turned in
 // place.  Values go to [dim][tokens]: eight tokens in neighbouring slots as 16 bytes, others an element at a time.
 #include "kv_pages.h"

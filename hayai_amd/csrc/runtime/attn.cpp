@@ -188,7 +188,7 @@ hh_status hh_engine::enqueue_attn_decode(int type, int kv_type, hh_attn_decode_a
     }
     // The sequences' own tokens: the kernel makes pieces by the lengths (hh_attn_plan).  Each workgroup that is not
     // needed costs its look at the lengths, so that their number follows what the tables have room for: eight a CU for
-    // long ones (64 sequences of 2000: 106 us, four 114), else four (64 of 8192 + 500: 46, eight 49).
+    // long ones (64 sequences of 2000: 109 us, four 117), else four, in half the room (64 of 8192 + 500: 50 us either way).
     p.row_tiles = (a.group + 15) / 16;
     const size_t keys = (size_t)a.entries << a.kv.shift, room = ((keys > p.prefix ? keys - p.prefix : 0) + 127) / 128;
     const size_t least = std::max<size_t>(1, cus / (heads * p.row_tiles));

@@ -588,8 +588,10 @@ hh_status hh_kv_copy_dev(hh_engine* e, const hh_kv_desc* kv, size_t layers, size
  * A row that sees no token gets zeros, one whose keys all score minus infinity 0 / 0, NaN.  Rows of no sequence stay as they were.  Lengths are taken to what the
  * table has room for; an entry that is read and outside [0, n_pages) stands for a page of zeros.  What lies
  * past a sequence's length, or past what a row sees, has no influence, NaN and infinities included.
- * Scores, weights' sums and outputs are summed in f32; over a 16-bit cache the products' operands are of the
- * cache's type: weights are rounded to it, and f32 queries too. */
+ * Scores, weights' sums and outputs are summed in f32, with weights of up to 2^8 for the largest score (2^15 over an f16
+ * cache); values that n tokens sum to more than f32 holds at that, from about 2^119 / n on, give infinities.  Over a
+ * 16-bit cache the products' operands are of the cache's type: weights are rounded to it, and f32 queries too (over f16
+ * those past 65504 to infinity). */
 typedef struct hh_attn_prompt_desc {
     int type;            /* of q and out */
     float scale;         /* > 0, finite: 1 / sqrt(head_dim) as a rule */
@@ -607,7 +609,7 @@ hh_status hh_attn_prompt_dev(hh_engine* e, const hh_attn_prompt_desc* d, const h
  * cached tokens (tables as above; none: zeros, as for the padding of a batch).
  * prefix: the sequences' first `prefix` tokens are the same, and prefix_pages (int32[prefix / page_size, rounded up])
  * names pages that hold them: row 0 of tables, say.  They are read once for all sequences.  A sequence of
- * fewer tokens reads its own table alone.  prefix 0 (prefix_pages unused, may be NULL): none are shared.  What the
+ * fewer tokens reads its own table alone, where its tokens may be others.  prefix 0 (prefix_pages unused, may be NULL): none are shared.  What the
  * tables' rows name for these tokens has to be the same keys and values, in the same pages or in copies. */
 typedef struct hh_attn_decode_desc {
     int type;            /* of q and out */
